@@ -361,6 +361,75 @@ int pm_k_predictor_mlp(const void* x, int B, int H, const void* w1, const float*
  * ascending id (rank_experts, src/cpp_worker/predictor.hpp:24-28, ranks the same way on the host). */
 int pm_k_rank_topn(const float* scores, int width, int n, int32_t* out, void* stream);
 
+/* ---- operators around the experts (no counterpart in the reference, which leaves them to transformers) ----
+ * Stateless, no scratch memory, safe to capture into a CUDA graph and to call from several threads and streams at
+ * once. Pitches (ld_*) are in elements and at least the row length; the last dimension is dense. */
+#define PM_F32 0
+#define PM_BF16 1
+#define PM_F16 2
+
+/* Router on given logits [n_tokens, num_expert] (PM_F32 / PM_BF16 / PM_F16): topk_ids, topk_w [n_tokens, top_k].
+ *   score   softmax(l)_e, or 1 / (1 + exp(-l_e))
+ *   choice  score + choice_bias[e]; an expert whose logit or choice is -inf cannot be chosen
+ *   groups  of num_expert / n_group neighbouring experts, valued by their largest choice or by the sum of their two
+ *           largest (a missing second counts as nothing); the topk_group best stay, ties to the lower group
+ *   ids     the top_k largest choices among them, descending, ties to the lower id; -1 where there are fewer
+ *   weight  the score (not the choice), with norm_topk divided by the sum of the selected ones + 1e-20, times routed_scale;
+ *           0 for id -1
+ * A row that holds a NaN (softmax: or +inf) gets ids -1 and weights NaN. Selection is that of exact arithmetic on the given
+ * logits: where two float32 choices are too close to tell apart, the row is decided in 64 bits.
+ * num_expert at most 1024, top_k at most 32, n_group at most 32 and a divisor of num_expert, and topk_group groups
+ * must hold top_k experts. */
+#define PM_SCORE_SOFTMAX 0
+#define PM_SCORE_SIGMOID 1
+#define PM_GROUP_MAX 0
+#define PM_GROUP_TOP2 1
+typedef struct pm_router {
+  int32_t num_expert, top_k;
+  int32_t scoring;          /* PM_SCORE_* */
+  int32_t n_group;          /* 1 = no groups */
+  int32_t topk_group;       /* groups that stay */
+  int32_t group_score;      /* PM_GROUP_* */
+  int32_t norm_topk;
+  float routed_scale;
+  const float* choice_bias; /* device f32 [num_expert] or NULL */
+} pm_router;
+int pm_k_route(const pm_router* router, const void* logits, int dtype, int64_t ld_logits, int n_tokens, int32_t* topk_ids,
+               float* topk_w, void* stream);
+
+/* y = act(x w^T + bias) + residual. x [M, K] and w [N, K] are of `dtype` (PM_BF16 or PM_F16), y and the optional residual
+ * [M, N] of `out_dtype` (PM_F32 or dtype), the optional bias [N] of bias_dtype (PM_F32 or dtype). Sums are float32, y is
+ * rounded once. y may be the residual itself (same address and pitch); it must not overlap the other inputs. x and w whose rows
+ * start on 16-byte boundaries (address and pitch) go to the tcgen05 kernel, others to a slower one. The optional
+ * err_flag (device int32) receives 1 if a bounded wait of the kernel gave up; the outputs concerned are then NaN. */
+#define PM_ACT_NONE 0
+#define PM_ACT_RELU 1
+#define PM_ACT_SILU 2
+#define PM_ACT_GELU 3      /* v/2 (1 + erf(v / sqrt 2)) */
+#define PM_ACT_GELU_TANH 4 /* v/2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+typedef struct pm_linear {
+  const void* x;
+  const void* w;
+  const void* bias;     /* or NULL */
+  const void* residual; /* or NULL */
+  void* y;
+  int64_t ld_x, ld_w, ld_residual, ld_y;
+  int32_t M, N, K;
+  int32_t dtype, out_dtype, bias_dtype, act;
+  int32_t* err_flag; /* or NULL */
+} pm_linear;
+int pm_k_linear(const pm_linear* a, void* stream);
+
+/* Per row of logits [n_rows, vocab] (PM_F32 / PM_BF16 / PM_F16), with p = softmax(row):
+ *   logp[r]     = ln p[targets[r]]; 0 for a negative target (no token), NaN for one >= vocab
+ *   entropy[r]  = -sum p ln p
+ *   top_ids, top_logp [n_rows, top_n] = the top_n largest, descending, ties to the lower id; logits of -inf are no alternatives,
+ *                 id -1 and -inf where fewer are left
+ * A row that holds NaN or +inf, or nothing but -inf, is no distribution: NaN and ids -1. logp (with targets) and entropy
+ * may be NULL; top_n at most 32, 0 for none. */
+int pm_k_token_logprobs(const void* logits, int dtype, int64_t ld_logits, int n_rows, int vocab, const int64_t* targets, int top_n,
+                        float* logp, float* entropy, int32_t* top_ids, float* top_logp, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -52,6 +52,19 @@ class pm_ffn_group(C.Structure):
                 ("ld_down", C.c_int32)]
 
 
+class pm_router(C.Structure):
+    _fields_ = [("num_expert", C.c_int32), ("top_k", C.c_int32), ("scoring", C.c_int32), ("n_group", C.c_int32),
+                ("topk_group", C.c_int32), ("group_score", C.c_int32), ("norm_topk", C.c_int32),
+                ("routed_scale", C.c_float), ("choice_bias", C.c_void_p)]
+
+
+class pm_linear(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+                ("ld_x", C.c_int64), ("ld_w", C.c_int64), ("ld_residual", C.c_int64), ("ld_y", C.c_int64),
+                ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("bias_dtype", C.c_int32), ("act", C.c_int32), ("err_flag", C.c_void_p)]
+
+
 _vp, _i, _i64, _u64, _f, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_size_t
 _cp = C.c_char_p
 
@@ -120,6 +133,9 @@ SIGNATURES = {
     "pm_k_combine": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
     "pm_k_predictor_mlp": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp]),
     "pm_k_rank_topn": (_i, [_vp, _i, _i, _vp, _vp]),
+    "pm_k_route": (_i, [C.POINTER(pm_router), _vp, _i, _i64, _i, _vp, _vp, _vp]),
+    "pm_k_linear": (_i, [C.POINTER(pm_linear), _vp]),
+    "pm_k_token_logprobs": (_i, [_vp, _i, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
 }
 _RAW = {"pm_version", "pm_last_error", "pm_k_swiglu_ffn_scratch_bytes", "pm_k_swiglu_ffn_static_capacity"}
 

@@ -96,6 +96,16 @@ int refuse_if_capturing(cudaStream_t s, const char* who) {
   return PM_OK;
 }
 
+int router_rule(const pm_router* r, const char* who, RouteRule* rule) {
+  const std::string name(who);
+  if (!r) return fail(PM_ERR_INVALID, name + ": null router");
+  if (r->scoring != PM_SCORE_SOFTMAX && r->scoring != PM_SCORE_SIGMOID) return fail(PM_ERR_INVALID, name + ": unknown scoring");
+  if (r->group_score != PM_GROUP_MAX && r->group_score != PM_GROUP_TOP2) return fail(PM_ERR_INVALID, name + ": unknown group_score");
+  *rule = RouteRule{r->num_expert, r->top_k, r->scoring == PM_SCORE_SIGMOID, r->n_group, r->topk_group,
+                    r->group_score == PM_GROUP_TOP2, r->norm_topk != 0, r->routed_scale, r->choice_bias};
+  return check_route_rule(*rule, who);
+}
+
 }  // namespace pm
 
 using namespace pm;
@@ -223,6 +233,71 @@ int pm_k_rank_topn(const float* scores, int width, int n, int32_t* out, void* st
   if (n == 0) return PM_OK;
   if (!scores || !out) return fail(PM_ERR_INVALID, "rank_topn: null pointer");
   PM_CUDA(launch_rank_topn(scores, width, n, out, (cudaStream_t)stream));
+  return PM_OK;
+}
+
+static bool is_dtype(int t) { return t == PM_F32 || t == PM_BF16 || t == PM_F16; }
+// Whether an address is a multiple of the type's size.
+static bool is_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == PM_F32 ? 3u : 1u)) == 0; }
+
+int pm_k_route(const pm_router* router, const void* logits, int dtype, int64_t ld_logits, int n_tokens, int32_t* topk_ids,
+               float* topk_w, void* stream) {
+  RouteRule rule;
+  const int rc = router_rule(router, "route", &rule);
+  if (rc != PM_OK) return rc;
+  if (n_tokens < 0 || n_tokens > (1 << 30)) return fail(PM_ERR_INVALID, "route: the number of tokens must be in [0, 2^30]");
+  if (!is_dtype(dtype)) return fail(PM_ERR_INVALID, "route: unknown logits type");
+  if (ld_logits < rule.E) return fail(PM_ERR_INVALID, "route: ld_logits is smaller than num_expert");
+  if (n_tokens == 0) return PM_OK;
+  if (!logits || !topk_ids || !topk_w) return fail(PM_ERR_INVALID, "route: null pointer");
+  if (!is_aligned(logits, dtype) || !is_aligned(topk_ids, PM_F32) || !is_aligned(topk_w, PM_F32) || !is_aligned(rule.bias, PM_F32))
+    return fail(PM_ERR_INVALID, "route: misaligned pointer");
+  PM_CUDA(launch_route(logits, dtype, ld_logits, n_tokens, rule, topk_ids, topk_w, (cudaStream_t)stream));
+  return PM_OK;
+}
+
+int pm_k_linear(const pm_linear* a, void* stream) {
+  if (!a) return fail(PM_ERR_INVALID, "linear: null arguments");
+  if (a->M < 0 || a->N <= 0 || a->K <= 0) return fail(PM_ERR_INVALID, "linear: N and K must be positive, M not negative");
+  if (a->M > (1 << 30) || a->N > (1 << 30) || a->K > (1 << 30)) return fail(PM_ERR_INVALID, "linear: a size is above 2^30");
+  if (a->dtype != PM_BF16 && a->dtype != PM_F16) return fail(PM_ERR_INVALID, "linear: dtype must be PM_BF16 or PM_F16");
+  if (a->out_dtype != PM_F32 && a->out_dtype != a->dtype) return fail(PM_ERR_INVALID, "linear: out_dtype must be PM_F32 or dtype");
+  if (a->bias && a->bias_dtype != PM_F32 && a->bias_dtype != a->dtype)
+    return fail(PM_ERR_INVALID, "linear: bias_dtype must be PM_F32 or dtype");
+  if (a->act < PM_ACT_NONE || a->act > PM_ACT_GELU_TANH) return fail(PM_ERR_INVALID, "linear: unknown activation");
+  if (a->ld_x < a->K || a->ld_w < a->K || a->ld_y < a->N || (a->residual && a->ld_residual < a->N))
+    return fail(PM_ERR_INVALID, "linear: a pitch is smaller than its row");
+  if (a->M == 0) return PM_OK;
+  if (!a->x || !a->w || !a->y) return fail(PM_ERR_INVALID, "linear: null pointer");
+  if (!is_aligned(a->x, a->dtype) || !is_aligned(a->w, a->dtype) || !is_aligned(a->y, a->out_dtype) ||
+      !is_aligned(a->residual, a->out_dtype) || (a->bias && !is_aligned(a->bias, a->bias_dtype)) || !is_aligned(a->err_flag, PM_F32))
+    return fail(PM_ERR_INVALID, "linear: misaligned pointer");
+  if (a->residual == a->y && a->ld_residual != a->ld_y)
+    return fail(PM_ERR_INVALID, "linear: y over the residual needs the residual's pitch");
+  LinearCall c{};
+  c.x = a->x; c.w = a->w; c.bias = a->bias; c.res = a->residual; c.y = a->y;
+  c.ldx = a->ld_x; c.ldw = a->ld_w; c.ldr = a->ld_residual; c.ldy = a->ld_y;
+  c.M = a->M; c.N = a->N; c.K = a->K;
+  c.type = a->dtype; c.out_type = a->out_dtype; c.bias_type = a->bias_dtype; c.act = a->act;
+  c.err = a->err_flag;
+  return launch_linear(c, (cudaStream_t)stream);
+}
+
+int pm_k_token_logprobs(const void* logits, int dtype, int64_t ld_logits, int n_rows, int vocab, const int64_t* targets, int top_n,
+                        float* logp, float* entropy, int32_t* top_ids, float* top_logp, void* stream) {
+  if (n_rows < 0 || vocab <= 0) return fail(PM_ERR_INVALID, "token_logprobs: vocab must be positive, n_rows not negative");
+  if (!is_dtype(dtype)) return fail(PM_ERR_INVALID, "token_logprobs: unknown logits type");
+  if (ld_logits < vocab) return fail(PM_ERR_INVALID, "token_logprobs: ld_logits is smaller than vocab");
+  if (top_n < 0 || top_n > 32 || top_n > vocab) return fail(PM_ERR_INVALID, "token_logprobs: top_n must be in [0, min(32, vocab)]");
+  if (n_rows > (1 << 28)) return fail(PM_ERR_INVALID, "token_logprobs: at most 2^28 rows");
+  if (n_rows == 0) return PM_OK;
+  if (!logits || (logp && !targets) || (top_n > 0 && (!top_ids || !top_logp)))
+    return fail(PM_ERR_INVALID, "token_logprobs: null pointer");
+  if (!is_aligned(logits, dtype) || ((uintptr_t)targets & 7) != 0 || !is_aligned(logp, PM_F32) || !is_aligned(entropy, PM_F32) ||
+      !is_aligned(top_ids, PM_F32) || !is_aligned(top_logp, PM_F32))
+    return fail(PM_ERR_INVALID, "token_logprobs: misaligned pointer");
+  PM_CUDA(launch_token_logprobs(logits, dtype, ld_logits, n_rows, vocab, targets, top_n, logp, entropy, top_ids, top_logp,
+                                (cudaStream_t)stream));
   return PM_OK;
 }
 

@@ -299,6 +299,35 @@ struct TcLaunch {
 };
 cudaError_t launch_prefill_ffn(const TcLaunch& a, cudaStream_t s, cudaEvent_t mid_event);
 
+// Map of a row-major matrix of 16-bit values [rows, k], pitch_elems apart: boxes of box_rows rows by 64 k, 128-byte swizzle,
+// zeros beyond the matrix. The base and the pitch lie on 16-byte boundaries. A copy moves bits, so bf16 stands for fp16 too.
+int tc_encode_matrix(CUtensorMap* map, const void* base, uint64_t k, uint64_t rows, uint64_t pitch_elems, int box_rows);
+
+// How a router turns logits into experts (route_select.cuh).
+struct RouteRule {
+  int32_t E, k, sigmoid, n_group, topk_group, group_top2, norm;
+  float scale;
+  const float* bias;  // device [E] or nullptr
+};
+int check_route_rule(const RouteRule& r, const char* who);
+int router_rule(const pm_router* r, const char* who, RouteRule* rule);  // checked
+cudaError_t launch_route(const void* logits, int dtype, int64_t ld, int n_tok, const RouteRule& rule, int32_t* ids, float* w,
+                         cudaStream_t s);
+
+// y = act(x w^T + bias) + residual (linear.cu). Types are PM_F32 / PM_BF16 / PM_F16; pitches in elements.
+struct LinearCall {
+  const void *x, *w, *bias, *res;
+  void* y;
+  int64_t ldx, ldw, ldr, ldy;
+  int32_t M, N, K, type, out_type, bias_type, act;
+  int32_t* err;
+};
+int launch_linear(const LinearCall& a, cudaStream_t s);
+
+// Log probability of targets[t], entropy and the n best alternatives of every row of logits (logprobs.cu).
+cudaError_t launch_token_logprobs(const void* logits, int dtype, int64_t ld, int T, int V, const int64_t* targets, int n,
+                                  float* logp, float* entropy, int32_t* top_ids, float* top_logp, cudaStream_t s);
+
 // out[r] = index of the r-th best of scores[0 .. width) (descending, ties to the lower index), r < n.
 cudaError_t launch_rank_topn(const float* scores, int width, int n, int32_t* out, cudaStream_t s);
 

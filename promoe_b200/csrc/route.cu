@@ -1,0 +1,107 @@
+// Stateless router on given logits: the experts of every token and their weights (route_select.cuh has the rule).
+// One warp per token, the row in registers: lane i holds npl = ceil(E / 32) neighbouring experts.
+#include <algorithm>
+
+#include "route_select.cuh"
+
+namespace pm {
+namespace {
+
+constexpr int kRouteWarps = 4;
+constexpr int kRouteMaxExperts = 1024;
+
+// Plain loads: the 16-bit forms of __ldg are pure inline assembly, which the compiler may move in front of a bounds test.
+__device__ __forceinline__ float load_logit(const float* p) { return *p; }
+__device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
+
+template <class T, int NPL>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_constant__ RouteRule rule, int vector_loads,
+             int32_t* __restrict__ topk_ids, float* __restrict__ topk_w) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp;
+  double* work = reinterpret_cast<double*>(smem_raw) + (size_t)warp * rule.E;
+  wait_for_predecessor();
+  if (t >= n_tok) return;
+  const int E = rule.E, npl = (E + 31) / 32, e0 = lane * npl;
+  const T* row = logits + t * ld;
+  float l[NPL];
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) l[j] = -CUDART_INF_F;
+  constexpr int kVec = 16 / sizeof(T);
+  if (vector_loads) {  // E = 32 npl, npl a multiple of kVec, rows on 16-byte boundaries
+    if constexpr (NPL % kVec == 0) {
+#pragma unroll
+      for (int j = 0; j < NPL; j += kVec)
+        if (j < npl) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + e0 + j));
+          const T* p = reinterpret_cast<const T*>(&v);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) l[j + i] = (float)p[i];
+        }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NPL; ++j)
+      if (j < npl && e0 + j < E) l[j] = load_logit(row + e0 + j);
+  }
+  float bias_max = 0.f;
+  if (rule.bias != nullptr) {
+    for (int e = lane; e < E; e += 32) {
+      const float b = fabsf(rule.bias[e]);
+      if (b <= 3.402823466e38f) bias_max = fmaxf(bias_max, b);
+    }
+    bias_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bias_max)));
+  }
+  int id;
+  float w;
+  route_token<NPL>(l, npl, rule, bias_max, work, lane, [&](int e) { return load_logit(row + e); }, id, w);
+  if (lane < rule.k) {
+    topk_ids[t * rule.k + lane] = id;
+    topk_w[t * rule.k + lane] = w;
+  }
+}
+
+template <class T, int NPL>
+cudaError_t launch(const T* logits, int64_t ld, int n_tok, const RouteRule& rule, int32_t* ids, float* w, cudaStream_t s) {
+  const int npl = (rule.E + 31) / 32, vec = 16 / (int)sizeof(T);
+  const int vector_loads = NPL % vec == 0 && npl % vec == 0 && rule.E == 32 * npl && ((uintptr_t)logits & 15) == 0 &&
+                           (ld * (int64_t)sizeof(T)) % 16 == 0;
+  // 64-bit choices of one row per warp: at most 32 KB
+  return launch_behind(route_kernel<T, NPL>, (n_tok + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32,
+                       (size_t)kRouteWarps * rule.E * 8, s, logits, ld, n_tok, rule, vector_loads, ids, w);
+}
+
+template <class T>
+cudaError_t pick(const T* logits, int64_t ld, int n_tok, const RouteRule& rule, int32_t* ids, float* w, cudaStream_t s) {
+  const int npl = (rule.E + 31) / 32;
+  if (npl <= 2) return launch<T, 2>(logits, ld, n_tok, rule, ids, w, s);
+  if (npl <= 8) return launch<T, 8>(logits, ld, n_tok, rule, ids, w, s);
+  return launch<T, 32>(logits, ld, n_tok, rule, ids, w, s);
+}
+
+}  // namespace
+
+int check_route_rule(const RouteRule& r, const char* who) {
+  const std::string name(who);
+  if (r.E <= 0 || r.E > kRouteMaxExperts) return fail(PM_ERR_INVALID, name + ": num_expert must be in [1, 1024]");
+  if (r.k <= 0 || r.k > 32 || r.k > r.E) return fail(PM_ERR_INVALID, name + ": top_k must be in [1, min(32, num_expert)]");
+  if (r.n_group < 1 || r.n_group > 32 || r.E % r.n_group != 0)
+    return fail(PM_ERR_INVALID, name + ": n_group must be in [1, 32] and divide num_expert");
+  if (r.topk_group < 1 || r.topk_group > r.n_group) return fail(PM_ERR_INVALID, name + ": topk_group must be in [1, n_group]");
+  if (r.k > r.topk_group * (r.E / r.n_group))
+    return fail(PM_ERR_INVALID, name + ": topk_group groups hold fewer than top_k experts");
+  return PM_OK;
+}
+
+cudaError_t launch_route(const void* logits, int dtype, int64_t ld, int n_tok, const RouteRule& rule, int32_t* ids, float* w,
+                         cudaStream_t s) {
+  if (n_tok <= 0) return cudaSuccess;
+  if (dtype == PM_F32) return pick((const float*)logits, ld, n_tok, rule, ids, w, s);
+  if (dtype == PM_BF16) return pick((const __nv_bfloat16*)logits, ld, n_tok, rule, ids, w, s);
+  return pick((const __half*)logits, ld, n_tok, rule, ids, w, s);
+}
+
+}  // namespace pm

@@ -12,16 +12,14 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
+  static const EncodeTiledFn fn = []() -> EncodeTiledFn {  // looked up once, also when two threads come first
     cudaDriverEntryPointQueryResult q;
     void* p = nullptr;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
         q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
+      return reinterpret_cast<EncodeTiledFn>(p);
+    return nullptr;
+  }();
   return fn;
 }
 
@@ -82,6 +80,12 @@ bool one_map_spans(const void* a, const void* b) {
 }
 
 }  // namespace
+
+int tc_encode_matrix(CUtensorMap* map, const void* base, uint64_t k, uint64_t rows, uint64_t pitch_elems, int box_rows) {
+  const cuuint64_t dims[2] = {k, rows}, strides[1] = {pitch_elems * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  return encode(map, base, 2, dims, strides, box);
+}
 
 bool tc_prefill_usable(const pm_ctx* c, const pm_layer_weights& w) {
   if (!c->tc_prefill || w.quant4 || encode_fn() == nullptr) return false;
