@@ -20,49 +20,47 @@ _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
 
 
-def _call(device: torch.device, fn, *args) -> None:
-    """fn(*args, stream) with `device` current, on its current stream."""
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+# The stream as an integer, without the Stream object that torch.cuda.current_stream makes (1 us of a call that takes 5).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, stream) with device `index` current, on its current stream."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
-def _rows(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES) -> torch.Tensor:
-    """A CUDA matrix with dense rows of `width` values."""
-    if not t.is_cuda or t.dim() != 2 or t.dtype not in dtypes:
+def _matrix(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES) -> tuple[int, int, int, int]:
+    """(device index, rows, width, pitch) of a CUDA matrix with dense rows, none over another."""
+    index, shape = t.get_device(), t.shape
+    if index < 0 or len(shape) != 2 or t.dtype not in dtypes:
         raise ValueError(f"{what} must be a 2-D CUDA tensor of {', '.join(str(d) for d in dtypes)}")
-    if width is not None and t.shape[1] != width:
-        raise ValueError(f"{what} must have rows of {width} values, not {t.shape[1]}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, n = shape
+    if width is not None and n != width:
+        raise ValueError(f"{what} must have rows of {width} values, not {n}")
+    pitch, inner = t.stride()
+    if inner != 1 and n > 1:
         raise ValueError(f"the rows of {what} must be dense")
+    if rows <= 1:
+        pitch = n  # the stride of a single row says nothing
+    elif pitch < n:
+        raise ValueError(f"the rows of {what} must not overlap (expanded tensors: call contiguous())")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient: these operators have no backward pass")
-    return t
+    return index, rows, n, pitch
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Distance of two rows; rows that lie over one another (a broadcast) are no matrix that the kernels take."""
-    if t.shape[0] <= 1:
-        return max(t.shape[1], 1)
-    if t.stride(0) < t.shape[1]:
-        raise ValueError("rows must not overlap (expanded tensors: call contiguous())")
-    return t.stride(0)
-
-
-def _result(out, shape, dtype, device, what: str) -> torch.Tensor:
+def _result(out, shape, dtype, index: int, what: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}")
+        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))
+    if out.shape != shape or out.dtype != dtype or out.get_device() != index or not out.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index}")
     return out
-
-
-def _same_device(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, not on {t.device}")
 
 
 class Router:
@@ -82,6 +80,7 @@ class Router:
             if not bias.is_cuda or bias.dtype != torch.float32 or bias.shape != (num_expert,) or not bias.is_contiguous():
                 raise ValueError("bias must be a contiguous float32 CUDA tensor of shape [num_expert]")
         self.num_expert, self.top_k, self.bias = num_expert, top_k, bias
+        self.device_index = None if bias is None else bias.get_device()
         self.rule = _lib.pm_router(num_expert, top_k, _SCORING[scoring], n_group, topk_group, _GROUP_SCORE[group_score],
                                    int(norm_topk), routed_scale, None if bias is None else bias.data_ptr())
         self._ref = C.byref(self.rule)
@@ -91,14 +90,13 @@ class Router:
 
     def __call__(self, logits: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None):
         """logits [T, num_expert] float32 / bf16 / fp16 -> (ids [T, top_k] int32, weights [T, top_k] float32)."""
-        _rows(logits, "logits", self.num_expert)
-        dev, T = logits.device, logits.shape[0]
-        _same_device(dev, bias=self.bias)
+        index, T, _, pitch = _matrix(logits, "logits", self.num_expert)
+        if self.device_index is not None and self.device_index != index:
+            raise ValueError(f"logits must be on cuda:{self.device_index}, where the bias is")
         shape = (T, self.top_k)
         ids, w = out if out is not None else (None, None)
-        ids, w = _result(ids, shape, torch.int32, dev, "ids"), _result(w, shape, torch.float32, dev, "weights")
-        _call(dev, self._fn, self._ref, logits.data_ptr(), _DTYPES[logits.dtype], _pitch(logits) if T > 1 else self.num_expert, T,
-              ids.data_ptr(), w.data_ptr())
+        ids, w = _result(ids, shape, torch.int32, index, "ids"), _result(w, shape, torch.float32, index, "weights")
+        _call(index, self._fn, self._ref, logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, ids.data_ptr(), w.data_ptr())
         return ids, w
 
 
@@ -111,7 +109,7 @@ class Linear:
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
                  out_dtype: torch.dtype | None = None):
         weight = weight.detach()
-        _rows(weight, "weight", dtypes=(torch.bfloat16, torch.float16))
+        index, N, K, pitch = _matrix(weight, "weight", dtypes=(torch.bfloat16, torch.float16))
         if activation not in _ACTS:
             raise ValueError(f"activation must be one of {[a for a in _ACTS if a]} or None")
         out_dtype = weight.dtype if out_dtype is None else out_dtype
@@ -119,36 +117,45 @@ class Linear:
             raise ValueError(f"out_dtype must be float32 or {weight.dtype}")
         if bias is not None:
             bias = bias.detach()
-            if bias.shape != (weight.shape[0],) or bias.dtype not in (torch.float32, weight.dtype) or not bias.is_contiguous():
-                raise ValueError(f"bias must be a contiguous tensor of shape [{weight.shape[0]}], float32 or {weight.dtype}")
-            _same_device(weight.device, bias=bias)
-        self.weight, self.bias, self.out_dtype, self.device = weight, bias, out_dtype, weight.device
-        self.N, self.K = weight.shape
-        self._fixed = dict(w=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(), ld_w=_pitch(weight),
-                           N=self.N, K=self.K, dtype=_DTYPES[weight.dtype], out_dtype=_DTYPES[out_dtype],
-                           bias_dtype=0 if bias is None else _DTYPES[bias.dtype], act=_ACTS[activation])
+            if bias.shape != (N,) or bias.dtype not in (torch.float32, weight.dtype) or not bias.is_contiguous():
+                raise ValueError(f"bias must be a contiguous tensor of shape [{N}], float32 or {weight.dtype}")
+            if bias.get_device() != index:
+                raise ValueError(f"bias must be on cuda:{index}, not on {bias.device}")
+        self.weight, self.bias, self.out_dtype, self.device_index, self.N, self.K = weight, bias, out_dtype, index, N, K
+        self._x_dtypes, self._y_dtypes = (weight.dtype,), (out_dtype,)
+        # what stays the same from call to call; a call works on a copy, so that two threads may call at once
+        self._call = bytes(_lib.pm_linear(w=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(), ld_w=pitch, N=N, K=K,
+                                          dtype=_DTYPES[weight.dtype], out_dtype=_DTYPES[out_dtype],
+                                          bias_dtype=0 if bias is None else _DTYPES[bias.dtype], act=_ACTS[activation]))
         self._fn = _lib.load().pm_k_linear
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [M, K] of the weight's type, residual [M, N] of out_dtype (dense rows, any pitch) -> y [M, N]. out may be the
         residual itself; it must not overlap x, the weight or the bias."""
-        _rows(x, "x", self.K, (self.weight.dtype,))
-        M, dev = x.shape[0], self.device
-        _same_device(dev, x=x, residual=residual, out=out)
-        if residual is not None:
-            _rows(residual, "residual", self.N, (self.out_dtype,))
-            if residual.shape[0] != M:
-                raise ValueError(f"residual must have {M} rows, not {residual.shape[0]}")
+        index = self.device_index
+        on, M, _, ld_x = _matrix(x, "x", self.K, self._x_dtypes)
         if out is None:
-            out = torch.empty((M, self.N), dtype=self.out_dtype, device=dev)
-        else:
-            _rows(out, "out", self.N, (self.out_dtype,))
-            if out.shape[0] != M:
-                raise ValueError(f"out must have {M} rows, not {out.shape[0]}")
-        a = _lib.pm_linear(x=x.data_ptr(), y=out.data_ptr(), residual=None if residual is None else residual.data_ptr(),
-                           ld_x=_pitch(x), ld_y=_pitch(out), ld_residual=0 if residual is None else _pitch(residual), M=M, **self._fixed)
-        _call(dev, self._fn, C.byref(a))
+            out = torch.empty((M, self.N), dtype=self.out_dtype, device=x.device)
+        on_y, rows, _, ld_y = _matrix(out, "out", self.N, self._y_dtypes)
+        if rows != M:
+            raise ValueError(f"out must have {M} rows, not {rows}")
+        a = _lib.pm_linear.from_buffer_copy(self._call)
+        a.x, a.y, a.ld_x, a.ld_y, a.M = x.data_ptr(), out.data_ptr(), ld_x, ld_y, M
+        if residual is not None:
+            on_r, rows, _, a.ld_residual = _matrix(residual, "residual", self.N, self._y_dtypes)
+            if rows != M:
+                raise ValueError(f"residual must have {M} rows, not {rows}")
+            if on_r != index:
+                raise ValueError(f"residual must be on cuda:{index}, where the weight is")
+            a.residual = residual.data_ptr()
+        if on != index or on_y != index:
+            raise ValueError(f"x and out must be on cuda:{index}, where the weight is")
+        _call(index, self._fn, C.byref(a))
         return out
+
+
+def _logprobs():
+    return _lib.load().pm_k_token_logprobs
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, out=None):
@@ -157,14 +164,12 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, 
 
     logits [T, V] float32 / bf16 / fp16, targets [T] int64; a negative target names no token (logp 0). Masked logits (-inf)
     have probability 0; pm_k_token_logprobs states what rows without a distribution give. out: the four results to fill."""
-    _rows(logits, "logits")
-    T, V = logits.shape
-    dev = logits.device
-    if targets.shape != (T,) or targets.dtype != torch.int64 or targets.device != dev or not targets.is_contiguous():
-        raise ValueError(f"targets must be a contiguous int64 tensor of shape [{T}] on {dev}")
+    index, T, V, pitch = _matrix(logits, "logits")
+    if targets.shape != (T,) or targets.dtype != torch.int64 or targets.get_device() != index or not targets.is_contiguous():
+        raise ValueError(f"targets must be a contiguous int64 tensor of shape [{T}] on cuda:{index}")
     logp, entropy, ids, best = out if out is not None else (None, None, None, None)
-    logp, entropy = _result(logp, (T,), torch.float32, dev, "logp"), _result(entropy, (T,), torch.float32, dev, "entropy")
-    ids, best = _result(ids, (T, top_n), torch.int32, dev, "top_ids"), _result(best, (T, top_n), torch.float32, dev, "top_logp")
-    _call(dev, _lib.load().pm_k_token_logprobs, logits.data_ptr(), _DTYPES[logits.dtype], _pitch(logits), T, V,
-          targets.data_ptr(), top_n, logp.data_ptr(), entropy.data_ptr(), ids.data_ptr(), best.data_ptr())
+    logp, entropy = _result(logp, (T,), torch.float32, index, "logp"), _result(entropy, (T,), torch.float32, index, "entropy")
+    ids, best = _result(ids, (T, top_n), torch.int32, index, "top_ids"), _result(best, (T, top_n), torch.float32, index, "top_logp")
+    _call(index, _logprobs(), logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, V, targets.data_ptr(), top_n, logp.data_ptr(),
+          entropy.data_ptr(), ids.data_ptr(), best.data_ptr())
     return logp, entropy, ids, best
