@@ -1,17 +1,26 @@
 // Log probability of a given token, entropy and the best alternatives of every row of vocabulary logits, in one pass:
 //   M = max l, S = sum 2^(l log2e - c), U = sum 2^(l log2e - c) (l log2e - c), c = M log2e rounded
 //   lse = c ln2 + ln S,  logp = l_target - lse,  H = ln S - ln2 U / S,  top: l - lse of the n largest
-// c is rounded once and used everywhere, so its rounding cancels; a logit costs one multiply-add, one exponential, one
-// addition, one multiply-add and the maximum.
+// c is rounded once and used everywhere, so its rounding cancels; two logits cost two exponentials and three packed
+// float32 instructions besides the widening and the maximum. Logits are raised to a value that has no probability beside any
+// other (kLow), which keeps 0 times infinity out of U; rows whose maximum is down there are summed again.
 //
 // A row is read by a cluster of CTAs (one where there are many rows); every thread keeps its own running maximum and
 // sums and rescales them when a batch of its values raises the maximum.
 //
-// The n best come out of the same pass. The first batch gives a threshold (of 32 groups of threads the n-th best
-// maximum: n values reach it); every value that reaches it goes to a list in shared memory, about 1.5 n per batch, and at the
-// end a value's place is the number of list entries before it. Entries are (ordered value, reversed index), so ties go to
-// the lower index and the result does not depend on the order in which the list was filled. A row whose list
-// overflows (many equal values, ascending rows) finds its n-th best entry by radix selection over the row instead.
+// The n best come out of the same pass. The first batch gives a floor (of 32 groups of threads the n-th best
+// maximum: n values reach it), later ones raise it; every 16-byte vector with a value that reaches the floor is noted, about
+// 1.5 n of them each time the part read doubles. At the end their values that reach the last floor go to a list, where a
+// value's place is the number of entries before it. Entries are (ordered value, reversed index), so ties go to the lower index and
+// the result does not depend on the order in which the list was filled, nor on the floors. A row whose lists overflow (many
+// equal values, ascending rows) finds its n-th best entry by radix selection over the row instead. (Sorting out the values of
+// a vector inside the loop costs registers and code there: 53 and, for n = 20, 90 us instead of 55 and 58 for 1024 rows of 131072.)
+//
+// What bounds it: long rows HBM. 4096 rows of 131072 bf16 take 166 us = 6.49 TB/s without alternatives, 194 us = 5.5 TB/s with
+// five and 211 us with twenty: the end of a row (two rankings, the noted vectors' way from L2) is latency that four CTAs per SM
+// cover in part. Short rows that end too (4096 of 2048: 12 us without alternatives, 23 with five; one warp per row instead
+// of four changed that by less than a fifth). One row of 131072: 7 to 9 us, the chain of load, floor, sums, two cluster
+// barriers and ranking. First form, with scalar arithmetic and the lists sorted out in the loop: 281 us for 4096 rows, 11.5 for one.
 //
 // Masked logits: -inf has probability 0 and is never an alternative (id -1, log probability -inf where fewer than n are
 // left). A row that holds NaN or +inf, or whose logits are all -inf, is no distribution: NaN and id -1. A negative target names
@@ -29,7 +38,7 @@ using sm100::cluster_sync;
 using sm100::map_to_rank;
 using sm100::smem_u32;
 
-constexpr int kListCap = 1024;
+constexpr int kCap = 1024;  // room in the lists
 constexpr int kMaxTop = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994531;
@@ -43,7 +52,6 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ Entry entry_of(float v, uint32_t index) { return ((Entry)order_of(v) << 32) | (0xffffffffu - index); }
-constexpr uint32_t kOrderNegInf = 0x007fffffu;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -58,34 +66,90 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
   return r;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 16 bytes of logits. kLow: no logit counts beside one that is more than kFar above it, and -inf is raised to it. kLowBits: a
+// register of it. raise(): all values at least kLow, NaN kept. top(): the larger (NaN ignored). pair(i): values 2i, 2i + 1. first(): the
+// lowest value of a 64-bit word.
+constexpr float kFar = 300.f;
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int kN = 4;
-  static __device__ __forceinline__ void widen(const uint4& v, float (&f)[4]) {
-    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  static constexpr float kLow = -0x1p64f;
+  static constexpr uint32_t kLowBits = 0xDF800000u;
+  static __device__ __forceinline__ uint32_t raise(uint32_t w) { return __float_as_uint(max_nan(__uint_as_float(w), kLow)); }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ float first(uint64_t v) { return __uint_as_float((uint32_t)v); }
+  static __device__ __forceinline__ uint64_t pair(const uint4& v, int i) {
+    return i == 0 ? pack2(__uint_as_float(v.x), __uint_as_float(v.y)) : pack2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int kN = 8;
-  static __device__ __forceinline__ void widen(const uint4& v, float (&f)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  static constexpr float kLow = -0x1p64f;
+  static constexpr uint32_t kLowBits = 0xDF80DF80u;
+  static __device__ __forceinline__ uint32_t raise(uint32_t w) {
+    const uint32_t low = kLowBits;
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ float first(uint64_t v) { return __uint_as_float((uint32_t)v << 16); }
+  static __device__ __forceinline__ uint64_t pair(const uint4& v, int i) {
+    const uint32_t w = (&v.x)[i];
+    return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
 };
 template <> struct Vec<__half> {
   static constexpr int kN = 8;
-  static __device__ __forceinline__ void widen(const uint4& v, float (&f)[8]) {
-    const __half2* p = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = __half22float2(p[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
+  static constexpr float kLow = -65504.f;
+  static constexpr uint32_t kLowBits = 0xFBFFFBFFu;
+  static __device__ __forceinline__ uint32_t raise(uint32_t w) {
+    const uint32_t low = kLowBits;
+    const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return fmaxf(f.x, f.y);
+  }
+  static __device__ __forceinline__ float first(uint64_t v) { return __half2float(__ushort_as_half((unsigned short)v)); }
+  static __device__ __forceinline__ uint64_t pair(const uint4& v, int i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&(&v.x)[i]));
+    return pack2(f.x, f.y);
   }
 };
 template <class T> __device__ __forceinline__ float widen_one(T v);
@@ -93,33 +157,30 @@ template <> __device__ __forceinline__ float widen_one(float v) { return v; }
 template <> __device__ __forceinline__ float widen_one(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float widen_one(__half v) { return __half2float(v); }
 
-// Running sums of one thread, or of a part of the row. m: largest value so far, c: m log2e (0 while m is -inf). For values
-// near the type's limits c stops at a number that float32 holds: below, the sum is then 0, as it should be beside any ordinary
-// value; rows whose maximum lies out there are summed again at the end.
+// Running sums of one thread, or of a part of the row. m: largest value so far (at least kLow), c: m log2e.
 struct Sums {
   float m, c, s, u;
 };
-__device__ __forceinline__ Sums no_sums() { return Sums{-CUDART_INF_F, 0.f, 0.f, 0.f}; }
-
-__device__ __forceinline__ void raise(Sums& a, float m) {  // m > a.m
-  const float c = fminf(fmaxf(m, -2e38f), 2e38f) * kLog2e, d = a.c - c;
-  const float f = a.s > 0.f ? exp2_fast(d) : 0.f;
-  a.u = a.s > 0.f ? f * (a.u + d * a.s) : (a.s != a.s ? a.s : 0.f);
-  a.s = a.s != a.s ? a.s : a.s * f;
+template <class T>
+__device__ __forceinline__ Sums no_sums() { return Sums{Vec<T>::kLow, Vec<T>::kLow * kLog2e, 0.f, 0.f}; }
+__device__ __forceinline__ void join(Sums& a, const Sums& b) {
+  const float m = fmaxf(a.m, b.m), c = m * kLog2e;
+  const float da = a.c - c, db = b.c - c, fa = exp2_fast(da), fb = exp2_fast(db);
+  a.u = fa * (a.u + da * a.s) + fb * (b.u + db * b.s);
+  a.s = fa * a.s + fb * b.s;
   a.m = m;
   a.c = c;
 }
-__device__ __forceinline__ void add_value(Sums& a, float l) {
-  const float t = fmaf(l, kLog2e, -a.c), e = exp2_fast(t);
-  a.s += e;
-  a.u = fmaf(e, fmaxf(t, -1e4f), a.u);  // masked values: 0 times a finite number
-}
-__device__ __forceinline__ void join(Sums& a, const Sums& b) {
-  if (b.m > a.m) raise(a, b.m);
-  const float d = b.m == -CUDART_INF_F ? 0.f : b.c - a.c;  // sums of a part without a finite value are 0 or NaN
-  const float f = exp2_fast(d);
-  a.u += b.s == 0.f ? 0.f : f * (b.u + fmaxf(d, -1e4f) * b.s);
-  a.s += f * b.s;
+// Over the first `width` lanes of every group of `width`; the group's first lane has the result.
+__device__ __forceinline__ void join_lanes(Sums& a, int width) {
+  for (int d = width >> 1; d >= 1; d >>= 1) {
+    Sums o;
+    o.m = __shfl_down_sync(0xffffffffu, a.m, d, width);
+    o.c = __shfl_down_sync(0xffffffffu, a.c, d, width);
+    o.s = __shfl_down_sync(0xffffffffu, a.s, d, width);
+    o.u = __shfl_down_sync(0xffffffffu, a.u, d, width);
+    join(a, o);
+  }
 }
 
 struct LogprobArgs {
@@ -134,17 +195,16 @@ struct LogprobArgs {
 
 template <int THREADS>
 struct LogprobShared {
-  Sums warp_sums[THREADS / 32];
-  Sums part;              // this CTA's sums, read by rank 0
+  alignas(16) Entry list[kCap];
+  Sums warp_sums[32];
+  alignas(16) Sums part;  // this CTA's sums, read by rank 0
   Entry best[kMaxTop];    // this CTA's n best in order, read by rank 0
-  float seg[32];
-  Entry list[kListCap];
-  int count;
+  float seg[32];          // largest value of each group of threads so far
+  int count, n_hot;
+  int32_t hot[kCap];   // 16-byte vectors that held a value that reached the floor
   uint32_t hist[256];
   Entry prefix;
   int need;
-  double lse;
-  int dead;
 };
 
 // Entries of `list` in order: out[r] = the r-th largest, r < n; 0 where there are fewer.
@@ -153,19 +213,36 @@ __device__ __forceinline__ void rank_list(const Entry* list, int count, Entry* o
   const int tid = threadIdx.x;
   for (int r = tid; r < n; r += THREADS)
     if (r >= count) out[r] = 0;
+  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
   for (int i = tid; i < count; i += THREADS) {
     const Entry mine = list[i];
-    int before = 0;
-    for (int j = 0; j < count; ++j) before += list[j] > mine;
+    int before = 0, j = 0;
+    for (; j + 8 <= count; j += 8) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const ulonglong2 o = pairs[j / 2 + k];
+        before += (o.x > mine) + (o.y > mine);
+      }
+    }
+    for (; j < count; ++j) before += list[j] > mine;
     if (before < n) out[before] = mine;
   }
+}
+
+// The n-th largest of 32 values, one per lane: the least of those that fewer than n exceed.
+__device__ __forceinline__ float nth_best(float mine, int n) {
+  int above = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) above += __shfl_sync(0xffffffffu, mine, i) > mine;
+  return value_of(__reduce_min_sync(0xffffffffu, above < n ? order_of(mine) : 0xffffffffu));
 }
 
 template <class T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   __shared__ LogprobShared<THREADS> sh;
-  constexpr int N = Vec<T>::kN;
+  using V = Vec<T>;
+  constexpr int N = V::kN, kBatch = kUnroll * THREADS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank();
   const int row = blockIdx.x / parts, n = a.n;
@@ -177,116 +254,162 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   const int v0 = (int)((long long)n_vec * rank / parts), v1 = (int)((long long)n_vec * (rank + 1) / parts);
   const uint4* body = reinterpret_cast<const uint4*>(l + head);
 
-  Sums a0 = no_sums();
-  if (tid == 0) sh.count = 0;
+  uint4 cur[kUnroll], next[kUnroll];
+  auto fetch = [&](int base) {
+    if (base + kBatch <= v1) {
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) next[k] = load_stream(body + base + k * THREADS + tid);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        next[k] = make_uint4(V::kLowBits, V::kLowBits, V::kLowBits, V::kLowBits);  // adds nothing
+        if (base + k * THREADS + tid < v1) next[k] = load_stream(body + base + k * THREADS + tid);
+      }
+    }
+  };
+  if (v0 < v1) fetch(v0);
+  int64_t target = -1;  // asked for early, used at the end
+  float at_target = 0.f;
+  if (tid == 0 && rank == 0 && a.logp != nullptr) {
+    target = a.targets[row];
+    if (target >= 0 && target < a.V) at_target = widen_one(l[target]);
+  }
+  if (tid == 0) sh.count = sh.n_hot = 0;
   __syncthreads();
   auto push = [&](Entry e) {
     const int at = atomicAdd(&sh.count, 1);
-    if (at < kListCap) sh.list[at] = e;
+    if (at < kCap) sh.list[at] = e;
+  };
+  float m = V::kLow, c = V::kLow * kLog2e;
+  uint64_t s2 = 0, u2 = 0, s3 = 0, u3 = 0;  // two pairs of running sums
+  auto raise_to = [&](float top) {
+    const float nc = top * kLog2e, d = c - nc, f = exp2_fast(d);
+    const uint64_t ff = pack2(f, f), dd = pack2(d, d);
+    u2 = fma2(ff, fma2(dd, s2, u2), 0);
+    u3 = fma2(ff, fma2(dd, s3, u3), 0);
+    s2 = fma2(ff, s2, 0);
+    s3 = fma2(ff, s3, 0);
+    m = top;
+    c = nc;
+  };
+  auto add_pair = [&](uint64_t v, uint64_t minus_c, uint64_t& s, uint64_t& u) {
+    const uint64_t t = fma2(v, pack2(kLog2e, kLog2e), minus_c);
+    float lo, hi;
+    unpack2(t, lo, hi);
+    const uint64_t e = pack2(exp2_fast(lo), exp2_fast(hi));
+    s = add2(s, e);
+    u = fma2(e, t, u);
   };
   // values before the first and behind the last 16-byte boundary
-  if (rank == 0) {
-    const int loose = head + (a.V - tail0);
-    if (tid < loose) {
-      const int i = tid < head ? tid : tail0 + tid - head;
-      const float v = widen_one(l[i]);
-      if (v > a0.m) raise(a0, v);
-      add_value(a0, v);
-      if (n > 0 && order_of(v) > kOrderNegInf && v == v) push(entry_of(v, (uint32_t)i));
-    }
+  if (rank == 0 && tid < head + a.V - tail0) {
+    const int i = tid < head ? tid : tail0 + tid - head;
+    const float v = widen_one(l[i]), raised = max_nan(v, V::kLow);
+    if (raised > m) raise_to(raised);
+    add_pair(pack2(raised, V::kLow), pack2(-c, -c), s2, u2);
+    if (raised == V::kLow) s2 = u2 = 0;  // what a masked value and the filler would count for beside nothing else
+    if (n > 0 && v > -CUDART_INF_F) push(entry_of(v, (uint32_t)i));
   }
-  Entry threshold = ((Entry)kOrderNegInf << 32) | 0xffffffffu;
-  float floor_v = -CUDART_INF_F;
-  uint4 next[kUnroll];
-  auto fetch = [&](int base) {
+  const float above_low = __int_as_float(__float_as_int(V::kLow) - 1);  // the next number; raised values are not noted
+  float floor_v = above_low;
+  auto group_best = [&]() {
+    constexpr int kGroup = THREADS / 32;
+    float g = m;
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int v = base + k * THREADS + tid;
-      if (v < v1) next[k] = load_stream(body + v);
-    }
+    for (int d = kGroup / 2; d >= 1; d >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
+    if (tid % kGroup == 0) sh.seg[tid / kGroup] = g;
   };
-  fetch(v0);
-  for (int base = v0; base < v1; base += kUnroll * THREADS) {
-    uint4 cur[kUnroll];
+  int batch = 0;
+  for (int base = v0; base < v1; base += kBatch, ++batch) {
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) cur[k] = next[k];
-    if (base + kUnroll * THREADS < v1) fetch(base + kUnroll * THREADS);
-    float top[kUnroll], all = -CUDART_INF_F;
+    if (base + kBatch < v1) fetch(base + kBatch);
+    uint32_t top_w = V::kLowBits;
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
-      top[k] = -CUDART_INF_F;
-      if (base + k * THREADS + tid < v1) {
-        float f[N];
-        Vec<T>::widen(cur[k], f);
-#pragma unroll
-        for (int i = 0; i < N; ++i) top[k] = fmaxf(top[k], f[i]);
-      }
-      all = fmaxf(all, top[k]);
+      cur[k].x = V::raise(cur[k].x);
+      cur[k].y = V::raise(cur[k].y);
+      cur[k].z = V::raise(cur[k].z);
+      cur[k].w = V::raise(cur[k].w);
+      top_w = V::larger(top_w, V::larger(V::larger(cur[k].x, cur[k].y), V::larger(cur[k].z, cur[k].w)));
     }
-    if (all > a0.m) raise(a0, all);
+    const float all = V::top(top_w);
+    if (all > m) raise_to(all);
+    const uint64_t minus_c = pack2(-c, -c);
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k)
-      if (base + k * THREADS + tid < v1) {
-        float f[N];
-        Vec<T>::widen(cur[k], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) add_value(a0, f[i]);
+      for (int i = 0; i < N / 2; i += 2) {
+        add_pair(V::pair(cur[k], i), minus_c, s2, u2);
+        add_pair(V::pair(cur[k], i + 1), minus_c, s3, u3);
       }
     if (n == 0) continue;
-    if (base == v0) {
-      // threshold: the n-th best of 32 groups' maxima
-      constexpr int kGroup = THREADS / 32;
-      float g = all;
-#pragma unroll
-      for (int m = kGroup / 2; m >= 1; m >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, m));
-      if (tid % kGroup == 0) sh.seg[tid / kGroup] = g;
-      __syncthreads();
-      const float mine = sh.seg[lane];
-      int before = 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float o = __shfl_sync(0xffffffffu, mine, i);
-        before += o > mine || (o == mine && i < lane);
-      }
-      floor_v = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, before == n - 1)) - 1);
-      if (floor_v > -CUDART_INF_F) threshold = (Entry)order_of(floor_v) << 32;
+    if ((batch & (batch + 1)) == 0) {  // batches 0, 1, 3, 7, ...
+      group_best();
+      // At first every group has to have its value there. Later a warp may see other groups' older, lower ones: they are
+      // maxima of those groups all the same. (It takes them once: they may rise while it compares them.)
+      if (batch == 0) __syncthreads();
+      else __syncwarp();
+      floor_v = fmaxf(nth_best(*(volatile float*)&sh.seg[lane], n), above_low);
     }
-    if (all >= floor_v && all > -CUDART_INF_F) {
+    if (all >= floor_v) {
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k)
-        if (top[k] >= floor_v && top[k] > -CUDART_INF_F) {
-          float f[N];
-          Vec<T>::widen(cur[k], f);
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (f[i] >= floor_v) {
-              const Entry e = entry_of(f[i], (uint32_t)(head + (base + k * THREADS + tid) * N + i));
-              if (e > threshold) push(e);
-            }
+      for (int k = 0; k < kUnroll; ++k) {
+        const int v = base + k * THREADS + tid;
+        if (V::top(V::larger(V::larger(cur[k].x, cur[k].y), V::larger(cur[k].z, cur[k].w))) >= floor_v && v < v1) {
+          const int at = atomicAdd(&sh.n_hot, 1);
+          if (at < kCap) sh.hot[at] = v;
         }
+      }
     }
   }
 
-  // sums of the warp, the CTA, the row
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) {
-    Sums o;
-    o.m = __shfl_xor_sync(0xffffffffu, a0.m, m);
-    o.c = __shfl_xor_sync(0xffffffffu, a0.c, m);
-    o.s = __shfl_xor_sync(0xffffffffu, a0.s, m);
-    o.u = __shfl_xor_sync(0xffffffffu, a0.u, m);
-    join(a0, o);
+  // sums of the thread, the warp, the CTA
+  Sums a0;
+  {
+    float s_lo, s_hi, u_lo, u_hi;
+    unpack2(add2(s2, s3), s_lo, s_hi);
+    unpack2(add2(u2, u3), u_lo, u_hi);
+    a0 = Sums{m, c, s_lo + s_hi, u_lo + u_hi};
   }
+  join_lanes(a0, 32);
   if (lane == 0) sh.warp_sums[warp] = a0;
+  if (n > 0 && batch > 1) group_best();
   __syncthreads();
-  if (tid == 0) {
-    Sums t = sh.warp_sums[0];
-    for (int w = 1; w < THREADS / 32; ++w) join(t, sh.warp_sums[w]);
-    sh.part = t;
+  if (warp == 0) {
+    Sums t = lane < THREADS / 32 ? sh.warp_sums[lane] : no_sums<T>();
+    join_lanes(t, THREADS / 32);
+    if (lane == 0) sh.part = t;
   }
   if (n > 0) {
-    int count = sh.count;
-    if (count > kListCap) {
+    const bool all_hot = sh.n_hot <= kCap;
+    int count = 0;
+    if (all_hot) {
+      // the noted vectors once more, against the last floor
+      // (after a single batch the loop's is the last)
+      if (batch > 1) floor_v = fmaxf(nth_best(sh.seg[lane], n), above_low);
+      const bool low = floor_v == above_low;
+      for (int i = tid; i < sh.n_hot; i += THREADS) {
+        const int at = head + sh.hot[i] * N;
+        const uint4 w = body[sh.hot[i]];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float x = widen_one(reinterpret_cast<const T*>(&w)[j]);
+          if (x >= floor_v) push(entry_of(x, (uint32_t)(at + j)));
+        }
+      }
+      __syncthreads();
+      count = sh.count;
+      if (low) __syncthreads();
+      if (low && count < n) {  // finite values from kLow down, if there are any
+        for (int i = head + v0 * N + tid; i < head + v1 * N; i += THREADS) {
+          const float x = widen_one(l[i]);
+          if (x > -CUDART_INF_F && x <= V::kLow) push(entry_of(x, (uint32_t)i));
+        }
+        __syncthreads();
+        count = sh.count;
+      }
+    }
+    if (!all_hot || count > kCap) {
       // radix selection of the n-th largest entry of this part, eight bits at a time from the top
       if (tid == 0) {
         sh.prefix = 0;
@@ -325,7 +448,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
         }
         __syncthreads();
       }
-      const Entry least = sh.prefix;  // the n-th largest (there are more than kListCap)
+      const Entry least = sh.prefix;  // the n-th largest, or the lowest if there are fewer
       if (tid == 0) sh.count = 0;
       __syncthreads();
       for (int pass = 0; pass < 2; ++pass) {
@@ -344,27 +467,24 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   if (parts > 1) {
     cluster_sync();
     if (rank == 0) {
-      if (tid == 0) {
-        Sums t = sh.part;
-        for (int p = 1; p < parts; ++p) {
-          const uint32_t at = map_to_rank(smem_u32(&sh.part), p);
-          Sums o;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.m) : "r"(at));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.c) : "r"(at + 4));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.s) : "r"(at + 8));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.u) : "r"(at + 12));
-          join(t, o);
+      if (warp == 0) {
+        Sums t = no_sums<T>();
+        if (lane < parts)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(t.m), "=f"(t.c), "=f"(t.s), "=f"(t.u)
+                       : "r"(map_to_rank(smem_u32(&sh.part), lane)));
+        join_lanes(t, 8);
+        __syncwarp();
+        if (lane == 0) {
+          sh.part = t;
+          sh.count = 0;
         }
-        sh.part = t;
-        sh.count = 0;
       }
       __syncthreads();
-      if (n > 0) {
-        for (int i = tid; i < parts * n; i += THREADS) {
-          Entry e;
-          asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(e) : "r"(map_to_rank(smem_u32(&sh.best[i % n]), i / n)));
-          if (e != 0) push(e);
-        }
+      for (int i = tid; i < parts * n; i += THREADS) {
+        Entry e;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(e) : "r"(map_to_rank(smem_u32(&sh.best[i % n]), i / n)));
+        if (e != 0) push(e);
       }
     }
     cluster_sync();  // nobody leaves before its part was read
@@ -374,45 +494,59 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   __syncthreads();
 
   Sums t = sh.part;
-  if (fabsf(t.m) > 1e37f && fabsf(t.m) < CUDART_INF_F) {
-    // m log2e may have overflowed (a row of the type's lowest value): once more, relative to the maximum
-    Sums b = no_sums();
+  const bool again = !(t.m > V::kLow + kFar) || t.m > 1e37f;
+  if (again) {
+    // A row of the type's lowest values, or one so large that c overflows: its true maximum, and everything relative to it
+    float top = -CUDART_INF_F;
     bool bad = false;
     for (int i = tid; i < a.V; i += THREADS) {
-      const float v = widen_one(l[i]), d = (v - t.m) * kLog2e, e = exp2_fast(d);
+      const float v = widen_one(l[i]);
       bad |= v != v;
-      b.s += e;
-      b.u = fmaf(e, fmaxf(d, -1e4f), b.u);
+      top = fmaxf(top, v);
     }
+    top = value_of(__reduce_max_sync(0xffffffffu, order_of(top)));
+    if (lane == 0) sh.warp_sums[warp].m = top;
+    bad = __syncthreads_or(bad);
+    for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, sh.warp_sums[w].m);
+    float s = 0.f, u = 0.f;
+    if (fabsf(top) < CUDART_INF_F)
+      for (int i = tid; i < a.V; i += THREADS) {
+        const float d = (widen_one(l[i]) - top) * kLog2e, e = exp2_fast(d);
+        s += e;
+        u = fmaf(e, fmaxf(d, -1e4f), u);
+      }
 #pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) {
-      b.s += __shfl_xor_sync(0xffffffffu, b.s, m);
-      b.u += __shfl_xor_sync(0xffffffffu, b.u, m);
+    for (int d = 16; d >= 1; d >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, d);
+      u += __shfl_xor_sync(0xffffffffu, u, d);
     }
-    if (lane == 0) sh.warp_sums[warp] = b;
     __syncthreads();
-    t.s = t.u = 0.f;
+    if (lane == 0) {
+      sh.warp_sums[warp].s = s;
+      sh.warp_sums[warp].u = u;
+    }
+    __syncthreads();
+    t = Sums{top, 0.f, 0.f, 0.f};
     for (int w = 0; w < THREADS / 32; ++w) {
       t.s += sh.warp_sums[w].s;
       t.u += sh.warp_sums[w].u;
     }
-    if (__syncthreads_or(bad)) t.s = CUDART_NAN_F;
+    if (bad) t.s = CUDART_NAN_F;
   }
+  if (warp != 0) return;
   const bool dead = !(t.s > 0.f) || !(fabsf(t.m) < CUDART_INF_F);
-  const double log_s = log((double)t.s);
-  const double lse = dead ? CUDART_NAN : (fabsf(t.m) > 1e37f ? (double)t.m : (double)t.c * kLn2) + log_s;
-  if (tid == 0) {
+  const float log_s = logf(t.s);
+  const double lse = dead ? CUDART_NAN : (again ? (double)t.m : (double)t.c * kLn2) + (double)log_s;
+  if (lane == 0) {
     if (a.logp != nullptr) {
-      const int64_t target = a.targets[row];
-      a.logp[row] = target < 0 ? 0.f : (dead || target >= a.V) ? CUDART_NAN_F : (float)((double)widen_one(l[target]) - lse);
+      a.logp[row] = target < 0 ? 0.f : dead || target >= a.V ? CUDART_NAN_F : (float)((double)at_target - lse);
     }
-    if (a.entropy != nullptr)
-      a.entropy[row] = dead ? CUDART_NAN_F : (float)(log_s - kLn2 * (double)t.u / (double)t.s);
+    if (a.entropy != nullptr) a.entropy[row] = dead ? CUDART_NAN_F : fmaf(-(float)kLn2, t.u / t.s, log_s);
   }
-  for (int r = tid; r < n; r += THREADS) {
-    const Entry e = dead ? 0 : sh.best[r];
-    a.top_ids[(int64_t)row * n + r] = e == 0 ? -1 : (int32_t)(0xffffffffu - (uint32_t)e);
-    a.top_logp[(int64_t)row * n + r] =
+  if (lane < n) {
+    const Entry e = dead ? 0 : sh.best[lane];
+    a.top_ids[(int64_t)row * n + lane] = e == 0 ? -1 : (int32_t)(0xffffffffu - (uint32_t)e);
+    a.top_logp[(int64_t)row * n + lane] =
         dead ? CUDART_NAN_F : e == 0 ? -CUDART_INF_F : (float)((double)value_of((uint32_t)(e >> 32)) - lse);
   }
 }
@@ -438,8 +572,11 @@ cudaError_t pick(const LogprobArgs& a, int sms, cudaStream_t s) {
   // a cluster per row while that fills the GPU no more than about twice and a part stays longer than a batch of 128 threads
   int parts = 1;
   while (parts < 8 && (int64_t)a.T * parts * 2 <= 2 * sms && a.V / (2 * parts) >= 4096) parts *= 2;
-  // a thread should have a whole batch, and each of the 32 groups of threads values for the threshold
-  if (a.V / parts >= 512 * kUnroll * Vec<T>::kN / 2) return launch<T, 512>(a, parts, s);
+  // Every thread should have half a batch, and each of the 32 groups of threads values for the floor. Parts of a row are
+  // short: more threads finish sooner. Whole rows leave room for other rows' CTAs, which work while one row is finished.
+  const int vectors = a.V / parts / Vec<T>::kN;
+  if (parts > 1 && vectors >= 512 * kUnroll / 2) return launch<T, 512>(a, parts, s);
+  if (vectors >= 256 * kUnroll / 2) return launch<T, 256>(a, parts, s);
   return launch<T, 128>(a, parts, s);
 }
 

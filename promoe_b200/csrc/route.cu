@@ -16,51 +16,57 @@ __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __b
 __device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
 
 template <class T, int NPL>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+__global__ void __launch_bounds__(kRouteWarps * 32, NPL <= 8 ? 8 : 4)
 route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_constant__ RouteRule rule, int vector_loads,
              int32_t* __restrict__ topk_ids, float* __restrict__ topk_w) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp;
-  double* work = reinterpret_cast<double*>(smem_raw) + (size_t)warp * rule.E;
-  wait_for_predecessor();
-  if (t >= n_tok) return;
   const int E = rule.E, npl = (E + 31) / 32, e0 = lane * npl;
-  const T* row = logits + t * ld;
-  float l[NPL];
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) l[j] = -CUDART_INF_F;
-  constexpr int kVec = 16 / sizeof(T);
-  if (vector_loads) {  // E = 32 npl, npl a multiple of kVec, rows on 16-byte boundaries
-    if constexpr (NPL % kVec == 0) {
-#pragma unroll
-      for (int j = 0; j < NPL; j += kVec)
-        if (j < npl) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + e0 + j));
-          const T* p = reinterpret_cast<const T*>(&v);
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) l[j + i] = (float)p[i];
-        }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (j < npl && e0 + j < E) l[j] = load_logit(row + e0 + j);
-  }
+  RouteScratch* scratch = reinterpret_cast<RouteScratch*>(smem_raw + warp * route_scratch_bytes(E));
+  wait_for_predecessor();
+
+  float b[NPL];
   float bias_max = 0.f;
   if (rule.bias != nullptr) {
-    for (int e = lane; e < E; e += 32) {
-      const float b = fabsf(rule.bias[e]);
-      if (b <= 3.402823466e38f) bias_max = fmaxf(bias_max, b);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+      b[j] = j < npl && e0 + j < E ? rule.bias[e0 + j] : 0.f;
+      if (fabsf(b[j]) <= 3.402823466e38f) bias_max = fmaxf(bias_max, fabsf(b[j]));
     }
     bias_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bias_max)));
   }
-  int id;
-  float w;
-  route_token<NPL>(l, npl, rule, bias_max, work, lane, [&](int e) { return load_logit(row + e); }, id, w);
-  if (lane < rule.k) {
-    topk_ids[t * rule.k + lane] = id;
-    topk_w[t * rule.k + lane] = w;
+  constexpr int kVec = 16 / sizeof(T);
+  float l[NPL];
+  auto load = [&](int64_t t) {
+    const T* row = logits + t * ld;
+    if (vector_loads) {  // E = 32 npl, npl a multiple of kVec, rows on 16-byte boundaries
+      if constexpr (NPL % kVec == 0) {
+#pragma unroll
+        for (int j = 0; j < NPL; j += kVec)
+          if (j < npl) {
+            const uint4 v = *reinterpret_cast<const uint4*>(row + e0 + j);
+            const T* p = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) l[j + i] = (float)p[i];
+          }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NPL; ++j)
+        if (j < npl && e0 + j < E) l[j] = load_logit(row + e0 + j);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) l[j] = -CUDART_INF_F;
+  const int64_t step = (int64_t)gridDim.x * kRouteWarps;
+  for (int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp; t < n_tok; t += step) {
+    load(t);
+    const T* row = logits + t * ld;
+    route_token<NPL>(l, npl, rule, b, bias_max, scratch, lane, [&](int e) { return load_logit(row + e); },
+                     [&](int j, int id, float w) {
+                       topk_ids[t * rule.k + j] = id;
+                       topk_w[t * rule.k + j] = w;
+                     });
   }
 }
 
@@ -69,9 +75,14 @@ cudaError_t launch(const T* logits, int64_t ld, int n_tok, const RouteRule& rule
   const int npl = (rule.E + 31) / 32, vec = 16 / (int)sizeof(T);
   const int vector_loads = NPL % vec == 0 && npl % vec == 0 && rule.E == 32 * npl && ((uintptr_t)logits & 15) == 0 &&
                            (ld * (int64_t)sizeof(T)) % 16 == 0;
-  // 64-bit choices of one row per warp: at most 32 KB
-  return launch_behind(route_kernel<T, NPL>, (n_tok + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32,
-                       (size_t)kRouteWarps * rule.E * 8, s, logits, ld, n_tok, rule, vector_loads, ids, w);
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+  // One row after the other per warp once every SM has its 48 warps; at most 34 KB of shared memory per block.
+  const int blocks = std::min((n_tok + kRouteWarps - 1) / kRouteWarps, sms * 48 / kRouteWarps);
+  return launch_behind(route_kernel<T, NPL>, blocks, kRouteWarps * 32, kRouteWarps * route_scratch_bytes(rule.E), s, logits, ld,
+                       n_tok, rule, vector_loads, ids, w);
 }
 
 template <class T>

@@ -108,68 +108,70 @@ __device__ __noinline__ int exact_rank(double* c, const RouteRule* rule, uint32_
   return mine;
 }
 
-// Experts lane * npl .. lane * npl + npl - 1 of the row are l[0 .. npl) of this lane (-inf beyond E; npl <= NPL).
-// work: E doubles of shared memory of this warp. bias_max: largest |finite bias|, 0 without one. logit(e) reads the row again.
-// Lane j < k gets the j-th id and its weight.
-template <int NPL, class Logit>
-__device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, const RouteRule& r, float bias_max, double* work,
-                                            int lane, const Logit& logit, int& id, float& weight) {
+// How the warp chooses. Lane i holds npl neighbouring experts, so lower lanes hold lower ids. The k-th largest of the lanes'
+// maxima is a floor that k experts reach, and usually few more do: those are laid out one per lane, in the order of
+// their ids, and each counts how many rank before it. Against k rounds of arg-max over all experts this is half the
+// instructions (16384 tokens of 256 experts in 8 groups, 8 of them chosen: 51.7 -> 10.4 us). Where more than 32
+// experts reach the floor (many equal logits, large k) the rounds remain.
+struct RouteScratch {  // shared memory of one warp, followed by E doubles
+  uint32_t key[33];    // candidates; then their values in rank order
+  uint32_t id[33];
+};
+__host__ __device__ __forceinline__ size_t route_scratch_bytes(int E) { return sizeof(RouteScratch) + 8 * (size_t)((E + 1) / 2 * 2); }
+
+// Row of a token: experts lane * npl .. lane * npl + npl - 1 are l[0 .. npl) of this lane (-inf beyond E; npl <= NPL), and
+// their correction biases b[0 .. npl), with bias_max the largest finite |bias| (both unused without a bias).
+// logit(e) reads the row again. write(j, id, weight) is called once for each j < k, by any lane.
+template <int NPL, class Logit, class Write>
+__device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, const RouteRule& r, const float (&b)[NPL], float bias_max,
+                                            RouteScratch* scratch, int lane, const Logit& logit, const Write& write) {
   const int E = r.E, e0 = lane * npl;
+  double* work = reinterpret_cast<double*>(scratch + 1);
   const bool by_logit = r.bias == nullptr, grouped = r.n_group > 1 && r.topk_group < r.n_group, sums = grouped && r.group_top2 != 0;
   float top = -CUDART_INF_F;
   bool odd = false;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j)
-    if (j < npl) {
-      odd |= !(l[j] <= 3.402823466e38f) && (l[j] != l[j] || !r.sigmoid);
-      top = fmaxf(top, l[j]);
-    }
-  id = -1;
-  if (__any_sync(0xffffffffu, odd)) {
-    weight = CUDART_NAN_F;
-    return;
+  for (int j = 0; j < NPL; ++j) {
+    odd |= !(l[j] <= 3.402823466e38f);  // NaN or +inf
+    top = fmaxf(top, l[j]);
   }
-  weight = 0.f;
+  if (__any_sync(0xffffffffu, odd)) {
+    bool dead = false;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) dead |= l[j] != l[j] || (!r.sigmoid && l[j] == CUDART_INF_F);
+    if (__any_sync(0xffffffffu, dead)) {
+      if (lane < r.k) write(lane, -1, CUDART_NAN_F);
+      return;
+    }
+  }
   top = key_value(__reduce_max_sync(0xffffffffu, order_key(top)));
-  if (top == -CUDART_INF_F) return;  // nothing to choose from
-  float sum = 0.f;
-  float s[NPL];
+  // A float32 score is off by at most 1e-6 of the largest (the exponential's argument is off by half a step, the
+  // exponential and the division by about two), a choice by that and half a step of its own.
+  float sum = 0.f, margin = 0.f;
+  uint32_t key[NPL];  // ordered choices, 0: cannot be chosen
   if (!r.sigmoid) {
+    const float base = top == -CUDART_INF_F ? 0.f : top;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-      s[j] = j < npl ? __expf(l[j] - top) : 0.f;
-      sum += s[j];
+      const float e = __expf(l[j] - base);
+      key[j] = __float_as_uint(e);
+      sum += e;
     }
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   }
-  uint32_t key[NPL];  // 0: cannot be chosen
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) key[j] = j < npl && l[j] > -CUDART_INF_F ? order_key(l[j]) : 0u;
-  // A float32 score is off by at most 1e-6 of the largest (the exponential's argument is off by half a step, the
-  // exponential and the division by about two), a choice by that and half a step of its own.
-  float margin = 0.f;
-  uint32_t* ck = reinterpret_cast<uint32_t*>(work);  // what the groups are valued by
-  if (grouped) __syncwarp();
   if (!by_logit || sums) {
     const float inv = r.sigmoid ? 1.f : 1.f / sum;
     margin = 4e-6f * (inv + bias_max);
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (j < npl && e0 + j < E) {
-        uint32_t ckey = 0u;
-        if (key[j] != 0u) {
-          float c = r.sigmoid ? __fdividef(1.f, 1.f + __expf(-fmaxf(l[j], -80.f))) : s[j] * inv;
-          if (!by_logit) c += r.bias[e0 + j];
-          if (c > -CUDART_INF_F) ckey = order_key(c);  // not NaN either
-        }
-        if (grouped) ck[e0 + j] = ckey;
-        if (!by_logit) key[j] = ckey;
-      }
-  } else if (grouped) {
+    for (int j = 0; j < NPL; ++j) {
+      float c = r.sigmoid ? __fdividef(1.f, 1.f + __expf(-fmaxf(l[j], -80.f))) : __uint_as_float(key[j]) * inv;
+      if (!by_logit) c += b[j];
+      key[j] = l[j] > -CUDART_INF_F && c > -CUDART_INF_F ? order_key(c) : 0u;  // not NaN either
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (j < npl && e0 + j < E) ck[e0 + j] = key[j];
+    for (int j = 0; j < NPL; ++j) key[j] = l[j] > -CUDART_INF_F ? order_key(l[j]) : 0u;
   }
   auto stage_exact = [&]() {
     __syncwarp();
@@ -181,38 +183,51 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   bool staged = false;
   uint32_t kept = 0xffffffffu;
   if (grouped) {
-    __syncwarp();
-    const int per = E / r.n_group, L = lanes_per_group(r.n_group);
-    const int g = lane / L, q = lane % L, steps = (per + L - 1) / L;
-    uint32_t a = 0u, b = 0u;  // the group's two best
-    if (g < r.n_group) {
-      int x = g % steps;  // groups start at different steps, so that they meet different banks
-      for (int i = 0; i < steps; ++i) {
-        const int at = q + L * x;
-        const uint32_t v = at < per ? ck[g * per + at] : 0u;
-        b = max(b, min(a, v));
-        a = max(a, v);
-        if (++x == steps) x = 0;
+    const int G = r.n_group, per = E / G, L = lanes_per_group(G);
+    uint32_t a = 0u, a2 = 0u;  // the two best of this lane's share of a group
+    auto take = [&](uint32_t v) {
+      a2 = max(a2, min(a, v));
+      a = max(a, v);
+    };
+    const bool aligned = npl * 32 == E && 32 % G == 0;  // lane i's experts all belong to group i / L
+    if (aligned) {
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) take(key[j]);
+    } else {
+      uint32_t* all = reinterpret_cast<uint32_t*>(work);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < NPL; ++j)
+        if (j < npl && e0 + j < E) all[e0 + j] = key[j];
+      __syncwarp();
+      const int g = lane / L, q = lane % L, steps = (per + L - 1) / L;
+      if (g < G) {
+        int x = g % steps;  // groups start at different steps, so that they meet different banks
+        for (int i = 0; i < steps; ++i) {
+          const int at = q + L * x;
+          take(at < per ? all[g * per + at] : 0u);
+          if (++x == steps) x = 0;
+        }
       }
     }
     for (int m = L >> 1; m >= 1; m >>= 1) {
-      const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, m), ob = __shfl_xor_sync(0xffffffffu, b, m);
-      b = max(max(b, ob), min(a, oa));
+      const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, m), ob = __shfl_xor_sync(0xffffffffu, a2, m);
+      a2 = max(max(a2, ob), min(a, oa));
       a = max(a, oa);
     }
-    uint32_t value = q == 0 ? a : 0u;
-    if (sums && value != 0u && b != 0u) value = order_key(key_value(a) + key_value(b));
+    uint32_t value = lane / L < G ? a : 0u;  // the same in every lane of a group
+    if (sums && value != 0u && a2 != 0u) value = order_key(key_value(a) + key_value(a2));
     kept = 0u;
     float last = 0.f;
     bool close = false;
     for (int i = 0; i <= r.topk_group; ++i) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, value);
       if (m == 0u) break;
-      const int win = __ffs(__ballot_sync(0xffffffffu, value == m)) - 1;
       if (i < r.topk_group) {
-        kept |= 1u << (win / L);
+        const int g = (__ffs(__ballot_sync(0xffffffffu, value == m)) - 1) / L;
+        kept |= 1u << g;
         last = key_value(m);
-        if (lane == win) value = 0u;
+        if (lane / L == g) value = 0u;
       } else {
         close = (!by_logit || sums) && last - key_value(m) < 2.f * margin;  // sums of two choices
       }
@@ -222,58 +237,123 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       staged = true;
       kept = exact_groups(work, &r, lane);
     }
-    int gj = e0 / per, rem = e0 - gj * per;
+    if (by_logit && sums) {  // from here on by the logits
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (j < npl) {
-        if (!((kept >> (gj & 31)) & 1u)) key[j] = 0u;
+      for (int j = 0; j < NPL; ++j) key[j] = key[j] != 0u ? order_key(l[j]) : 0u;
+    }
+    if (aligned) {
+      const bool in = (kept >> (lane / L)) & 1u;
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) key[j] = in ? key[j] : 0u;
+    } else {
+      int g = e0 / per, rem = e0 - g * per;
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
         if (++rem == per) {
           rem = 0;
-          ++gj;
+          ++g;
         }
       }
+    }
   }
-  // k rounds: the best of every lane, the warp's best of those. Lower lanes hold lower ids, a lane keeps the first of equals.
-  uint32_t best = 0u;
-  int at = 0;
-  auto scan = [&]() {
-    best = 0u;
+  const int want = by_logit ? r.k : r.k + 1;  // one more to compare the last with
+  uint32_t floor_key = 0u;
+  {
+    uint32_t best = 0u;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) best = max(best, key[j]);
+    for (int got = 0; got < want;) {
+      floor_key = __reduce_max_sync(0xffffffffu, best);
+      if (floor_key == 0u) break;
+      got += __popc(__ballot_sync(0xffffffffu, best == floor_key));
+      if (best == floor_key) best = 0u;
+    }
+  }
+  if (floor_key == 0u) floor_key = 1u;  // fewer lanes than that: everything that can be chosen
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) mine += key[j] >= floor_key;
+  int before = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += v;
+  }
+  const int n = __shfl_sync(0xffffffffu, before, 31);
+  before -= mine;
+  bool close = false;
+  int rank = 32, id = -1;
+  __syncwarp();
+  if (n <= 32) {
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
-      if (j < npl && key[j] > best) {
-        best = key[j];
-        at = j;
+      if (key[j] >= floor_key) {
+        scratch->key[before] = key[j];
+        scratch->id[before] = (uint32_t)(e0 + j);
+        ++before;
       }
-  };
-  scan();
-  float last = 0.f;
-  bool close = false;
-  const int rounds = by_logit ? r.k : r.k + 1;
-  for (int i = 0; i < rounds && !close; ++i) {
-    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-    if (m == 0u) break;
-    const int win = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
-    const int e = __shfl_sync(0xffffffffu, e0 + at, win);
-    if (!by_logit) {
-      const float v = key_value(m);
-      if (i > 0) close = last - v < margin;
-      last = v;
+    __syncwarp();
+    if (lane < n) {
+      const uint32_t v = scratch->key[lane];
+      id = (int)scratch->id[lane];
+      rank = 0;
+      for (int i = 0; i < n; ++i) {
+        const uint32_t o = scratch->key[i];
+        rank += o > v || (o == v && i < lane);
+      }
     }
-    if (i < r.k && lane == i) id = e;
-    if (lane == win) {
+    if (!by_logit) {
+      const uint32_t v = lane < n ? scratch->key[lane] : 0u;
+      __syncwarp();
+      if (lane < n) scratch->key[rank] = v;
+      __syncwarp();
+      const uint32_t next = lane < n && rank + 1 < n ? scratch->key[rank + 1] : 0u;
+      close = __any_sync(0xffffffffu, lane < n && rank < r.k && next != 0u && key_value(v) - key_value(next) < margin);
+    }
+  } else {
+    // k rounds: the best of every lane, the warp's best of those; a lane keeps the first of equals
+    uint32_t best = 0u;
+    int at = 0;
+    auto scan = [&]() {
+      best = 0u;
 #pragma unroll
       for (int j = 0; j < NPL; ++j)
-        if (j == at) key[j] = 0u;
-      scan();
+        if (key[j] > best) {
+          best = key[j];
+          at = j;
+        }
+    };
+    scan();
+    float last = 0.f;
+    for (int i = 0; i < want && !close; ++i) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+      if (m == 0u) break;
+      const int win = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
+      const int e = __shfl_sync(0xffffffffu, e0 + at, win);
+      if (!by_logit) {
+        const float v = key_value(m);
+        if (i > 0) close = last - v < margin;
+        last = v;
+      }
+      if (i < r.k && lane == i) id = e;
+      if (lane == win) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+          if (j == at) key[j] = 0u;
+        scan();
+      }
     }
+    rank = lane;
   }
   if (close) {
     if (!staged) stage_exact();
     id = exact_rank(work, &r, kept, lane);
+    rank = lane;
   }
-  if (lane >= r.k) id = -1;
+  const bool chosen = id >= 0 && rank < r.k;
   float w = 0.f;
-  if (id >= 0) {
+  if (chosen) {
     const float v = logit(id);
     w = r.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top) / sum;
   }
@@ -283,7 +363,9 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
     for (int m = 16; m >= 1; m >>= 1) all += __shfl_xor_sync(0xffffffffu, all, m);
     w = w / (all + 1e-20f);
   }
-  weight = w * r.scale;
+  if (chosen) write(rank, id, w * r.scale);
+  const int found = __popc(__ballot_sync(0xffffffffu, chosen));
+  if (lane >= found && lane < r.k) write(lane, -1, 0.f);
 }
 
 }  // namespace pm
