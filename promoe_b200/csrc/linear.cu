@@ -29,6 +29,9 @@ constexpr int kTcThreads = (4 + kEpiWarps) * 32;
 constexpr int kWBytes = 128 * 128;  // a CTA's 128 weight rows of a k step
 constexpr int kMaxStages = 12;
 constexpr int kSmemMost = 232448;
+// k of one accumulator of float32 outputs. The tensor cores cut their running sums off where float32 ends, which shrinks a sum by
+// about 2^-24 of itself per addition of 16 k: 2.1e-6 for K = 2048 in one accumulator, TODO in four.
+constexpr int kPromoteK = 512;
 
 struct LinearTc {
   void* y;
@@ -36,8 +39,10 @@ struct LinearTc {
   int64_t ldy, ldr;
   int32_t M, N, k_tiles, act, bias_type, f16;
   int32_t width, tok_tiles, w_tiles;  // token columns of a tile; tiles
-  int32_t stage_bytes, n_stages, ring_bytes;
-  int32_t split, tmem_cols;
+  int32_t atoms, stage_bytes, n_stages;  // 64-k atoms of a step; k_tiles counts steps
+  int32_t chunk;                         // steps that one accumulator takes
+  int32_t split, part_offset, shared_bytes;  // CTAs (pairs) on a tile; their partial sums behind the ring; all of these bytes
+  int32_t tmem_cols;
   int32_t* err;
 };
 
@@ -103,25 +108,56 @@ __device__ __forceinline__ void tile_at(const LinearTc& a, int tile, int& wt, in
   wt = band * kBand + in - tt * high;
 }
 
+// C neighbouring tokens from token m on of weight row n (one row per lane), `left` of them inside y: bias, activation,
+// residual, rounding, store.
+template <class OT, int C>
+__device__ __forceinline__ void finish(const LinearTc& a, float (&o)[C], float bias, int64_t m, int n, int left) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] += bias;
+  activate_all(o, a.act);
+  const OT* src = static_cast<const OT*>(a.res) + m * a.ldr + n;
+  OT* dst = static_cast<OT*>(a.y) + m * a.ldy + n;
+  if (__all_sync(0xffffffffu, left >= C)) {
+    if (a.res != nullptr) {
+      OT r[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) r[c] = src[c * a.ldr];
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] += to_float<OT>(r[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) dst[c * a.ldy] = from_float<OT>(o[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (c < left) {
+        float v = o[c];
+        if (a.res != nullptr) v += to_float<OT>(src[c * a.ldr]);
+        dst[c * a.ldy] = from_float<OT>(v);
+      }
+  }
+}
+
 template <int CG, class OT>
 __global__ void __launch_bounds__(kTcThreads, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                  const __grid_constant__ LinearTc a) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  LinShared& sh = *reinterpret_cast<LinShared*>(stages + a.ring_bytes);
+  LinShared& sh = *reinterpret_cast<LinShared*>(stages + a.shared_bytes);
+  constexpr bool kPromote = sizeof(OT) == 4;  // float32 outputs: accumulators of a.chunk steps, added up in registers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int per_tile = CG == 2 ? 2 : a.split;  // CTAs on one tile
+  const uint32_t cta = cluster_rank(), rank = CG == 2 ? cta & 1 : 0, part_rank = CG == 2 ? cta >> 1 : cta;
+  const int per_tile = CG * a.split;
   const int first = blockIdx.x / per_tile, step = gridDim.x / per_tile;
   const int n_tiles = a.w_tiles * a.tok_tiles, n_stages = a.n_stages;
-  const bool split = CG == 1 && a.split > 1;
-  const int k0 = split ? (int)((long long)a.k_tiles * rank / a.split) : 0;
-  const int k1 = split ? (int)((long long)a.k_tiles * (rank + 1) / a.split) : a.k_tiles;
+  const bool split = a.split > 1;
+  const int k0 = split ? (int)((long long)a.k_tiles * part_rank / a.split) : 0;
+  const int k1 = split ? (int)((long long)a.k_tiles * (part_rank + 1) / a.split) : a.k_tiles;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < n_stages; ++s) {
-      mbar_init(&sh.full[s], 1);
+      mbar_init(&sh.full[s], 2);  // the two producers
       mbar_init(&sh.empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -138,39 +174,37 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   tc_fence_before();
   __syncthreads();
   if (CG == 2) cluster_sync_diverged();
+  else if (split) cluster_arrive_diverged();  // waited for before the partial sums are sent
   tc_fence_after();
   const uint32_t tmem_base = sh.tmem_base;
   const uint32_t acc_cols = a.tmem_cols / 2;  // distance of the two accumulators
   let_successor_start();
   wait_for_predecessor();
 
-  if (warp == 0 && lane == 0) {
-    // ---- producer: 128 weight rows and this CTA's share of the token rows ----------------------------
+  const uint32_t full0 = smem_u32(&sh.full[0]), empty0 = smem_u32(&sh.empty[0]), stage0 = smem_u32(stages);
+  const int lead = CG == 2 ? (int)(cta & ~1u) : 0;  // the pair's first CTA
+  if ((warp == 0 || warp == 3) && lane == 0) {
+    // ---- producers: one thread for this CTA's 128 weight rows, one for its share of the token rows ------------------
+    const bool tokens = warp == 3;
     const int rows = a.width / CG;
+    const uint32_t bytes = CG * a.atoms * (tokens ? (uint32_t)rows * 128 : (uint32_t)kWBytes), atom_bytes = kWBytes + rows * 128;
+    const CUtensorMap* map = tokens ? &map_x : &map_w;
+    const uint32_t dst0 = stage0 + (tokens ? kWBytes : 0), full_of_pair = CG == 2 ? map_to_rank(full0, lead) : full0;
     int at = 0, steps = 0;
     uint32_t turn = 0;
     bool ok = true;
     for (int tile = first; tile < n_tiles && ok; tile += step) {
       int wt, tt;
       tile_at(a, tile, wt, tt);
-      const int w_row = wt * 128 * CG + (CG == 2 ? (int)rank * 128 : 0);
-      const int x_row = tt * a.width + (CG == 2 ? (int)rank * rows : 0);
+      const int row = tokens ? tt * a.width + (int)rank * rows : wt * 128 * CG + (int)rank * 128;
       for (int kt = k0; kt < k1; ++kt, ++steps) {
-        if (turn > 0 && !mbar_wait(&sh.empty[at], (turn - 1) & 1, &sh.abort)) {
+        if (turn > 0 && !mbar_wait(empty0 + at * 8, (turn - 1) & 1, &sh.abort)) {
           ok = false;
           break;
         }
-        unsigned char* dst = stages + (size_t)at * a.stage_bytes;
-        if (CG == 2) {
-          if (rank == 0) mbar_arrive_expect_tx(&sh.full[at], 2 * a.stage_bytes);
-          const uint32_t bar = map_to_rank(smem_u32(&sh.full[at]), 0);
-          tma_load_2d(dst, &map_w, bar, kt * 64, w_row);
-          tma_load_2d(dst + kWBytes, &map_x, bar, kt * 64, x_row);
-        } else {
-          mbar_arrive_expect_tx(&sh.full[at], a.stage_bytes);
-          tma_load_2d_single(dst, &map_w, &sh.full[at], kt * 64, w_row);
-          tma_load_2d_single(dst + kWBytes, &map_x, &sh.full[at], kt * 64, x_row);
-        }
+        if (rank == 0) mbar_arrive_expect_tx(full0 + at * 8, bytes);
+        for (int i = 0; i < a.atoms; ++i)
+          tma_load_2d_at<CG>(dst0 + at * a.stage_bytes + i * atom_bytes, map, full_of_pair + at * 8, (kt * a.atoms + i) * 64, row);
         if (++at == n_stages) {
           at = 0;
           ++turn;
@@ -181,131 +215,154 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     for (int k = max(0, steps - n_stages); k < steps && ok; ++k)
       ok = mbar_wait(&sh.empty[k % n_stages], (k / n_stages) & 1, &sh.abort);
     if (!ok) sh.abort = 1;
-  } else if (warp == 1 && lane == 0 && (CG == 1 || rank == 0)) {
+  } else if (warp == 1 && lane == 0 && rank == 0) {
     // ---- MMA issuer ----------------------------------------------------------------------------------
     const uint32_t idesc = a.f16 ? umma_idesc_f16(128 * CG, a.width) : umma_idesc_bf16(128 * CG, a.width);
+    const uint64_t desc0 = umma_desc_k_sw128(stage0);
+    const uint32_t atom16 = (uint32_t)(kWBytes + a.width / CG * 128) >> 4;
+    const uint16_t both = (uint16_t)(3u << lead);
     int at = 0, it = 0;
     uint32_t turn = 0;
     bool ok = true;
-    for (int tile = first; tile < n_tiles && ok; tile += step, ++it) {
-      const int acc = it & 1;
-      if (it >= 2 && !mbar_wait(&sh.acc_empty[acc], ((it >> 1) - 1) & 1, &sh.abort)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t d = tmem_base + (uint32_t)acc * acc_cols;
-      for (int kt = k0; kt < k1; ++kt) {
-        if (!mbar_wait(&sh.full[at], turn & 1, &sh.abort)) {
+    for (int tile = first; tile < n_tiles && ok; tile += step)
+      for (int kc = k0; kc < k1 && ok; kc += a.chunk, ++it) {
+        const int acc = it & 1, end = min(k1, kc + a.chunk);
+        if (it >= 2 && !mbar_wait(&sh.acc_empty[acc], ((it >> 1) - 1) & 1, &sh.abort)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t addr = smem_u32(stages + (size_t)at * a.stage_bytes);
+        const uint32_t d = tmem_base + (uint32_t)acc * acc_cols;
+        uint32_t more = 0;
+        for (int kt = kc; kt < end; ++kt) {
+          if (!mbar_wait(full0 + at * 8, turn & 1, &sh.abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint64_t da = desc0 + (uint32_t)(at * (a.stage_bytes >> 4));
+          for (int i = 0; i < a.atoms; ++i, da += atom16) {
+            const uint64_t db = da + (kWBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // 16 k = 32 bytes inside the swizzled row
-          const uint64_t da = umma_desc_k_sw128(addr + k * 32), db = umma_desc_k_sw128(addr + kWBytes + k * 32);
-          const uint32_t more = (kt > k0 || k > 0) ? 1u : 0u;
-          if (CG == 2) umma_bf16(d, da, db, idesc, more);
-          else umma_single(d, da, db, idesc, more);
+            for (int k = 0; k < 4; ++k) {  // 16 k = 32 bytes inside the swizzled row
+              umma_at<CG>(d, da + 2 * k, db + 2 * k, idesc, more);
+              more = 1;
+            }
+          }
+          umma_commit_at<CG>(empty0 + at * 8, both);
+          if (++at == n_stages) {
+            at = 0;
+            ++turn;
+          }
         }
-        if (CG == 2) umma_commit_pair(&sh.empty[at]);
-        else umma_commit_single(&sh.empty[at]);
-        if (++at == n_stages) {
-          at = 0;
-          ++turn;
-        }
+        if (ok) umma_commit_at<CG>(smem_u32(&sh.acc_full[acc]), both);
       }
-      if (ok) {
-        if (CG == 2) umma_commit_pair(&sh.acc_full[acc]);
-        else umma_commit_single(&sh.acc_full[acc]);
-      }
-    }
     if (!ok) sh.abort = 1;
   } else if (warp >= 4) {
     // ---- epilogue: warp w drains accumulator rows 32w .. 32w+31, two warps of a quadrant share the columns ------
     const int w = warp & 3, half = (warp - 4) >> 2;
     const float nan = __int_as_float(0x7fffffff);
+    const uint32_t acc_free = CG == 2 ? map_to_rank(smem_u32(&sh.acc_empty[0]), lead) : smem_u32(&sh.acc_empty[0]);
     int it = 0;
     bool ok = true;
-    for (int tile = first; tile < n_tiles; tile += step, ++it) {
+    for (int tile = first; tile < n_tiles; tile += step) {
       int wt, tt;
       tile_at(a, tile, wt, tt);
-      const int acc = it & 1;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (it >> 1) & 1, &sh.abort));
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + (uint32_t)acc * acc_cols + ((uint32_t)(32 * w) << 16);
-      const int n = wt * 128 * CG + (CG == 2 ? (int)rank * 128 : 0) + 32 * w + lane;
+      const int n = (wt * CG + (int)rank) * 128 + 32 * w + lane;
       const int m0 = tt * a.width, cols = min(a.width, a.M - m0);
-      if (split) {
-        // partial sums to shared memory (the ring is empty now), column by column
-        float* part = reinterpret_cast<float*>(stages);
-        for (int c0 = half * 32; c0 < cols; c0 += 64) {
-          uint32_t v[32];
-          tmem_ld32(taddr + c0, v);
-          tmem_ld_wait();
+      const float b = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
+      auto give = [&](float (&o)[32], int c0) {
+        if (!ok) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = nan;
+        }
+        if (!split) {
+          finish<OT, 32>(a, o, b, m0 + c0, n, n < a.N ? cols - c0 : 0);
+        } else {
+          // column c0 + c to the CTA that finishes it, which keeps [source][its columns][128 rows]
+          const int per = (a.width + a.split - 1) / a.split;
+          const uint32_t mine = stage0 + a.part_offset + 4u * (uint32_t)((int)part_rank * per * 128 + 32 * w + lane);
+          int owner = c0 / per, at = c0 - owner * per;
+          uint32_t dst = map_to_rank(mine, CG * owner + rank) + 512u * (uint32_t)at;
 #pragma unroll
           for (int c = 0; c < 32; ++c)
-            if (c0 + c < cols) part[(c0 + c) * 128 + 32 * w + lane] = ok ? __uint_as_float(v[c]) : nan;
+            if (c0 + c < cols) {
+              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(o[c]) : "memory");
+              dst += 512;
+              if (++at == per) {
+                at = 0;
+                ++owner;
+                if (owner < a.split) dst = map_to_rank(mine, CG * owner + rank);
+              }
+            }
         }
-        continue;
+      };
+      if (CG == 1 && split) cluster_wait_diverged();
+      float sums[kPromote ? 2 : 1][32];
+      for (int kc = k0; kc < k1; kc += a.chunk, ++it) {
+        const int acc = it & 1;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (it >> 1) & 1, &sh.abort));
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + (uint32_t)acc * acc_cols + ((uint32_t)(32 * w) << 16);
+        if (kPromote) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // at most 128 columns
+            const int c0 = half * 32 + 64 * i;
+            if (c0 < cols) {
+              uint32_t v[32];
+              tmem_ld32(taddr + c0, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 32; ++c) sums[kPromote ? i : 0][c] = kc == k0 ? __uint_as_float(v[c]) : sums[kPromote ? i : 0][c] + __uint_as_float(v[c]);
+            }
+          }
+        } else {
+          for (int c0 = half * 32; c0 < cols; c0 += 64) {
+            uint32_t v[32];
+            tmem_ld32(taddr + c0, v);
+            tmem_ld_wait();
+            float o[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __uint_as_float(v[c]);
+            give(o, c0);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) mbar_arrive_cluster(acc_free + acc * 8);
+          else mbar_arrive(acc_free + acc * 8);
+        }
       }
-      const float b = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
-      for (int c0 = half * 32; c0 < cols; c0 += 64) {
-        uint32_t v[32];
-        tmem_ld32(taddr + c0, v);
-        const int left = n < a.N ? cols - c0 : 0;
-        OT r[32];
-        if (a.res != nullptr) {
-          const OT* src = static_cast<const OT*>(a.res) + (int64_t)(m0 + c0) * a.ldr + n;
+      if (kPromote) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) r[c] = c < left ? src[c * a.ldr] : from_float<OT>(0.f);
-        }
-        tmem_ld_wait();
-        float o[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = ok ? __uint_as_float(v[c]) + b : nan;
-        activate_all(o, a.act);
-        if (a.res != nullptr) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] += to_float<OT>(r[c]);
-        }
-        OT* dst = static_cast<OT*>(a.y) + (int64_t)(m0 + c0) * a.ldy + n;
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
-          if (c < left) dst[c * a.ldy] = from_float<OT>(o[c]);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&sh.acc_empty[acc]), 0));
-        else mbar_arrive(smem_u32(&sh.acc_empty[acc]));
+        for (int i = 0; i < 2; ++i)
+          if (half * 32 + 64 * i < cols) give(sums[kPromote ? i : 0], half * 32 + 64 * i);
       }
     }
     if (!ok && lane == 0) sh.abort = 1;
   }
   __syncwarp();
   if (split) {
+    if (CG == 1 && warp < 4) cluster_wait_diverged();
     __syncthreads();
-    cluster_sync_diverged();  // every rank's partial sums are in place
+    cluster_sync_diverged();  // every CTA's partial sums have arrived where they are finished
     if (warp >= 4) {
       int wt, tt;
       tile_at(a, first, wt, tt);
-      const int m0 = tt * a.width, cols = min(a.width, a.M - m0);
-      const uint32_t part = smem_u32(stages);
-      for (int task = (warp - 4) + kEpiWarps * (int)rank; task < cols * 4; task += kEpiWarps * a.split) {
-        const int c = task >> 2, row = (task & 3) * 32 + lane, n = wt * 128 + row;
-        float v = 0.f;
+      const int per = (a.width + a.split - 1) / a.split, c_first = (int)part_rank * per;
+      const int m0 = tt * a.width, mine = min(per, min(a.width, a.M - m0) - c_first);
+      const float* part = reinterpret_cast<const float*>(stages + a.part_offset);
+      const int row = (warp & 3) * 32 + lane, n = (wt * CG + (int)rank) * 128 + row;
+      const float b = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
+      for (int c0 = ((warp - 4) >> 2) * 8; c0 < mine; c0 += 16) {
+        float o[8] = {};
         for (int r = 0; r < a.split; ++r) {
-          float p;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(map_to_rank(part, r) + 4u * (uint32_t)(c * 128 + row)));
-          v += p;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c0 + c < mine) o[c] += part[(r * per + c0 + c) * 128 + row];
         }
-        if (n < a.N) {
-          v = activate_one(v + load_bias(a.bias, a.bias_type, n), a.act);
-          if (a.res != nullptr) v += to_float<OT>(static_cast<const OT*>(a.res)[(int64_t)(m0 + c) * a.ldr + n]);
-          static_cast<OT*>(a.y)[(int64_t)(m0 + c) * a.ldy + n] = from_float<OT>(v);
-        }
+        finish<OT, 8>(a, o, b, m0 + c_first + c0, n, n < a.N ? mine - c0 : 0);
       }
     }
   }
@@ -424,39 +481,61 @@ cudaError_t launch_plain(const LinearCall& a, cudaStream_t s) {
 
 // ---- launch plan ------------------------------------------------------------------------------------------
 struct LinearShape {
-  int cg = 1, split = 1, tok_tiles = 1, width = 16;
+  int cg = 1, split = 1, tok_tiles = 1, width = 16, atoms = 1;
 };
 
-// Estimated cycles of a shape. A k step of 64 takes 2 cycles per token column on the tensor cores, and its operands
-// come from L2 at about 48 bytes per cycle and SM; the rest is what a tile and a launch cost besides.
-double shape_cost(const LinearShape& c, int N, int k_tiles, int sms) {
-  const int w_tiles = (N + 128 * c.cg - 1) / (128 * c.cg), units = sms / c.cg;
-  const long long ctas = (long long)w_tiles * c.tok_tiles * c.split;
-  const long long waves = (ctas + units - 1) / units;
-  const double step = std::max(2.0 * c.width, (kWBytes + c.width / c.cg * 128) / 48.0);
-  const int steps = (k_tiles + c.split - 1) / c.split;
-  return waves * (steps * step + 600.0 + (c.split > 1 ? 1200.0 + 8.0 * c.width : 0.0)) + 2.0 * c.width;
+// Narrow steps take two atoms of 64 k: waits and commits cost 75 ns per step.
+int atoms_for(int cg, int width) { return kWBytes + width / cg * 128 <= 24 * 1024 ? 2 : 1; }
+
+// Estimated ns of a shape, from measured slopes: an atom's MMAs take 2 cycles per token column and 200 ns at least (the weight
+// rows' way from shared memory), its operands come at up to 120 bytes per ns and CTA and 12300 over all of them from L2, at
+// 6500 from HBM; a launch and the last tile's epilogue cost 3.5 us + 8 ns per column, joining partial sums 1 us + 30 ns per column.
+// cap: clusters of cg * split CTAs that the GPU holds at once.
+double shape_cost(const LinearShape& c, int M, int N, int K, int cap) {
+  const int per = c.cg * c.split, k_atoms = (K + 63) / 64;
+  const long long tiles = (long long)((N + 128 * c.cg - 1) / (128 * c.cg)) * c.tok_tiles;
+  const double active = (double)std::min<long long>(tiles, cap) * per, bytes = kWBytes + c.width / c.cg * 128;
+  const double mma = std::max(200.0, 2.0 * c.width / 1.9) + 75.0 / c.atoms;
+  const double atom = std::max({mma, bytes / 120.0, bytes * active / 12300.0});
+  const double stream = (double)((tiles + cap - 1) / cap) * ((k_atoms + c.split - 1) / c.split) * atom;
+  const double fixed = 3500.0 + 8.0 * c.width + (c.split > 1 ? 1000.0 + 30.0 * c.width : 0.0);
+  return std::max(stream, ((double)N * K + (double)M * K) * 2 / 6500.0) + fixed;
 }
 
-LinearShape choose_shape(int M, int N, int k_tiles, int sms) {
+constexpr int kMaxCluster = 8;
+
+// Clusters of each size that the current device holds, one CTA per SM.
+cudaError_t cluster_capacity(int dev, int (&cap)[kMaxCluster + 1]);
+
+struct PlanKey {
+  int M, N, K, promote, dev;
+  bool operator==(const PlanKey& o) const { return M == o.M && N == o.N && K == o.K && promote == o.promote && dev == o.dev; }
+};
+
+LinearShape choose_shape(int M, int N, int K, bool promote, const int (&cap)[kMaxCluster + 1]) {
   LinearShape best;
   double cost = 0;
+  const int most = promote ? 128 : 256;  // float32 outputs keep their sums in registers
   for (int cg = 1; cg <= 2; ++cg) {
-    const int grain = 16 * cg, least = (M + 255) / 256;
-    for (int t = least; t <= least + 3; ++t)
-      for (int split = 1; split <= (cg == 1 ? 8 : 1); ++split) {
-        if (split > k_tiles) break;
-        LinearShape c;
-        c.cg = cg;
-        c.split = split;
-        c.width = ((M + t - 1) / t + grain - 1) / grain * grain;
-        c.tok_tiles = (M + c.width - 1) / c.width;
-        const double x = shape_cost(c, N, k_tiles, sms);
+    const int grain = 16 * cg, least = (M + most - 1) / most;
+    for (int t = least; t <= least + 8; ++t) {
+      LinearShape c;
+      c.cg = cg;
+      c.width = ((M + t - 1) / t + grain - 1) / grain * grain;
+      c.tok_tiles = (M + c.width - 1) / c.width;
+      c.atoms = atoms_for(cg, c.width);
+      const int steps = (K + 64 * c.atoms - 1) / (64 * c.atoms);
+      for (c.split = 1; c.split * cg <= kMaxCluster && c.split <= steps; ++c.split) {
+        // shared tiles: one round of clusters, and partial sums that leave the ring enough room
+        if (c.split > 1 && (c.width > 128 || (long long)((N + 128 * cg - 1) / (128 * cg)) * c.tok_tiles > cap[cg * c.split])) break;
+        const double x = shape_cost(c, M, N, K, cap[cg * c.split]);
         if (cost == 0 || x < cost) {
           cost = x;
           best = c;
         }
       }
+      if (c.width == grain) break;
+    }
   }
   return best;
 }
@@ -491,6 +570,33 @@ cudaError_t launch_tc_for(int out_type, const CUtensorMap& map_w, const CUtensor
   return launch_tc<CG, __half>(map_w, map_x, t, grid, cluster, smem, s);
 }
 
+cudaError_t cluster_capacity(int dev, int (&cap)[kMaxCluster + 1]) {
+  static std::atomic<int> known[64][kMaxCluster + 1];
+  auto kern = linear_tc_kernel<1, __nv_bfloat16>;
+  for (int c = 1; c <= kMaxCluster; ++c) {
+    const bool keep = dev >= 0 && dev < 64;
+    int n = keep ? known[dev][c].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+      if (e != cudaSuccess) return e;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = 1024 * c;
+      cfg.blockDim = kTcThreads;
+      cfg.dynamicSmemBytes = kSmemMost;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim = {(unsigned)c, 1, 1};
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if ((e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) != cudaSuccess) return e;
+      if (n <= 0) return cudaErrorNotSupported;
+      if (keep) known[dev][c].store(n, std::memory_order_relaxed);
+    }
+    cap[c] = n;
+  }
+  return cudaSuccess;
+}
+
 bool tma_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld < ((int64_t)1 << 38); }
 
 }  // namespace
@@ -500,24 +606,36 @@ int launch_linear(const LinearCall& a, cudaStream_t s) {
     PM_CUDA(a.type == PM_BF16 ? launch_plain<__nv_bfloat16>(a, s) : launch_plain<__half>(a, s));
     return PM_OK;
   }
-  int dev = 0, sms = 0;
+  int dev = 0, cap[kMaxCluster + 1];
   PM_CUDA(cudaGetDevice(&dev));
-  PM_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const int k_tiles = (a.K + 63) / 64;
-  const LinearShape c = choose_shape(a.M, a.N, k_tiles, sms);
+  PM_CUDA(cluster_capacity(dev, cap));
+  // The shape follows from the sizes alone; a thread remembers the last few.
+  const bool promote = a.out_type == PM_F32;
+  const PlanKey key{a.M, a.N, a.K, promote, dev};
+  struct Plan {
+    PlanKey key;
+    LinearShape shape;
+  };
+  static thread_local Plan plans[16] = {};
+  Plan& plan = plans[(unsigned)(a.M * 31 + a.N * 7 + a.K) % 16];
+  if (!(plan.key == key)) plan = Plan{key, choose_shape(a.M, a.N, a.K, promote, cap)};
+  const LinearShape& c = plan.shape;
   LinearTc t{};
   t.y = a.y; t.res = a.res; t.bias = a.bias;
   t.ldy = a.ldy; t.ldr = a.ldr;
-  t.M = a.M; t.N = a.N; t.k_tiles = k_tiles; t.act = a.act; t.bias_type = a.bias_type; t.f16 = a.type == PM_F16;
+  t.M = a.M; t.N = a.N; t.act = a.act; t.bias_type = a.bias_type; t.f16 = a.type == PM_F16;
   t.width = c.width; t.tok_tiles = c.tok_tiles; t.w_tiles = (a.N + 128 * c.cg - 1) / (128 * c.cg);
+  t.atoms = c.atoms; t.k_tiles = (a.K + 64 * c.atoms - 1) / (64 * c.atoms);
+  t.chunk = promote ? kPromoteK / 64 / c.atoms : t.k_tiles;
   t.split = c.split; t.err = a.err;
-  t.stage_bytes = kWBytes + c.width / c.cg * 128;
-  const int room = kSmemMost - 1024 - (int)sizeof(LinShared), steps = (k_tiles + c.split - 1) / c.split;
-  const long long n_tiles = (long long)t.w_tiles * t.tok_tiles, units = sms / c.cg;
+  t.stage_bytes = c.atoms * (kWBytes + c.width / c.cg * 128);
+  const int part_bytes = c.split > 1 ? (c.width + c.split - 1) / c.split * c.split * 512 : 0;
+  const int room = kSmemMost - 1024 - (int)sizeof(LinShared) - part_bytes, steps = (t.k_tiles + c.split - 1) / c.split;
+  const long long n_tiles = (long long)t.w_tiles * t.tok_tiles, units = cap[c.cg * c.split];
   const long long tiles_each = c.split > 1 ? 1 : (n_tiles + units - 1) / units;
   t.n_stages = (int)std::min<long long>(std::min(kMaxStages, room / t.stage_bytes), steps * tiles_each);
-  t.ring_bytes = t.stage_bytes * t.n_stages;
-  if (c.split > 1) t.ring_bytes = std::max(t.ring_bytes, c.width * 512);
+  t.part_offset = t.stage_bytes * t.n_stages;
+  t.shared_bytes = t.part_offset + part_bytes;
   t.tmem_cols = 64;  // two accumulators, each at a multiple of 32 columns; the allocation is a power of two
   while (t.tmem_cols < 2 * c.width) t.tmem_cols *= 2;
   CUtensorMap map_w, map_x;
@@ -527,10 +645,10 @@ int launch_linear(const LinearCall& a, cudaStream_t s) {
   if (rc != PM_OK) return rc;
   // Beside the grouped FFN's kernel, which takes all tensor memory after it has let its successor in, no block of this one
   // may start (each would wait for the other): 64 KB do not fit there. Pairs allocate together, so only one per SM.
-  const size_t smem = std::max<size_t>(1024 + t.ring_bytes + sizeof(LinShared), (c.cg == 2 ? 120 : 64) * 1024);
-  const int cluster = c.cg == 2 ? 2 : c.split;
-  if (n_tiles * c.split > 0x7fffffffll) return fail(PM_ERR_INVALID, "linear: too many tiles");
-  const long long grid = c.split > 1 ? n_tiles * c.split : std::min(n_tiles, units) * c.cg;
+  const size_t smem = std::max<size_t>(1024 + t.shared_bytes + sizeof(LinShared), (c.cg == 2 ? 120 : 64) * 1024);
+  const int cluster = c.cg * c.split;
+  if (n_tiles * cluster > 0x7fffffffll) return fail(PM_ERR_INVALID, "linear: too many tiles");
+  const long long grid = (c.split > 1 ? n_tiles : std::min(n_tiles, units)) * cluster;
   PM_CUDA(c.cg == 2 ? launch_tc_for<2>(a.out_type, map_w, map_x, t, (int)grid, cluster, smem, s)
                     : launch_tc_for<1>(a.out_type, map_w, map_x, t, (int)grid, cluster, smem, s));
   return PM_OK;
