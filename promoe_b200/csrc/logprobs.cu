@@ -3,7 +3,8 @@
 //   lse = c ln2 + ln S,  logp = l_target - lse,  H = ln S - ln2 U / S,  top: l - lse of the n largest
 // c is rounded once and used everywhere, so its rounding cancels; two logits cost two exponentials and three packed
 // float32 instructions besides the widening and the maximum. Logits are raised to a value that has no probability beside any
-// other (kLow), which keeps 0 times infinity out of U; rows whose maximum is down there are summed again.
+// other (kLow), which keeps 0 times infinity out of U; rows whose maximum is down there are summed again. (Raising only
+// once a thread has met a masked logit changed nothing.)
 //
 // A row is read by a cluster of CTAs (one where there are many rows); every thread keeps its own running maximum and
 // sums and rescales them when a batch of its values raises the maximum.
@@ -18,7 +19,8 @@
 //
 // What bounds it: long rows HBM. 4096 rows of 131072 bf16 take 166 us = 6.49 TB/s without alternatives, 194 us = 5.5 TB/s with
 // five and 211 us with twenty: the end of a row (two rankings, the noted vectors' way from L2) is latency that four CTAs per SM
-// cover in part. Short rows that end too (4096 of 2048: 12 us without alternatives, 23 with five; one warp per row instead
+// cover in part. That is at 1965 MHz; after some hundred passes the 1000 W limit takes the clock to 1680 MHz, and the same
+// passes take 197, 229 and about 250 us. Short rows that end too (4096 of 2048: 12 us without alternatives, 23 with five; one warp per row instead
 // of four changed that by less than a fifth). One row of 131072: 7 to 9 us, the chain of load, floor, sums, two cluster
 // barriers and ranking. First form, with scalar arithmetic and the lists sorted out in the loop: 281 us for 4096 rows, 11.5 for one.
 //
@@ -268,12 +270,10 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     }
   };
   if (v0 < v1) fetch(v0);
-  int64_t target = -1;  // asked for early, used at the end
-  float at_target = 0.f;
-  if (tid == 0 && rank == 0 && a.logp != nullptr) {
-    target = a.targets[row];
-    if (target >= 0 && target < a.V) at_target = widen_one(l[target]);
-  }
+  // The target's logit is asked for in two steps, each well before its result is needed.
+  int64_t target = -1;
+  T at_target{};
+  if (tid == 0 && rank == 0 && a.logp != nullptr) target = a.targets[row];
   if (tid == 0) sh.count = sh.n_hot = 0;
   __syncthreads();
   auto push = [&](Entry e) {
@@ -362,6 +362,8 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
       }
     }
   }
+
+  if (target >= 0 && target < a.V) at_target = l[target];
 
   // sums of the thread, the warp, the CTA
   Sums a0;
@@ -497,24 +499,38 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   const bool again = !(t.m > V::kLow + kFar) || t.m > 1e37f;
   if (again) {
     // A row of the type's lowest values, or one so large that c overflows: its true maximum, and everything relative to it
+    auto whole_row = [&](auto f) {
+      if (tid < head + a.V - tail0) f(widen_one(l[tid < head ? tid : tail0 + tid - head]));
+      for (int v = tid; v < n_vec; v += 4 * THREADS) {
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (v + k * THREADS < n_vec) w[k] = body[v + k * THREADS];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (v + k * THREADS < n_vec) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) f(widen_one(reinterpret_cast<const T*>(&w[k])[j]));
+          }
+      }
+    };
     float top = -CUDART_INF_F;
     bool bad = false;
-    for (int i = tid; i < a.V; i += THREADS) {
-      const float v = widen_one(l[i]);
+    whole_row([&](float v) {
       bad |= v != v;
       top = fmaxf(top, v);
-    }
+    });
     top = value_of(__reduce_max_sync(0xffffffffu, order_of(top)));
     if (lane == 0) sh.warp_sums[warp].m = top;
     bad = __syncthreads_or(bad);
     for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, sh.warp_sums[w].m);
     float s = 0.f, u = 0.f;
     if (fabsf(top) < CUDART_INF_F)
-      for (int i = tid; i < a.V; i += THREADS) {
-        const float d = (widen_one(l[i]) - top) * kLog2e, e = exp2_fast(d);
+      whole_row([&](float v) {
+        const float d = (v - top) * kLog2e, e = exp2_fast(d);
         s += e;
         u = fmaf(e, fmaxf(d, -1e4f), u);
-      }
+      });
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) {
       s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -539,7 +555,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   const double lse = dead ? CUDART_NAN : (again ? (double)t.m : (double)t.c * kLn2) + (double)log_s;
   if (lane == 0) {
     if (a.logp != nullptr) {
-      a.logp[row] = target < 0 ? 0.f : dead || target >= a.V ? CUDART_NAN_F : (float)((double)at_target - lse);
+      a.logp[row] = target < 0 ? 0.f : dead || target >= a.V ? CUDART_NAN_F : (float)((double)widen_one(at_target) - lse);
     }
     if (a.entropy != nullptr) a.entropy[row] = dead ? CUDART_NAN_F : fmaf(-(float)kLn2, t.u / t.s, log_s);
   }
