@@ -26,15 +26,7 @@ route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_c
   wait_for_predecessor();
 
   float b[NPL];
-  float bias_max = 0.f;
-  if (rule.bias != nullptr) {
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-      b[j] = j < npl && e0 + j < E ? rule.bias[e0 + j] : 0.f;
-      if (fabsf(b[j]) <= 3.402823466e38f) bias_max = fmaxf(bias_max, fabsf(b[j]));
-    }
-    bias_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bias_max)));
-  }
+  const float bias_max = load_choice_bias<NPL>(rule, npl, lane, b);
   constexpr int kVec = 16 / sizeof(T);
   float l[NPL];
   auto load = [&](int64_t t) {

@@ -21,9 +21,11 @@
 
 namespace pm {
 
-__device__ __forceinline__ uint32_t order_key(float v) {  // ascending with v; 0 is below every number
-  const uint32_t b = __float_as_uint(v + 0.f);            // -0 and 0 are the same
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// Numbers as integers in the same order; the key of -inf, kNone, stands for what cannot be chosen.
+constexpr uint32_t kNone = 0x007fffffu;
+__device__ __forceinline__ uint32_t order_key(float v) {  // not for -0
+  const uint32_t b = __float_as_uint(v);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
@@ -110,31 +112,46 @@ __device__ __noinline__ int exact_rank(double* c, const RouteRule* rule, uint32_
 
 // How the warp chooses. Lane i holds npl neighbouring experts, so lower lanes hold lower ids. The k-th largest of the lanes'
 // maxima is a floor that k experts reach, and usually few more do: those are laid out one per lane, in the order of
-// their ids, and each counts how many rank before it. Against k rounds of arg-max over all experts this is half the
-// instructions (16384 tokens of 256 experts in 8 groups, 8 of them chosen: 51.7 -> 10.4 us). Where more than 32
-// experts reach the floor (many equal logits, large k) the rounds remain.
-struct RouteScratch {  // shared memory of one warp, followed by E doubles
-  uint32_t key[33];    // candidates; then their values in rank order
-  uint32_t id[33];
+// their ids, and each counts how many rank before it. Where more than 32 experts reach the floor (many equal logits,
+// large k) there are k rounds of arg-max over all experts instead.
+struct alignas(16) RouteScratch {  // shared memory of one warp, followed by E doubles
+  uint32_t key[36];                // candidates; then their values in rank order
+  uint32_t id[36];
 };
 __host__ __device__ __forceinline__ size_t route_scratch_bytes(int E) { return sizeof(RouteScratch) + 8 * (size_t)((E + 1) / 2 * 2); }
 
-// Row of a token: experts lane * npl .. lane * npl + npl - 1 are l[0 .. npl) of this lane (-inf beyond E; npl <= NPL), and
-// their correction biases b[0 .. npl), with bias_max the largest finite |bias| (both unused without a bias).
-// logit(e) reads the row again. write(j, id, weight) is called once for each j < k, by any lane.
+__device__ __forceinline__ float fast_sigmoid(float l) {  // off by 2e-7; 0 for -inf, 1 for +inf
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + exp2f(l * -1.4426950408889634f)));
+  return y;
+}
+
+// A router's correction bias in the registers of a warp: what route_token's b holds. Returns the largest finite magnitude.
+template <int NPL>
+__device__ __forceinline__ float load_choice_bias(const RouteRule& r, int npl, int lane, float (&b)[NPL]) {
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < NPL; ++j) {
+    const int e = lane * npl + j;
+    float v = 0.f;
+    if (r.bias != nullptr && j < npl && e < r.E) v = r.bias[e];
+    if (fabsf(v) <= 3.402823466e38f) most = fmaxf(most, fabsf(v));
+    b[j] = v == v ? v : -CUDART_INF_F;  // no choice can be made with a NaN
+  }
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+}
+
+// Row of a token: experts lane * npl .. lane * npl + npl - 1 are l[0 .. npl) of this lane (-inf beyond E; npl <= NPL), b and
+// bias_max from load_choice_bias. logit(e) reads the row again. write(j, id, weight) is called once for each j < k, by any lane.
 template <int NPL, class Logit, class Write>
 __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, const RouteRule& r, const float (&b)[NPL], float bias_max,
                                             RouteScratch* scratch, int lane, const Logit& logit, const Write& write) {
   const int E = r.E, e0 = lane * npl;
   double* work = reinterpret_cast<double*>(scratch + 1);
   const bool by_logit = r.bias == nullptr, grouped = r.n_group > 1 && r.topk_group < r.n_group, sums = grouped && r.group_top2 != 0;
-  float top = -CUDART_INF_F;
   bool odd = false;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) {
-    odd |= !(l[j] <= 3.402823466e38f);  // NaN or +inf
-    top = fmaxf(top, l[j]);
-  }
+  for (int j = 0; j < NPL; ++j) odd |= !(l[j] < CUDART_INF_F);
   if (__any_sync(0xffffffffu, odd)) {
     bool dead = false;
 #pragma unroll
@@ -144,16 +161,19 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       return;
     }
   }
-  top = key_value(__reduce_max_sync(0xffffffffu, order_key(top)));
   // A float32 score is off by at most 1e-6 of the largest (the exponential's argument is off by half a step, the
   // exponential and the division by about two), a choice by that and half a step of its own.
-  float sum = 0.f, margin = 0.f;
-  uint32_t key[NPL];  // ordered choices, 0: cannot be chosen
+  float sum = 0.f, top = 0.f, margin = 0.f;
+  uint32_t key[NPL];  // ordered choices
   if (!r.sigmoid) {
-    const float base = top == -CUDART_INF_F ? 0.f : top;
+    top = -CUDART_INF_F;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) top = fmaxf(top, l[j]);
+    top = key_value(__reduce_max_sync(0xffffffffu, order_key(top)));
+    if (top == -CUDART_INF_F) top = 0.f;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-      const float e = __expf(l[j] - base);
+      const float e = __expf(l[j] - top);
       key[j] = __float_as_uint(e);
       sum += e;
     }
@@ -163,15 +183,18 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   if (!by_logit || sums) {
     const float inv = r.sigmoid ? 1.f : 1.f / sum;
     margin = 4e-6f * (inv + bias_max);
+    if (r.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-      float c = r.sigmoid ? __fdividef(1.f, 1.f + __expf(-fmaxf(l[j], -80.f))) : __uint_as_float(key[j]) * inv;
-      if (!by_logit) c += b[j];
-      key[j] = l[j] > -CUDART_INF_F && c > -CUDART_INF_F ? order_key(c) : 0u;  // not NaN either
+      for (int j = 0; j < NPL; ++j) key[j] = __float_as_uint(fast_sigmoid(l[j]) + b[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) key[j] = __float_as_uint(fmaf(__uint_as_float(key[j]), inv, b[j]));
     }
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) key[j] = l[j] > -CUDART_INF_F ? order_key(__uint_as_float(key[j])) : kNone;
   } else {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) key[j] = l[j] > -CUDART_INF_F ? order_key(l[j]) : 0u;
+    for (int j = 0; j < NPL; ++j) key[j] = order_key(l[j] + 0.f);
   }
   auto stage_exact = [&]() {
     __syncwarp();
@@ -184,12 +207,13 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   uint32_t kept = 0xffffffffu;
   if (grouped) {
     const int G = r.n_group, per = E / G, L = lanes_per_group(G);
-    uint32_t a = 0u, a2 = 0u;  // the two best of this lane's share of a group
+    const bool aligned = npl * 32 == E && 32 % G == 0;  // lane i's experts all belong to group i / L
+    const int group = lane / L;                         // this lane's share of the valuation, and with `aligned` its experts'
+    uint32_t a = kNone, a2 = kNone;                     // the two best of it
     auto take = [&](uint32_t v) {
       a2 = max(a2, min(a, v));
       a = max(a, v);
     };
-    const bool aligned = npl * 32 == E && 32 % G == 0;  // lane i's experts all belong to group i / L
     if (aligned) {
 #pragma unroll
       for (int j = 0; j < NPL; ++j) take(key[j]);
@@ -200,12 +224,12 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       for (int j = 0; j < NPL; ++j)
         if (j < npl && e0 + j < E) all[e0 + j] = key[j];
       __syncwarp();
-      const int g = lane / L, q = lane % L, steps = (per + L - 1) / L;
-      if (g < G) {
-        int x = g % steps;  // groups start at different steps, so that they meet different banks
+      const int q = lane % L, steps = (per + L - 1) / L;
+      if (group < G) {
+        int x = group % steps;  // groups start at different steps, so that they meet different banks
         for (int i = 0; i < steps; ++i) {
           const int at = q + L * x;
-          take(at < per ? all[g * per + at] : 0u);
+          take(at < per ? all[group * per + at] : kNone);
           if (++x == steps) x = 0;
         }
       }
@@ -215,41 +239,46 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       a2 = max(max(a2, ob), min(a, oa));
       a = max(a, oa);
     }
-    uint32_t value = lane / L < G ? a : 0u;  // the same in every lane of a group
-    if (sums && value != 0u && a2 != 0u) value = order_key(key_value(a) + key_value(a2));
-    kept = 0u;
+    uint32_t value = a;  // the same in every lane of a group; kNone in lanes without one
+    if (sums && a2 != kNone) value = order_key(key_value(a) + key_value(a2) + 0.f);
+    bool in = false;
     float last = 0.f;
-    bool close = false;
-    for (int i = 0; i <= r.topk_group; ++i) {
+    for (int i = 0; i < r.topk_group; ++i) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, value);
-      if (m == 0u) break;
-      if (i < r.topk_group) {
-        const int g = (__ffs(__ballot_sync(0xffffffffu, value == m)) - 1) / L;
-        kept |= 1u << g;
-        last = key_value(m);
-        if (lane / L == g) value = 0u;
-      } else {
-        close = (!by_logit || sums) && last - key_value(m) < 2.f * margin;  // sums of two choices
-      }
+      if (m == kNone) break;
+      bool mine = value == m;
+      const unsigned who = __ballot_sync(0xffffffffu, mine);
+      if (__popc(who) != L) mine = group == (__ffs(who) - 1) / L;  // equal groups: the lowest
+      in |= mine;
+      if (mine) value = kNone;
+      last = key_value(m);
+    }
+    kept = __ballot_sync(0xffffffffu, in);
+    const uint32_t next = __reduce_max_sync(0xffffffffu, value);
+    const bool close = (!by_logit || sums) && next != kNone && last - key_value(next) < 2.f * margin;  // sums of two choices
+    if (L > 1) {  // from bits of lanes to bits of groups
+      uint32_t of_groups = 0u;
+      for (int g = 0; g < G; ++g) of_groups |= ((kept >> (g * L)) & 1u) << g;
+      kept = of_groups;
     }
     if (close) {
       stage_exact();
       staged = true;
       kept = exact_groups(work, &r, lane);
+      in = (kept >> group) & 1u;
     }
     if (by_logit && sums) {  // from here on by the logits
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = key[j] != 0u ? order_key(l[j]) : 0u;
+      for (int j = 0; j < NPL; ++j) key[j] = order_key(l[j] + 0.f);
     }
     if (aligned) {
-      const bool in = (kept >> (lane / L)) & 1u;
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = in ? key[j] : 0u;
+      for (int j = 0; j < NPL; ++j) key[j] = in ? key[j] : kNone;
     } else {
       int g = e0 / per, rem = e0 - g * per;
 #pragma unroll
       for (int j = 0; j < NPL; ++j) {
-        if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
+        if (!((kept >> (g & 31)) & 1u)) key[j] = kNone;
         if (++rem == per) {
           rem = 0;
           ++g;
@@ -258,19 +287,18 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
     }
   }
   const int want = by_logit ? r.k : r.k + 1;  // one more to compare the last with
-  uint32_t floor_key = 0u;
+  uint32_t floor_key = kNone;
   {
-    uint32_t best = 0u;
+    uint32_t best = kNone;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) best = max(best, key[j]);
-    for (int got = 0; got < want;) {
+    for (int i = 0; i < want; ++i) {  // equal maxima leave together, which only lowers the floor
       floor_key = __reduce_max_sync(0xffffffffu, best);
-      if (floor_key == 0u) break;
-      got += __popc(__ballot_sync(0xffffffffu, best == floor_key));
-      if (best == floor_key) best = 0u;
+      if (floor_key == kNone) break;
+      if (best == floor_key) best = kNone;
     }
   }
-  if (floor_key == 0u) floor_key = 1u;  // fewer lanes than that: everything that can be chosen
+  floor_key = max(floor_key, kNone + 1u);  // fewer lanes than that: everything that can be chosen
   int mine = 0;
 #pragma unroll
   for (int j = 0; j < NPL; ++j) mine += key[j] >= floor_key;
@@ -286,6 +314,8 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   int rank = 32, id = -1;
   __syncwarp();
   if (n <= 32) {
+    scratch->key[lane] = 0u;
+    __syncwarp();
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
       if (key[j] >= floor_key) {
@@ -294,29 +324,29 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
         ++before;
       }
     __syncwarp();
-    if (lane < n) {
-      const uint32_t v = scratch->key[lane];
-      id = (int)scratch->id[lane];
-      rank = 0;
-      for (int i = 0; i < n; ++i) {
-        const uint32_t o = scratch->key[i];
-        rank += o > v || (o == v && i < lane);
-      }
+    const uint32_t v = scratch->key[lane];
+    const uint4* four = reinterpret_cast<const uint4*>(scratch->key);
+    rank = 0;
+    for (int i = 0; i < n; i += 4) {  // of equals the one in the lower lane, with the lower id, ranks first
+      const uint4 o = four[i / 4];
+      rank += (o.x + (i < lane ? 1u : 0u) > v) + (o.y + (i + 1 < lane ? 1u : 0u) > v) + (o.z + (i + 2 < lane ? 1u : 0u) > v) +
+              (o.w + (i + 3 < lane ? 1u : 0u) > v);
     }
+    if (lane < n) id = (int)scratch->id[lane];
+    else rank = 32;
     if (!by_logit) {
-      const uint32_t v = lane < n ? scratch->key[lane] : 0u;
       __syncwarp();
       if (lane < n) scratch->key[rank] = v;
       __syncwarp();
       const uint32_t next = lane < n && rank + 1 < n ? scratch->key[rank + 1] : 0u;
-      close = __any_sync(0xffffffffu, lane < n && rank < r.k && next != 0u && key_value(v) - key_value(next) < margin);
+      close = __any_sync(0xffffffffu, rank < r.k && next != 0u && key_value(v) - key_value(next) < margin);
     }
   } else {
     // k rounds: the best of every lane, the warp's best of those; a lane keeps the first of equals
-    uint32_t best = 0u;
+    uint32_t best = kNone;
     int at = 0;
     auto scan = [&]() {
-      best = 0u;
+      best = kNone;
 #pragma unroll
       for (int j = 0; j < NPL; ++j)
         if (key[j] > best) {
@@ -328,7 +358,7 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
     float last = 0.f;
     for (int i = 0; i < want && !close; ++i) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-      if (m == 0u) break;
+      if (m == kNone) break;
       const int win = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
       const int e = __shfl_sync(0xffffffffu, e0 + at, win);
       if (!by_logit) {
@@ -340,7 +370,7 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       if (lane == win) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-          if (j == at) key[j] = 0u;
+          if (j == at) key[j] = kNone;
         scan();
       }
     }
@@ -355,13 +385,13 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   float w = 0.f;
   if (chosen) {
     const float v = logit(id);
-    w = r.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - top) / sum;
+    w = r.sigmoid ? __fdividef(1.f, 1.f + expf(-v)) : __fdividef(expf(v - top), sum);
   }
   if (r.norm) {
     float all = w;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) all += __shfl_xor_sync(0xffffffffu, all, m);
-    w = w / (all + 1e-20f);
+    w = __fdividef(w, all + 1e-20f);
   }
   if (chosen) write(rank, id, w * r.scale);
   const int found = __popc(__ballot_sync(0xffffffffu, chosen));
