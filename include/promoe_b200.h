@@ -200,6 +200,13 @@ typedef struct pm_layer_weights {
   int32_t quant4;       /* routed experts are uint4 group-128 (params: q, scale/zero per matrix) */
 } pm_layer_weights;
 int pm_layer_set_weights(pm_ctx* ctx, int layer, const pm_layer_weights* w);
+/* Gives a layer whose weights are set a router other than softmax with greedy top-k: sigmoid scores, a correction bias,
+ * groups (struct pm_router, below; at most 256 experts, num_expert and top_k those of the context and the layer). Its norm_topk
+ * and routed_scale stand in for the weights'; the logits stay gate_w x + gate_bias. choice_bias must outlive the
+ * layer. A token for which fewer than top_k experts can be chosen is computed with those; one whose logits
+ * hold a NaN yields NaN. router = NULL, or setting the weights again, takes the router back. */
+struct pm_router;
+int pm_layer_set_router(pm_ctx* ctx, int layer, const struct pm_router* router);
 
 /* One MoE layer forward on device buffers: x [T, hidden] bf16 -> y [T, hidden] bf16.
  * Runs K1 (route) and K2 (permute), reads the expert counts back, performs the

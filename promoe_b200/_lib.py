@@ -106,6 +106,7 @@ SIGNATURES = {
     "pm_iter_marks_read": (_i, [_vp, C.POINTER(pm_stats), _sz, C.POINTER(_sz)]),
     "pm_profile_read": (_i, [_vp, C.POINTER(pm_profile), _i]),
     "pm_layer_set_weights": (_i, [_vp, _i, C.POINTER(pm_layer_weights)]),
+    "pm_layer_set_router": (_i, [_vp, _i, C.POINTER(pm_router)]),
     "pm_moe_forward": (_i, [_vp, _i, _vp, _i, _vp, _vp]),
     "pm_moe_forward_routed": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp]),
     "pm_moe_forward_routed_begin": (_i, [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp,

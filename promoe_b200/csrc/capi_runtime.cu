@@ -441,7 +441,27 @@ int pm_layer_set_weights(pm_ctx* ctx, int layer, const pm_layer_weights* w) {
   if (w->quant4 && (w->hidden % 128 != 0 || w->inter % 128 != 0))
     return fail(PM_ERR_INVALID, "quant4 layer needs hidden and inter to be multiples of 128");
   ctx->layers[layer].w = *w;
+  ctx->layers[layer].rule = pm::RouteRule{};
   ctx->layers[layer].set = true;
+  return PM_OK;
+}
+
+int pm_layer_set_router(pm_ctx* ctx, int layer, const pm_router* r) {
+  if (need(ctx)) return PM_ERR_INVALID;
+  if (layer < 0 || layer >= ctx->cfg.num_layer) return fail(PM_ERR_INVALID, "layer out of range");
+  if (!ctx->layers[layer].set) return fail(PM_ERR_STATE, "set_router: the layer's weights have to be set first");
+  if (!r) {
+    ctx->layers[layer].rule = pm::RouteRule{};
+    return PM_OK;
+  }
+  pm::RouteRule rule;
+  const int rc = router_rule(r, "set_router", &rule);
+  if (rc != PM_OK) return rc;
+  if (rule.E != ctx->cfg.num_expert) return fail(PM_ERR_INVALID, "set_router: num_expert is not the context's");
+  if (rule.E > 256) return fail(PM_ERR_INVALID, "set_router: a layer's router takes at most 256 experts");
+  if (rule.k != ctx->layers[layer].w.top_k) return fail(PM_ERR_INVALID, "set_router: top_k is not the layer's");
+  if (((uintptr_t)rule.bias & 3) != 0) return fail(PM_ERR_INVALID, "set_router: misaligned pointer");
+  ctx->layers[layer].rule = rule;
   return PM_OK;
 }
 

@@ -32,6 +32,10 @@ combine_kernel(const float* __restrict__ yexp, const int32_t* __restrict__ pos,
   for (int h = threadIdx.x * 4; h < H; h += kCombineThreads * 4) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j = 0; j < k; ++j) {
+      if (p_s[j] < 0) {  // no expert: a weight of 0, or NaN where the token has no routing at all
+        if (w_s[j] != 0.f) acc.x = acc.y = acc.z = acc.w = w_s[j];
+        continue;
+      }
       float4 v = *reinterpret_cast<const float4*>(yexp + (size_t)p_s[j] * H + h);
       float w = w_s[j];
       acc.x = fmaf(w, v.x, acc.x);

@@ -16,7 +16,7 @@
 //   lanes are then combined by a butterfly over lane ^ 16, 8, 4, 2, 1.
 #include <algorithm>
 
-#include "pm_common.cuh"
+#include "route_select.cuh"
 
 namespace pm {
 namespace {
@@ -160,16 +160,43 @@ __device__ __forceinline__ int finish_token(const float* logit_s, int t, int lan
   return sel_e;
 }
 
-// TOK tokens per CTA, EPW expert rows per warp at a time (see launch_gate_topk for the choice).
-template <int TOK, int EPW, int UNROLL>
+// The same for a layer with a router rule (route_select.cuh): softmax or sigmoid scores, a correction bias, groups. `scratch`:
+// route_scratch_bytes(E) of this warp. Lane j < k returns the j-th expert, -1 where there are fewer.
+__device__ __forceinline__ int finish_token_by_rule(const float* logit_s, int t, int lane, bool has_shared_gate, const RouteRule& rule,
+                                                    RouteScratch* scratch, const int32_t* __restrict__ expert_slot,
+                                                    int32_t* __restrict__ topk_ids, float* __restrict__ topk_w,
+                                                    int32_t* __restrict__ topk_slot, float* __restrict__ shared_scale,
+                                                    float* __restrict__ logits_out) {
+  const int E = rule.E, k = rule.k, npl = (E + 31) / 32;
+  if (logits_out != nullptr)
+    for (int e = lane; e < E; e += 32) logits_out[(size_t)t * E + e] = logit_s[e];
+  if (has_shared_gate && lane == 0 && shared_scale != nullptr)
+    shared_scale[t] = 1.f / (1.f + __expf(-logit_s[E]));
+  constexpr int kPerLane = kMaxExperts / 32;
+  float l[kPerLane], b[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) l[i] = i < npl && lane * npl + i < E ? logit_s[lane * npl + i] : -CUDART_INF_F;
+  const float bias_max = load_choice_bias<kPerLane>(rule, npl, lane, b);
+  route_token<kPerLane>(l, npl, rule, b, bias_max, scratch, lane, [&](int e) { return logit_s[e]; }, [&](int j, int id, float w) {
+    topk_ids[(size_t)t * k + j] = id;
+    topk_w[(size_t)t * k + j] = w;
+    if (topk_slot != nullptr) topk_slot[(size_t)t * k + j] = expert_slot != nullptr && id >= 0 ? expert_slot[id] : -1;
+  });
+  __syncwarp();
+  return lane < k ? topk_ids[(size_t)t * k + lane] : -1;  // what this warp has just written
+}
+
+// TOK tokens per CTA, EPW expert rows per warp at a time (see launch_gate_topk for the choice). RULE: the layer's router has
+// a rule; a kernel of its own, so that the others keep their registers.
+template <int TOK, int EPW, int UNROLL, bool RULE>
 __global__ void __launch_bounds__(kMaxGateThreads)
 gate_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w_gate,
                  const float* __restrict__ bias, const __nv_bfloat16* __restrict__ w_shared_gate,
                  int T, int H, int E, int k, int norm_topk, float routed_scale,
                  const int32_t* __restrict__ expert_slot, int32_t* __restrict__ topk_ids,
                  float* __restrict__ topk_w, int32_t* __restrict__ topk_slot,
-                 float* __restrict__ shared_scale, float* __restrict__ logits_out) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];  // TOK rows of H bf16
+                 float* __restrict__ shared_scale, float* __restrict__ logits_out, const __grid_constant__ RouteRule rule) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];  // TOK rows of H bf16, later the choice's scratch
   __shared__ float logit_all[TOK * (kMaxExperts + 1)];
   wait_for_predecessor();
 
@@ -211,6 +238,13 @@ gate_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __res
   }
   __syncthreads();
 
+  if constexpr (RULE) {
+    for (int tt = warp; tt < n_tok; tt += nwarp)
+      finish_token_by_rule(logit_all + tt * (E + 1), t0 + tt, lane, w_shared_gate != nullptr, rule,
+                           reinterpret_cast<RouteScratch*>(smem_raw + warp * route_scratch_bytes(E)), expert_slot, topk_ids, topk_w,
+                           topk_slot, shared_scale, logits_out);
+    return;
+  }
   for (int tt = warp; tt < n_tok; tt += nwarp)  // warp tt finishes token t0 + tt
     finish_token(logit_all + tt * (E + 1), t0 + tt, lane, w_shared_gate != nullptr, E, k, norm_topk, routed_scale, expert_slot,
                  topk_ids, topk_w, topk_slot, shared_scale, logits_out);
@@ -223,7 +257,7 @@ gate_topk_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __res
 // experts went from 55.1 to 45.9 us with it; in two launches (CUDA graph) the router took 9.2 us and the permutation 3.2.
 constexpr int kRouteCtas = 8, kRouteThreads = 512, kRouteMaxTokens = 16, kRouteMaxTopK = 16;
 
-template <int TOK>
+template <int TOK, bool RULE>
 __global__ void __cluster_dims__(kRouteCtas, 1, 1) __launch_bounds__(kRouteThreads)
 route_small_kernel(const __grid_constant__ RouteArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];  // the token rows, padded to a multiple of TOK
@@ -277,8 +311,14 @@ route_small_kernel(const __grid_constant__ RouteArgs a) {
   if (rank != 0) return;
 
   for (int t = warp; t < T; t += kRouteThreads / 32) {
-    const int e = finish_token(logit_all + t * (E + 1), t, lane, a.w_shared_gate != nullptr, E, k, a.norm_topk,
-                               a.routed_scale, a.expert_slot, a.topk_ids, a.topk_w, a.topk_slot, a.shared_scale, nullptr);
+    int e;
+    if constexpr (RULE)
+      e = finish_token_by_rule(logit_all + t * (E + 1), t, lane, a.w_shared_gate != nullptr, a.rule,
+                               reinterpret_cast<RouteScratch*>(smem_raw + warp * route_scratch_bytes(E)), a.expert_slot, a.topk_ids,
+                               a.topk_w, a.topk_slot, a.shared_scale, nullptr);
+    else
+      e = finish_token(logit_all + t * (E + 1), t, lane, a.w_shared_gate != nullptr, E, k, a.norm_topk, a.routed_scale,
+                       a.expert_slot, a.topk_ids, a.topk_w, a.topk_slot, a.shared_scale, nullptr);
     if (lane < k) ids_s[t * k + lane] = e;
   }
   __syncthreads();
@@ -286,10 +326,10 @@ route_small_kernel(const __grid_constant__ RouteArgs a) {
   int e = -1, before = 0;
   if (tid < R) {
     e = ids_s[tid];
-    if (e < 0 || e >= E) {  // only where no logit compares (NaN): dropped and flagged, as by the permutation
+    if (e < 0 || e >= E) {  // no expert (-1, by a rule), or where no logit compares (NaN): dropped, the latter flagged, as by the permutation
+      if (e != -1 && a.err_flag != nullptr) atomicExch(a.err_flag, 1);
       e = -1;
       a.pos[tid] = -1;
-      if (a.err_flag != nullptr) atomicExch(a.err_flag, 1);
     } else {
       for (int j = 0; j < tid; ++j) before += ids_s[j] == e;
       atomicAdd(&cnt[e], 1);
@@ -326,18 +366,18 @@ template <int TOK, int EPW, int UNROLL>
 cudaError_t launch_gate(const __nv_bfloat16* x, const __nv_bfloat16* w_gate, const float* bias,
                         const __nv_bfloat16* w_shared_gate, int T, int H, int E, int k, int norm_topk,
                         float routed_scale, const int32_t* expert_slot, int32_t* topk_ids, float* topk_w,
-                        int32_t* topk_slot, float* shared_scale, float* logits_out, cudaStream_t s) {
+                        int32_t* topk_slot, float* shared_scale, float* logits_out, const RouteRule& rule, cudaStream_t s) {
   const int n_rows = E + (w_shared_gate != nullptr ? 1 : 0);
   const int warps = std::min(kMaxGateThreads / 32, (n_rows + EPW - 1) / EPW);
-  const size_t smem = (size_t)TOK * H * 2;
-  auto kern = gate_topk_kernel<TOK, EPW, UNROLL>;
-  static SmemOptIn once;
+  const size_t smem = std::max((size_t)TOK * H * 2, rule.E > 0 ? std::min(TOK, warps) * route_scratch_bytes(E) : 0);
+  auto kern = rule.E > 0 ? gate_topk_kernel<TOK, EPW, UNROLL, true> : gate_topk_kernel<TOK, EPW, UNROLL, false>;
+  static SmemOptIn once[2];
   if (smem > 32 * 1024) {
-    cudaError_t e = opt_in_smem(once, kern);
+    cudaError_t e = opt_in_smem(once[rule.E > 0], kern);
     if (e != cudaSuccess) return e;
   }
   return launch_behind(kern, (T + TOK - 1) / TOK, warps * 32, smem, s, x, w_gate, bias, w_shared_gate, T, H, E, k, norm_topk,
-                       routed_scale, expert_slot, topk_ids, topk_w, topk_slot, shared_scale, logits_out);
+                       routed_scale, expert_slot, topk_ids, topk_w, topk_slot, shared_scale, logits_out, rule);
 }
 
 size_t route_small_smem(int T, int H) { return (size_t)(T > 1 ? (T + 3) / 4 * 4 : 1) * H * 2; }
@@ -347,11 +387,14 @@ size_t route_small_smem(int T, int H) { return (size_t)(T > 1 ? (T + 3) / 4 * 4 
 bool route_small_usable(int T, int H) { return T <= kRouteMaxTokens && route_small_smem(T, H) <= 160 * 1024; }
 
 cudaError_t launch_route_small(const RouteArgs& a, cudaStream_t s) {
-  const size_t smem = route_small_smem(a.T, a.H);
-  auto kern = a.T > 1 ? route_small_kernel<4> : route_small_kernel<1>;
-  static SmemOptIn once[2];
+  const size_t smem = std::max(route_small_smem(a.T, a.H),
+                               a.rule.E > 0 ? std::min(a.T, kRouteThreads / 32) * route_scratch_bytes(a.E) : 0);
+  const bool many = a.T > 1, rule = a.rule.E > 0;
+  auto kern = rule ? (many ? route_small_kernel<4, true> : route_small_kernel<1, true>)
+                   : (many ? route_small_kernel<4, false> : route_small_kernel<1, false>);
+  static SmemOptIn once[4];
   if (smem > 16 * 1024) {  // beside 19 KB of static shared memory
-    cudaError_t e = opt_in_smem(once[a.T > 1], kern);
+    cudaError_t e = opt_in_smem(once[2 * rule + many], kern);
     if (e != cudaSuccess) return e;
   }
   return launch_behind(kern, kRouteCtas, kRouteThreads, smem, s, a);
@@ -360,11 +403,12 @@ cudaError_t launch_route_small(const RouteArgs& a, cudaStream_t s) {
 cudaError_t launch_gate_topk(const __nv_bfloat16* x, const __nv_bfloat16* w_gate, const float* bias,
                              const __nv_bfloat16* w_shared_gate, int T, int H, int E, int k, int norm_topk,
                              float routed_scale, const int32_t* expert_slot, int32_t* topk_ids, float* topk_w,
-                             int32_t* topk_slot, float* shared_scale, float* logits_out, cudaStream_t s) {
+                             int32_t* topk_slot, float* shared_scale, float* logits_out, cudaStream_t s, const RouteRule* rule) {
   if (T <= 0) return cudaSuccess;
+  const RouteRule none{}, &by = rule != nullptr ? *rule : none;
   auto go = [&](auto launch) {
     return launch(x, w_gate, bias, w_shared_gate, T, H, E, k, norm_topk, routed_scale, expert_slot, topk_ids, topk_w,
-                  topk_slot, shared_scale, logits_out, s);
+                  topk_slot, shared_scale, logits_out, by, s);
   };
   // Up to two waves of one CTA per SM a token has a CTA to itself (most loads in flight); then 4, and from
   // about three waves of 4 on, 8 tokens share a CTA's reads of the router matrix. Few experts: one or two

@@ -112,12 +112,20 @@ cudaError_t launch_behind(void (*kern)(P...), dim3 grid, dim3 block, size_t smem
 }
 #endif
 
-// Kernel launchers (defined in the .cu files). All take the caller's stream.
+// How a router turns logits into experts (route_select.cuh). E = 0: softmax, greedy top-k.
+struct RouteRule {
+  int32_t E, k, sigmoid, n_group, topk_group, group_top2, norm;
+  float scale;
+  const float* bias;  // device [E] or nullptr
+};
+
+// Kernel launchers (defined in the .cu files). All take the caller's stream. A router's `rule` (or nullptr) stands in
+// for norm_topk and routed_scale; its E and k are the call's.
 cudaError_t launch_gate_topk(const __nv_bfloat16* x, const __nv_bfloat16* w_gate, const float* bias,
                              const __nv_bfloat16* w_shared_gate, int T, int H, int E, int k,
                              int norm_topk, float routed_scale, const int32_t* expert_slot,
                              int32_t* topk_ids, float* topk_w, int32_t* topk_slot,
-                             float* shared_scale, float* logits_out, cudaStream_t s);
+                             float* shared_scale, float* logits_out, cudaStream_t s, const RouteRule* rule = nullptr);
 
 // Router and permutation of a decode batch (at most 16 tokens) in one launch: launch_gate_topk followed by
 // launch_permute on its ids. Usable when the token rows fit shared memory.
@@ -135,6 +143,7 @@ struct RouteArgs {
   int32_t *counts, *offsets, *row_token, *pos, *err_flag;
   int32_t tail_rows, zero_n;
   int32_t* zero_words;
+  RouteRule rule;  // E = 0: none
 };
 bool route_small_usable(int T, int H);
 cudaError_t launch_route_small(const RouteArgs& a, cudaStream_t s);
@@ -303,12 +312,6 @@ cudaError_t launch_prefill_ffn(const TcLaunch& a, cudaStream_t s, cudaEvent_t mi
 // zeros beyond the matrix. The base and the pitch lie on 16-byte boundaries. A copy moves bits, so bf16 stands for fp16 too.
 int tc_encode_matrix(CUtensorMap* map, const void* base, uint64_t k, uint64_t rows, uint64_t pitch_elems, int box_rows);
 
-// How a router turns logits into experts (route_select.cuh).
-struct RouteRule {
-  int32_t E, k, sigmoid, n_group, topk_group, group_top2, norm;
-  float scale;
-  const float* bias;  // device [E] or nullptr
-};
 int check_route_rule(const RouteRule& r, const char* who);
 int router_rule(const pm_router* r, const char* who, RouteRule* rule);  // checked
 cudaError_t launch_route(const void* logits, int dtype, int64_t ld, int n_tok, const RouteRule& rule, int32_t* ids, float* w,

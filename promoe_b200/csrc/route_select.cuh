@@ -34,7 +34,7 @@ __device__ __forceinline__ int lanes_per_group(int G) { return 1 << (31 - __clz(
 
 // ---- the same ranking in 64 bits; c[E] is shared memory of the warp ------------------------------------------
 // Logits in c become choices.
-__device__ __noinline__ void exact_choices(double* c, const RouteRule* rule, int lane) {
+static __device__ __noinline__ void exact_choices(double* c, const RouteRule* rule, int lane) {
   const int E = rule->E;
   double mx = -CUDART_INF, sum = 0.0;
   __syncwarp();
@@ -56,7 +56,7 @@ __device__ __noinline__ void exact_choices(double* c, const RouteRule* rule, int
 }
 
 // The groups that stay, as bits.
-__device__ __noinline__ uint32_t exact_groups(const double* c, const RouteRule* rule, int lane) {
+static __device__ __noinline__ uint32_t exact_groups(const double* c, const RouteRule* rule, int lane) {
   const int per = rule->E / rule->n_group;
   double value = -CUDART_INF;  // lane g: group g
   if (lane < rule->n_group) {
@@ -81,7 +81,7 @@ __device__ __noinline__ uint32_t exact_groups(const double* c, const RouteRule* 
 }
 
 // Lane j < k returns the j-th of the experts in the groups `kept`, -1 if there are fewer. Uses c up.
-__device__ __noinline__ int exact_rank(double* c, const RouteRule* rule, uint32_t kept, int lane) {
+static __device__ __noinline__ int exact_rank(double* c, const RouteRule* rule, uint32_t kept, int lane) {
   const int E = rule->E, per = E / rule->n_group;
   for (int e = lane; e < E; e += 32)
     if (!((kept >> (e / per)) & 1u)) c[e] = -CUDART_INF;

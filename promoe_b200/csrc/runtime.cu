@@ -965,6 +965,7 @@ int rt_forward(pm_ctx* c, int layer, const void* xv, int T, void* yv, cudaStream
     a.counts = c->d_counts; a.offsets = c->d_offsets; a.row_token = c->d_row_token; a.pos = c->d_pos; a.err_flag = c->d_err;
     a.tail_rows = n_shared * T;
     a.zero_words = zero_words; a.zero_n = zero_words != nullptr ? kMaxFusedGroups + 1 : 0;
+    a.rule = ly.rule;
     PM_CUDA(launch_route_small(a, s));
     c->kernel_launches += 1;
   } else {
@@ -974,7 +975,7 @@ int rt_forward(pm_ctx* c, int layer, const void* xv, int T, void* yv, cudaStream
     } else {
       PM_CUDA(launch_gate_topk(x, (const __nv_bfloat16*)w.gate_w, w.gate_bias, (const __nv_bfloat16*)w.shared_gate_w,
                                T, H, E, k, w.norm_topk, w.routed_scale, ly.slot_table_dev, c->d_topk_ids,
-                               c->d_topk_w, c->d_topk_slot, c->d_shared_scale, nullptr, s));
+                               c->d_topk_w, c->d_topk_slot, c->d_shared_scale, nullptr, s, &ly.rule));
       c->kernel_launches += 1;
     }
     PM_CUDA(launch_permute(ids_dev, R, k, E, c->d_counts, c->d_offsets, c->d_row_token, c->d_pos, c->d_err,

@@ -102,6 +102,7 @@ struct pm_ctx {
   struct Layer {
     pm_layer_weights w{};
     bool set = false;
+    pm::RouteRule rule{};               // E = 0: the weights' softmax, greedy top-k
     int32_t* slot_table_dev = nullptr;  // [E] slot of each expert, -1 if absent
     bool slot_table_dirty = true;
   };

@@ -259,6 +259,16 @@ class ExpertCache:
         self._hidden = w.hidden
         _lib.call("pm_layer_set_weights", self._ctx, layer, C.byref(w))
 
+    def set_router(self, layer: int, router) -> None:
+        """Gives a layer whose weights are set a router other than softmax with greedy top-k (a promoe_b200.ops.Router: sigmoid
+        scores, a correction bias, groups); its norm_topk and routed_scale stand in for the layer's. None takes it back."""
+        if router is None:
+            _lib.call("pm_layer_set_router", self._ctx, layer, None)
+            return
+        _lib.call("pm_layer_set_router", self._ctx, layer, C.byref(router.rule))
+        if router.bias is not None:
+            self._keep.append(router.bias)
+
     def set_predictor(self, src: int, dst: int, w1: torch.Tensor, b1: torch.Tensor | None, w2: torch.Tensor,
                       b2: torch.Tensor | None) -> None:
         for t in (w1, b1, w2, b2):

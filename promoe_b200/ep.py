@@ -66,7 +66,8 @@ class CudaBackend:
     def __init__(self, cache, layers, device, geometry: Geometry, rank: int, predictors=None, predict_map=None,
                  global_tokens: int = 0, n_predict: int = 0):
         """layers[l] = dict(gate_w, gate_bias, shared (3 tensors or None), shared_gate_w, top_k, norm_topk,
-        routed_scale, inter) with full-width (all experts) router weights. predictors[(src, dst)] =
+        routed_scale, inter) with full-width (all experts) router weights, and optionally router, a promoe_b200.ops.Router
+        that chooses by another rule than softmax with greedy top-k. predictors[(src, dst)] =
         (w1, b1, w2, b2) device tensors over ALL experts; predict_map[src] = (first, last + 1) of the
         layers index src predicts; n_predict: experts prefetched per predicted layer over ALL ranks
         (the global top n_predict; every owner prefetches the ones it holds). global_tokens: tokens in
@@ -148,11 +149,19 @@ class CudaBackend:
         E, k = p["gate_w"].shape[0], p["top_k"]
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         has_gate = p["shared_gate_w"] is not None
+        router, logits = p.get("router"), None
+        if router is not None:
+            if "logits" not in b:
+                b["logits"] = torch.empty((T, E), dtype=torch.float32, device=self.device)
+            logits = b["logits"]
         self._lib.call("pm_k_gate_topk", x.data_ptr(), p["gate_w"].data_ptr(), ptr(p["gate_bias"]),
                        ptr(p["shared_gate_w"]), T, H, E, k, int(p["norm_topk"]), float(p["routed_scale"]), None,
-                       b["ids"].data_ptr(), b["w"].data_ptr(), None, b["ss"].data_ptr() if has_gate else None, None,
+                       b["ids"].data_ptr(), b["w"].data_ptr(), None, b["ss"].data_ptr() if has_gate else None, ptr(logits),
                        self._stream())
         self.launches += 1
+        if router is not None:  # a rule of the layer's own, on the same logits
+            router(logits, out=(b["ids"], b["w"]))
+            self.launches += 1
         return b["ids"], b["w"], b["ss"] if has_gate else None
 
     def permute(self, ids, b):

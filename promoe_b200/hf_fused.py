@@ -7,13 +7,19 @@ experts of a block in two 3-D parameters instead (`experts.gate_up_proj [E, 2I, 
 same job for that layout: every expert's three matrices are sliced out of the fused tensors and
 registered with the cache, the fused tensors are released, and the block's forward becomes one call
 into the fused device path. Supported blocks: Qwen2-MoE (shared expert with sigmoid gate),
-Mixtral (renormalised top-k), DeepSeek-V2 with greedy top-k (shared experts, routed scaling).
+Mixtral (renormalised top-k), DeepSeek-V2 with greedy or group-limited top-k (shared experts, routed scaling), and blocks
+whose gate ranks sigmoid scores with a correction bias.
+
+`install_linears` hands the model's other matrix products to the library too, `score_tokens` says what a text's tokens were
+worth to the model.
 """
 from __future__ import annotations
 
 import torch
 
+from . import ops
 from .engine import ExpertCache
+from .moe_block import describe_router, set_router
 
 
 def find_moe_blocks(model: torch.nn.Module) -> list[tuple[str, torch.nn.Module]]:
@@ -38,9 +44,7 @@ def _describe(block) -> dict:
         norm = True
     else:
         norm = bool(getattr(gate, "norm_topk_prob", getattr(block, "norm_topk_prob", False)))
-    if getattr(block, "topk_method", "greedy") != "greedy":
-        raise ValueError("only greedy top-k routing is supported (group-limited routing is not)")
-    return dict(E=E, H=H, I=two_i // 2, top_k=int(top_k), norm_topk=norm,
+    return dict(router=describe_router(block), E=E, H=H, I=two_i // 2, top_k=int(top_k), norm_topk=norm,
                 routed_scale=float(getattr(block, "routed_scaling_factor", 1.0) or 1.0),
                 shared=getattr(block, "shared_expert", None) or getattr(block, "shared_experts", None),
                 shared_gate=getattr(block, "shared_expert_gate", None))
@@ -82,6 +86,7 @@ def inject_hf_fused_model(model: torch.nn.Module, cache_rate: float = 0.375, cac
         sgw = to_dev(d["shared_gate"].weight.reshape(-1)) if d["shared_gate"] is not None else None
         cache.set_layer_weights(layer, to_dev(block.gate.weight), d["I"], d["top_k"], d["norm_topk"], d["routed_scale"],
                                 shared=shared, shared_gate_w=sgw)
+        set_router(cache, layer, d, d["E"], dev)
         # the fused tensors are no longer needed: the experts live in the cache now
         block.experts.gate_up_proj = torch.nn.Parameter(torch.empty(0, dtype=torch.bfloat16), requires_grad=False)
         block.experts.down_proj = torch.nn.Parameter(torch.empty(0, dtype=torch.bfloat16), requires_grad=False)
@@ -102,3 +107,83 @@ def _replace_forward(block, cache: ExpertCache, layer: int):
         return cache.forward(layer, x.contiguous()).view(shape).to(hidden_states.dtype)
 
     block.forward = fused_forward
+
+
+def install_linears(model: torch.nn.Module) -> int:
+    """Replaces the forward of every torch.nn.Linear with bf16 or fp16 weights on a GPU by promoe_b200.ops.Linear (bias in the
+    product's epilogue), and of gated MLPs (`gate_proj`, `up_proj`, `down_proj` around a SiLU: dense layers between MoE blocks)
+    by three such products, SiLU in the first one's epilogue. For inference: calls with tensors that require a gradient
+    keep the module's own forward. Call it once the model is on its device; weights are used in place. MoE blocks that
+    inject_hf_fused_model replaced do not call theirs any more. Returns the number of replaced modules."""
+    def usable(m):
+        return (isinstance(m, torch.nn.Linear) and m.weight.is_cuda and m.weight.dtype in (torch.bfloat16, torch.float16)
+                and m.weight.dim() == 2 and (m.bias is None or m.bias.dtype == m.weight.dtype) and "_promoe_linear" not in vars(m))
+
+    def rows(x):
+        return x.reshape(-1, x.shape[-1])
+
+    def takes(x, lin):
+        return x.is_cuda and x.dtype == lin.weight.dtype and not (torch.is_grad_enabled() and x.requires_grad)
+
+    def replace_linear(m):
+        lin, own = ops.Linear(m.weight, m.bias), m.forward
+
+        def forward(x):
+            if not takes(x, lin):
+                return own(x)
+            return lin(rows(x)).view(*x.shape[:-1], lin.N)
+        m._promoe_linear, m.forward = lin, forward
+
+    def replace_mlp(m):
+        gate, up, down, own = ops.Linear(m.gate_proj.weight, m.gate_proj.bias, "silu"), m.up_proj, m.down_proj, m.forward
+
+        def forward(x):
+            if not takes(x, gate):
+                return own(x)
+            return down(gate(rows(x)).mul_(up(rows(x)))).view(*x.shape[:-1], -1)
+        m._promoe_linear, m.forward = gate, forward
+
+    replaced = 0
+    for m in list(model.modules()):
+        if usable(m):
+            replace_linear(m)
+            replaced += 1
+    for m in list(model.modules()):
+        if "_promoe_linear" in vars(m):
+            continue
+        parts = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        act = type(getattr(m, "act_fn", None)).__name__.lower()
+        if all(isinstance(p, torch.nn.Linear) and "_promoe_linear" in vars(p) for p in parts) and act in ("silu", "siluactivation"):
+            replace_mlp(m)
+            replaced += 1
+    return replaced
+
+
+@torch.no_grad()
+def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, top_n: int = 0) -> dict:
+    """What a causal LM thinks of a text: for every position but the last, the log probability of the token that follows, the
+    entropy of the model's prediction there and its top_n favourites. input_ids [B, S] -> {"logp": [B, S - 1], "entropy": [B, S - 1],
+    "top_ids", "top_logp": [B, S - 1, top_n]}. Tokens outside attention_mask are not scored (logp 0). The vocabulary
+    projection (bf16 or fp16, on the GPU) runs with float32 logits, for as many positions at a time as 64 Mi logits hold,
+    so a long text does not need all its logits at once."""
+    head = model.get_output_embeddings()
+    trunk = getattr(model, model.base_model_prefix)
+    hidden = trunk(input_ids=input_ids, attention_mask=attention_mask).last_hidden_state
+    lin = ops.Linear(head.weight, getattr(head, "bias", None), out_dtype=torch.float32)
+    B, S = input_ids.shape
+    x = hidden[:, :-1].reshape(B * (S - 1), -1).to(head.weight.dtype)
+    targets = input_ids[:, 1:].to(torch.int64)
+    if attention_mask is not None:
+        targets = targets.masked_fill(attention_mask[:, 1:] == 0, -100)
+    targets = targets.reshape(-1)
+    T = x.shape[0]
+    new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=x.device)  # noqa: E731
+    logp, entropy, ids, best = new(T), new(T), new(T, top_n, dtype=torch.int32), new(T, top_n)
+    step = max(1, min(T, (1 << 26) // lin.N))
+    logits = new(step, lin.N)
+    for t0 in range(0, T, step):
+        t1 = min(T, t0 + step)
+        lin(x[t0:t1], out=logits[:t1 - t0])
+        ops.token_logprobs(logits[:t1 - t0], targets[t0:t1], top_n, out=(logp[t0:t1], entropy[t0:t1], ids[t0:t1], best[t0:t1]))
+    return {"logp": logp.view(B, S - 1), "entropy": entropy.view(B, S - 1), "top_ids": ids.view(B, S - 1, top_n),
+            "top_logp": best.view(B, S - 1, top_n)}

@@ -12,6 +12,8 @@ from __future__ import annotations
 
 import torch
 
+from .ops import Router
+
 
 def _first(module, names):
     for n in names:
@@ -25,10 +27,50 @@ def _bf16_dev(t: torch.Tensor, device) -> torch.Tensor:
     return t.detach().to(device=device, dtype=torch.bfloat16).contiguous()
 
 
+def describe_router(block: torch.nn.Module, config=None) -> dict | None:
+    """Arguments of the promoe_b200.ops.Router that the block's routing needs, besides num_expert, top_k, norm_topk and
+    routed_scale; None for softmax with greedy top-k. Blocks whose gate carries a correction bias (`e_score_correction_bias`)
+    rank sigmoid scores + bias and value groups by their two best; `topk_method="group_limited_greedy"` ranks softmax
+    probabilities and values groups by their best."""
+    gate = block.gate
+    cfg = config if config is not None else getattr(block, "config", None)
+
+    def attr(*names):
+        for obj in (gate, block, cfg):
+            for n in names:
+                v = getattr(obj, n, None)
+                if v is not None:
+                    return v
+        return None
+    groups = dict(n_group=int(attr("n_group", "num_group") or 1), topk_group=int(attr("topk_group") or 1))
+    if groups["n_group"] == 1:
+        groups["topk_group"] = 1
+    bias = getattr(gate, "e_score_correction_bias", None)
+    method = getattr(gate, "topk_method", getattr(block, "topk_method", None))
+    if bias is not None and method in (None, "noaux_tc"):
+        scoring = getattr(gate, "scoring_func", getattr(block, "scoring_func", "sigmoid"))
+        return dict(scoring=scoring, bias=bias, group_score="top2", **groups)
+    if method == "group_limited_greedy":
+        return dict(scoring="softmax", group_score="max", **groups)
+    if method in (None, "greedy"):
+        return None
+    raise ValueError(f"the router selects greedily, by groups or with a correction bias; this block uses {method!r}")
+
+
+def set_router(cache, layer: int, d: dict, num_expert: int, device) -> None:
+    """Gives the layer the router that describe_router found, if any."""
+    if d["router"] is None:
+        return
+    kw = dict(d["router"])
+    if kw.get("bias") is not None:
+        kw["bias"] = kw["bias"].detach().to(device=device, dtype=torch.float32).contiguous()
+    cache.set_router(layer, Router(num_expert, d["top_k"], norm_topk=d["norm_topk"], routed_scale=d["routed_scale"], **kw))
+
+
 def describe_block(block: torch.nn.Module, config=None) -> dict:
     """Extracts what the fused layer needs from an HF 4.x style MoE block:
     Qwen2-MoE (`gate`, `experts[i].{gate,up,down}_proj`, `shared_expert`, `shared_expert_gate`),
-    DeepSeek-MoE / V2 (`gate.weight`, `shared_experts`, routed_scaling_factor),
+    DeepSeek-MoE / V2 (`gate.weight`, `shared_experts`, routed_scaling_factor; greedy or group-limited),
     Mixtral (`gate`, `experts[i].{w1,w3,w2}`, top-k renormalised)."""
     gate = block.gate
     gate_w = gate.weight
@@ -38,9 +80,7 @@ def describe_block(block: torch.nn.Module, config=None) -> dict:
     # uint4 experts in this library's layout (promoe_b200.quant4.adapt_quantised_linear): packed rows
     quant4 = getattr(proj, "qweight", None) is not None and getattr(proj, "scale_zero", None) is not None
     inter = proj.qweight.shape[0] if quant4 else proj.weight.shape[0]
-    method = getattr(gate, "topk_method", getattr(block, "topk_method", "greedy"))
-    if method not in (None, "greedy"):
-        raise ValueError(f"the fused router selects the k largest probabilities (greedy); this block uses {method!r}")
+    router = describe_router(block, config)
     shared = _first(block, ("shared_expert", "shared_experts"))
     shared_gate = getattr(block, "shared_expert_gate", None)
     cfg = config if config is not None else getattr(block, "config", None)
@@ -54,7 +94,7 @@ def describe_block(block: torch.nn.Module, config=None) -> dict:
         norm = bool(getattr(block, "norm_topk_prob", getattr(gate, "norm_topk_prob", getattr(cfg, "norm_topk_prob", False))))
     scale = float(getattr(block, "routed_scaling_factor", getattr(gate, "routed_scaling_factor", 1.0)) or 1.0)
     return dict(gate_w=gate_w, inter=inter, top_k=int(top_k), norm_topk=norm, routed_scale=scale,
-                shared=shared, shared_gate=shared_gate, quant4=quant4)
+                shared=shared, shared_gate=shared_gate, quant4=quant4, router=router)
 
 
 def install_fused_forward(block: torch.nn.Module, cache, layer_id: int, device="cuda", config=None,
@@ -72,6 +112,7 @@ def install_fused_forward(block: torch.nn.Module, cache, layer_id: int, device="
         sgw = _bf16_dev(d["shared_gate"].weight.reshape(-1), dev)
     cache.set_layer_weights(layer_id, _bf16_dev(d["gate_w"], dev), d["inter"], d["top_k"], d["norm_topk"],
                             d["routed_scale"], shared=shared, shared_gate_w=sgw, quant4=d["quant4"])
+    set_router(cache, layer_id, d, d["gate_w"].shape[0], dev)
     block._promoe_layer_id = layer_id
     block._promoe_cache = cache
     if not hasattr(block, "_unfused_forward"):

@@ -95,3 +95,28 @@ def test_the_python_handles_check_before_a_device_is_needed(lib):
         ops.Router(64, 6)(torch.zeros((3, 64)))
     with pytest.raises(ValueError):
         ops.token_logprobs(torch.zeros((3, 64)), torch.zeros(3, dtype=torch.int64))
+
+
+def test_a_layer_refuses_a_router_that_does_not_fit(lib):
+    ctx = C.c_void_p()
+    _lib.call("pm_ctx_create", C.byref(ctx), 2, 16, b"num_expert_per_token=4")
+
+    def set_router(layer=0, **over):
+        r = dict(num_expert=16, top_k=4, scoring=1, n_group=4, topk_group=2, group_score=1, norm_topk=1, routed_scale=2.5)
+        r.update(over)
+        _lib.call("pm_layer_set_router", ctx, layer, C.byref(_lib.pm_router(**r)))
+
+    with pytest.raises(_lib.PromoeError) as e:
+        set_router()
+    assert e.value.code == 3  # the weights come first
+    w = _lib.pm_layer_weights()
+    w.hidden, w.inter, w.top_k = 128, 64, 4
+    _lib.call("pm_layer_set_weights", ctx, 0, C.byref(w))
+    set_router()
+    for bad in (dict(layer=-1), dict(layer=2), dict(num_expert=32), dict(top_k=3), dict(n_group=3), dict(topk_group=5), dict(scoring=7),
+                dict(choice_bias=PTR + 2), dict(n_group=8, topk_group=1)):
+        with pytest.raises(_lib.PromoeError) as e:
+            set_router(**bad)
+        assert e.value.code == 1
+    _lib.call("pm_layer_set_router", ctx, 0, None)
+    _lib.call("pm_ctx_destroy", ctx)
