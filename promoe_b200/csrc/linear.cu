@@ -70,13 +70,20 @@ __device__ __forceinline__ float load_bias(const void* bias, int type, int n) {
   return __half2float(static_cast<const __half*>(bias)[n]);
 }
 
+// Short code (the epilogue is unrolled over columns, and a launch of few tiles pays for every instruction it fetches): quick
+// divisions, and the error function's complement by formula 7.1.26 of Abramowitz and Stegun (1.5e-7).
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
   if (ACT == PM_ACT_RELU) return v < 0.f ? 0.f : v;  // NaN stays
-  if (ACT == PM_ACT_SILU) return v / (1.f + __expf(-v));
-  if (ACT == PM_ACT_GELU) return 0.5f * v * erfcf(v * -0.70710678118654752f);
+  if (ACT == PM_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
+  if (ACT == PM_ACT_GELU) {  // v/2 erfc(-v / sqrt 2)
+    const float x = fabsf(v) * 0.70710678f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = p * __expf(-x * x);  // erfc(x)
+    return 0.5f * v * (v > 0.f ? 2.f - tail : tail);
+  }
   if (ACT == PM_ACT_GELU_TANH)  // 0.5 v (1 + tanh u) = v / (1 + exp(-2u))
-    return v / (1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
+    return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
   return v;
 }
 template <int N>
@@ -109,32 +116,37 @@ __device__ __forceinline__ void tile_at(const LinearTc& a, int tile, int& wt, in
 }
 
 // C neighbouring tokens from token m on of weight row n (one row per lane), `left` of them inside y: bias, activation,
-// residual, rounding, store.
+// residual, rounding, store. A chunk that lies inside y as a whole takes a form without tests: those made 17 instructions of
+// the 6 per output, which bounds products with a short K.
 template <class OT, int C>
 __device__ __forceinline__ void finish(const LinearTc& a, float (&o)[C], float bias, int64_t m, int n, int left) {
+  const bool whole = __all_sync(0xffffffffu, left >= C), add = a.res != nullptr;
+  OT r[C];
+  if (add) {
+    const OT* src = static_cast<const OT*>(a.res) + m * a.ldr + n;
+    if (whole) {
+#pragma unroll
+      for (int c = 0; c < C; ++c, src += a.ldr) r[c] = *src;
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c, src += a.ldr) r[c] = c < left ? *src : from_float<OT>(0.f);
+    }
+  }
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] += bias;
   activate_all(o, a.act);
-  const OT* src = static_cast<const OT*>(a.res) + m * a.ldr + n;
+  if (add) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] += to_float<OT>(r[c]);
+  }
   OT* dst = static_cast<OT*>(a.y) + m * a.ldy + n;
-  if (__all_sync(0xffffffffu, left >= C)) {
-    if (a.res != nullptr) {
-      OT r[C];
+  if (whole) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) r[c] = src[c * a.ldr];
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c] += to_float<OT>(r[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) dst[c * a.ldy] = from_float<OT>(o[c]);
+    for (int c = 0; c < C; ++c, dst += a.ldy) *dst = from_float<OT>(o[c]);
   } else {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (c < left) {
-        float v = o[c];
-        if (a.res != nullptr) v += to_float<OT>(src[c * a.ldr]);
-        dst[c * a.ldy] = from_float<OT>(v);
-      }
+    for (int c = 0; c < C; ++c, dst += a.ldy)
+      if (c < left) *dst = from_float<OT>(o[c]);
   }
 }
 
@@ -271,13 +283,13 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       const int n = (wt * CG + (int)rank) * 128 + 32 * w + lane;
       const int m0 = tt * a.width, cols = min(a.width, a.M - m0);
       const float b = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
-      auto give = [&](float (&o)[32], int c0) {
+      auto give = [&](float (&o)[16], int c0) {
         if (!ok) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = nan;
+          for (int c = 0; c < 16; ++c) o[c] = nan;
         }
         if (!split) {
-          finish<OT, 32>(a, o, b, m0 + c0, n, n < a.N ? cols - c0 : 0);
+          finish<OT, 16>(a, o, b, m0 + c0, n, n < a.N ? cols - c0 : 0);
         } else {
           // column c0 + c to the CTA that finishes it, which keeps [source][its columns][128 rows]
           const int per = (a.width + a.split - 1) / a.split;
@@ -285,7 +297,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           int owner = c0 / per, at = c0 - owner * per;
           uint32_t dst = map_to_rank(mine, CG * owner + rank) + 512u * (uint32_t)at;
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
+          for (int c = 0; c < 16; ++c)
             if (c0 + c < cols) {
               asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(o[c]) : "memory");
               dst += 512;
@@ -298,7 +310,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         }
       };
       if (CG == 1 && split) cluster_wait_diverged();
-      float sums[kPromote ? 2 : 1][32];
+      float sums[kPromote ? 4 : 1][16];
       for (int kc = k0; kc < k1; kc += a.chunk, ++it) {
         const int acc = it & 1;
         ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], (it >> 1) & 1, &sh.abort));
@@ -306,24 +318,26 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         const uint32_t taddr = tmem_base + (uint32_t)acc * acc_cols + ((uint32_t)(32 * w) << 16);
         if (kPromote) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {  // at most 128 columns
-            const int c0 = half * 32 + 64 * i;
+          for (int i = 0; i < 4; ++i) {  // at most 128 columns
+            const int c0 = half * 16 + 32 * i;
             if (c0 < cols) {
-              uint32_t v[32];
-              tmem_ld32(taddr + c0, v);
+              uint32_t v[16];
+              tmem_ld16(taddr + c0, v);
               tmem_ld_wait();
+              float(&to)[16] = sums[kPromote ? i : 0];
 #pragma unroll
-              for (int c = 0; c < 32; ++c) sums[kPromote ? i : 0][c] = kc == k0 ? __uint_as_float(v[c]) : sums[kPromote ? i : 0][c] + __uint_as_float(v[c]);
+              for (int c = 0; c < 16; ++c) to[c] = kc == k0 ? __uint_as_float(v[c]) : to[c] + __uint_as_float(v[c]);
             }
           }
         } else {
-          for (int c0 = half * 32; c0 < cols; c0 += 64) {
-            uint32_t v[32];
-            tmem_ld32(taddr + c0, v);
+#pragma unroll 1
+          for (int c0 = half * 16; c0 < cols; c0 += 32) {
+            uint32_t v[16];
+            tmem_ld16(taddr + c0, v);
             tmem_ld_wait();
-            float o[32];
+            float o[16];
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __uint_as_float(v[c]);
+            for (int c = 0; c < 16; ++c) o[c] = __uint_as_float(v[c]);
             give(o, c0);
           }
         }
@@ -336,8 +350,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       }
       if (kPromote) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (half * 32 + 64 * i < cols) give(sums[kPromote ? i : 0], half * 32 + 64 * i);
+        for (int i = 0; i < 4; ++i)
+          if (half * 16 + 32 * i < cols) give(sums[kPromote ? i : 0], half * 16 + 32 * i);
       }
     }
     if (!ok && lane == 0) sh.abort = 1;
@@ -517,12 +531,12 @@ LinearShape choose_shape(int M, int N, int K, bool promote, const int (&cap)[kMa
   double cost = 0;
   const int most = promote ? 128 : 256;  // float32 outputs keep their sums in registers
   for (int cg = 1; cg <= 2; ++cg) {
-    const int grain = 16 * cg, least = (M + most - 1) / most;
-    for (int t = least; t <= least + 8; ++t) {
+    const int grain = 16 * cg;
+    for (int w = grain; w <= most; w += grain) {
       LinearShape c;
       c.cg = cg;
-      c.width = ((M + t - 1) / t + grain - 1) / grain * grain;
-      c.tok_tiles = (M + c.width - 1) / c.width;
+      c.tok_tiles = (M + w - 1) / w;
+      c.width = ((M + c.tok_tiles - 1) / c.tok_tiles + grain - 1) / grain * grain;  // tiles of equal width
       c.atoms = atoms_for(cg, c.width);
       const int steps = (K + 64 * c.atoms - 1) / (64 * c.atoms);
       for (c.split = 1; c.split * cg <= kMaxCluster && c.split <= steps; ++c.split) {
@@ -534,7 +548,7 @@ LinearShape choose_shape(int M, int N, int K, bool promote, const int (&cap)[kMa
           best = c;
         }
       }
-      if (c.width == grain) break;
+      if (c.tok_tiles == 1) break;
     }
   }
   return best;
