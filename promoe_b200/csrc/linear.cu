@@ -30,7 +30,7 @@ constexpr int kWBytes = 128 * 128;  // a CTA's 128 weight rows of a k step
 constexpr int kMaxStages = 12;
 constexpr int kSmemMost = 232448;
 // k of one accumulator of float32 outputs. The tensor cores cut their running sums off where float32 ends, which shrinks a sum by
-// about 2^-24 of itself per addition of 16 k: 2.1e-6 for K = 2048 in one accumulator, TODO in four.
+// about 2^-24 of itself per addition of 16 k: 2.1e-6 for K = 2048 in one accumulator, 4.7e-7 in four.
 constexpr int kPromoteK = 512;
 
 struct LinearTc {
@@ -397,100 +397,194 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 }
 
 // ---- rows that TMA cannot fetch -------------------------------------------------------------------------
-// Tiles of 64 tokens x 64 weight rows, steps of 32 k through shared memory, eight warps of 32 x 16 outputs, the next step's
-// values fetched into registers while the present one is multiplied. Loads are 2 bytes per lane, a warp reads one row's 64 bytes.
-constexpr int kPlainTok = 64, kPlainW = 64, kPlainK = 32, kPlainPitch = kPlainK + 8;
+// Tiles of BM tokens x BN weight rows in steps of 64 k, eight warps (mma.sync). Rows may start at any multiple of two bytes:
+// the aligned 16-byte words that hold a step's values come into a ring of kRing steps (cp.async; each word holds at least one
+// of the row's bytes, so it is mapped memory), and a thread shifts its eight values out of two of them into the tile: 15
+// instructions instead of eight loads. What bounds it: the steps' two barriers and, with few tiles, the SMs that have none.
+// 86 rows of 2611 -> 15580 take 105 us (180 with two-byte loads straight into the tile), 4000 of 2001 -> 2001 295 us = 109
+// TFLOP/s, 125 of 1506 -> 111 20 us (36), one of 3001 -> 4001 28 us. Rows on 16-byte boundaries are five to ten times faster.
+constexpr int kPlainThreads = 256;
 
 template <class T>
-__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&x)[4], const uint32_t (&w)[2]);
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&x)[4], uint32_t w0, uint32_t w1);
 template <>
-__device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&x)[4], const uint32_t (&w)[2]) {
+__device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&x)[4], uint32_t w0, uint32_t w1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(w[0]), "r"(w[1]));
+               : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(w0), "r"(w1));
 }
 template <>
-__device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&x)[4], const uint32_t (&w)[2]) {
+__device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&x)[4], uint32_t w0, uint32_t w1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(w[0]), "r"(w[1]));
+               : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(w0), "r"(w1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix2(uint32_t& r0, uint32_t& r1, uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr));
 }
 
-template <class T, class OT>
-__global__ void __launch_bounds__(256)
+// The eight values that start `shift` bytes into lo, of which `valid` are the row's, the others zero.
+__device__ __forceinline__ uint4 eight_from(const uint4& lo, const uint4& hi, int shift, int valid) {
+  uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  if (shift & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (shift & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  const int bits = (shift & 2) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+  if (valid < 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 2 * i + 1 < valid ? w[i] : 2 * i < valid ? w[i] & 0xffffu : 0u;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, uintptr_t src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <int BM, int BN>
+struct PlainTile {
+  static constexpr int kK = 64, kPitch = kK + 8, kVec = kK / 8;  // 16 bytes of padding: ldmatrix meets every bank once
+  static constexpr int kRows = BM + BN, kWords = kVec + 1, kRing = BM >= 64 ? 3 : 4;
+  static constexpr int kPer = (kRows + 31) / 32;  // rows per thread: eight threads take a row's eights
+  static constexpr size_t bytes() { return (size_t)kRows * kPitch * 2 + (size_t)kRing * kRows * kWords * 16; }
+};
+
+template <class T, class OT, int BM, int BN>
+__global__ void __launch_bounds__(kPlainThreads)
 linear_plain_kernel(const __grid_constant__ LinearCall a) {
-  __shared__ __align__(16) uint16_t xs[kPlainTok * kPlainPitch], ws[kPlainW * kPlainPitch];
+  using P = PlainTile<BM, BN>;
+  constexpr int kWarpsM = BM >= 32 ? BM / 32 : 1, kWarpsN = 8 / kWarpsM;
+  constexpr int kM = BM >= 32 ? 2 : 1, kN = BN / kWarpsN / 8;  // 16 x 8 pieces of a warp
+  static_assert(BN % (kWarpsN * 8) == 0, "whole pieces");
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  uint16_t* tile = reinterpret_cast<uint16_t*>(smem_raw);  // token rows, then weight rows
+  unsigned char* ring = smem_raw + (size_t)P::kRows * P::kPitch * 2;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int w_tiles = (a.N + kPlainW - 1) / kPlainW;
-  const int m0 = blockIdx.x / w_tiles * kPlainTok, n0 = blockIdx.x % w_tiles * kPlainW;
-  const int wm = (warp & 1) * 32, wn = (warp >> 1) * 16;
+  const int w_tiles = (a.N + BN - 1) / BN;
+  const int m0 = blockIdx.x / w_tiles * BM, n0 = blockIdx.x % w_tiles * BN;
+  const int wm = warp % kWarpsM * 16 * kM, wn = warp / kWarpsM * 8 * kN;
+  const int steps = (a.K + P::kK - 1) / P::kK;
   wait_for_predecessor();
-  const uint16_t* __restrict__ x = static_cast<const uint16_t*>(a.x);
-  const uint16_t* __restrict__ w = static_cast<const uint16_t*>(a.w);
-  float acc[2][2][4] = {};
-  uint16_t xr[8], wr[8];
-  auto fetch = [&](int k0) {
-    const int k = k0 + lane;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int m = m0 + warp + 8 * i, n = n0 + warp + 8 * i;
-      xr[i] = m < a.M && k < a.K ? x[(int64_t)m * a.ldx + k] : (uint16_t)0;
-      wr[i] = n < a.N && k < a.K ? w[(int64_t)n * a.ldw + k] : (uint16_t)0;
-    }
+  // Eight neighbouring threads take the first eight words of a row, rows tid / 8, + 32, ...; the ninth word of row r is thread r's.
+  const int v = tid & 7, r0 = tid >> 3;
+  auto row_at = [&](int r) -> uintptr_t {  // 0 outside the matrices
+    const bool tok = r < BM;
+    const int row = tok ? m0 + r : n0 + r - BM;
+    if (r >= P::kRows || row >= (tok ? a.M : a.N)) return 0;
+    return (uintptr_t)(tok ? a.x : a.w) + (uintptr_t)((int64_t)row * (tok ? a.ldx : a.ldw) * 2);
   };
-  fetch(0);
-  for (int k0 = 0; k0 < a.K; k0 += kPlainK) {
-    __syncthreads();
+  uintptr_t word[P::kPer];
+  uint32_t shifts = 0, rows_in = 0;  // of each row: half the byte offset in its first word; whether it exists
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      xs[(warp + 8 * i) * kPlainPitch + lane] = xr[i];
-      ws[(warp + 8 * i) * kPlainPitch + lane] = wr[i];
+  for (int i = 0; i < P::kPer; ++i) {
+    const uintptr_t row = row_at(r0 + 32 * i);
+    word[i] = (row & ~(uintptr_t)15) + 16u * v;
+    shifts |= (uint32_t)(row & 14) >> 1 << (4 * i);
+    rows_in |= (uint32_t)(row != 0) << i;
+  }
+  const uintptr_t ninth_row = row_at(tid), ninth = (ninth_row & ~(uintptr_t)15) + 128u;
+  const uint32_t ninth_end = ninth_row != 0 ? 2u * (uint32_t)a.K + (uint32_t)(ninth_row & 15) : 0u;  // words start before it
+  const uint32_t ring0 = smem_u32(ring);
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      const uint32_t dst = ring0 + (uint32_t)(step % P::kRing) * (P::kRows * P::kWords * 16), off = (uint32_t)step * (P::kK * 2);
+#pragma unroll
+      for (int i = 0; i < P::kPer; ++i)
+        if ((rows_in >> i & 1) && off + 16u * v < 2u * (uint32_t)a.K + (shifts >> (4 * i) & 7) * 2u)
+          cp_async_16(dst + 16u * (uint32_t)((r0 + 32 * i) * P::kWords + v), word[i] + off);
+      if (off + 128u < ninth_end) cp_async_16(dst + 16u * (uint32_t)(tid * P::kWords + P::kVec), ninth + off);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float acc[kM][kN][4] = {};
+  const uint32_t base = smem_u32(tile);
+  // ldmatrix: lanes 0-15 give the rows of the first 8 k, lanes 16-31 of the next
+  const uint32_t x_at = base + 2u * (uint32_t)((wm + (lane & 15)) * P::kPitch + (lane >> 4) * 8);
+  const uint32_t w_at = base + 2u * (uint32_t)((BM + wn + (lane & 7)) * P::kPitch + (lane >> 3 & 1) * 8);
+#pragma unroll
+  for (int i = 0; i < P::kRing - 1; ++i) fetch(i);
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(P::kRing - 2) : "memory");
+    __syncthreads();  // the step's words are there, and the tile has been read
+    const uint4* words = reinterpret_cast<const uint4*>(ring + (size_t)(step % P::kRing) * (P::kRows * P::kWords * 16));
+    const int valid = min(8, a.K - step * P::kK - v * 8);
+#pragma unroll
+    for (int i = 0; i < P::kPer; ++i) {
+      const int r = r0 + 32 * i;
+      if (P::kRows % 32 == 0 || r < P::kRows) {
+        uint4 e = make_uint4(0, 0, 0, 0);
+        if ((rows_in >> i & 1) && valid > 0)
+          e = eight_from(words[r * P::kWords + v], words[r * P::kWords + v + 1], (int)(shifts >> (4 * i) & 7) * 2, valid);
+        *reinterpret_cast<uint4*>(tile + r * P::kPitch + v * 8) = e;
+      }
     }
     __syncthreads();
-    if (k0 + kPlainK < a.K) fetch(k0 + kPlainK);
-    const int g = lane >> 2, q = (lane & 3) * 2;
+    fetch(step + P::kRing - 1);  // over the words of the step before this one
 #pragma unroll
-    for (int kk = 0; kk < kPlainK; kk += 16) {
-      uint32_t xf[2][4], wf[2][2];
+    for (int kk = 0; kk < P::kK; kk += 16) {
+      uint32_t xf[kM][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint16_t* p = xs + (wm + 16 * i + g) * kPlainPitch + kk + q;
-        xf[i][0] = *reinterpret_cast<const uint32_t*>(p);
-        xf[i][1] = *reinterpret_cast<const uint32_t*>(p + 8 * kPlainPitch);
-        xf[i][2] = *reinterpret_cast<const uint32_t*>(p + 8);
-        xf[i][3] = *reinterpret_cast<const uint32_t*>(p + 8 * kPlainPitch + 8);
-        const uint16_t* v = ws + (wn + 8 * i + g) * kPlainPitch + kk + q;
-        wf[i][0] = *reinterpret_cast<const uint32_t*>(v);
-        wf[i][1] = *reinterpret_cast<const uint32_t*>(v + 8);
+      for (int i = 0; i < kM; ++i) ldmatrix4(xf[i], x_at + 2u * (uint32_t)(16 * i * P::kPitch + kk));
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        uint32_t w0, w1;
+        ldmatrix2(w0, w1, w_at + 2u * (uint32_t)(8 * j * P::kPitch + kk));
+#pragma unroll
+        for (int i = 0; i < kM; ++i) mma_16x8x16<T>(acc[i][j], xf[i], w0, w1);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) mma_16x8x16<T>(acc[i][j], xf[i], wf[j]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < kN; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int e = 0; e < 2; ++e) {
+      const int n = n0 + wn + 8 * j + (lane & 3) * 2 + e;
+      if (n >= a.N) continue;
+      const float b = load_bias(a.bias, a.bias_type, n);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int m = m0 + wm + 16 * i + (lane >> 2) + (e >> 1) * 8, n = n0 + wn + 8 * j + (lane & 3) * 2 + (e & 1);
-        if (m < a.M && n < a.N) {
-          float v = activate_one(acc[i][j][e] + load_bias(a.bias, a.bias_type, n), a.act);
+      for (int i = 0; i < kM; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int m = m0 + wm + 16 * i + (lane >> 2) + 8 * h;
+          if (m >= a.M) continue;
+          float v = activate_one(acc[i][j][2 * h + e] + b, a.act);
           if (a.res != nullptr) v += to_float<OT>(static_cast<const OT*>(a.res)[(int64_t)m * a.ldr + n]);
           static_cast<OT*>(a.y)[(int64_t)m * a.ldy + n] = from_float<OT>(v);
         }
-      }
+    }
+}
+
+template <class T, class OT, int BM, int BN>
+cudaError_t launch_plain_tiles(const LinearCall& a, cudaStream_t s) {
+  const long long tiles = (long long)((a.N + BN - 1) / BN) * ((a.M + BM - 1) / BM);
+  if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
+  auto kern = linear_plain_kernel<T, OT, BM, BN>;
+  static SmemOptIn once;
+  cudaError_t e = opt_in_smem(once, kern);
+  if (e != cudaSuccess) return e;
+  return launch_behind(kern, (unsigned)tiles, kPlainThreads, PlainTile<BM, BN>::bytes(), s, a);
+}
+
+template <class T, class OT>
+cudaError_t launch_plain_for(const LinearCall& a, cudaStream_t s) {
+  // Few tokens need few rows of the tile; narrow weight tiles where wide ones would leave SMs without any.
+  if (a.M <= 16) return launch_plain_tiles<T, OT, 16, 64>(a, s);
+  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) < 148) return launch_plain_tiles<T, OT, 32, 64>(a, s);
+  return launch_plain_tiles<T, OT, 64, 128>(a, s);
 }
 
 template <class T>
 cudaError_t launch_plain(const LinearCall& a, cudaStream_t s) {
-  const long long tiles = (long long)((a.N + kPlainW - 1) / kPlainW) * ((a.M + kPlainTok - 1) / kPlainTok);
-  if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
-  const unsigned grid = (unsigned)tiles;
-  if (a.out_type == PM_F32) return launch_behind(linear_plain_kernel<T, float>, grid, 256, 0, s, a);
-  return launch_behind(linear_plain_kernel<T, T>, grid, 256, 0, s, a);
+  return a.out_type == PM_F32 ? launch_plain_for<T, float>(a, s) : launch_plain_for<T, T>(a, s);
 }
 
 // ---- launch plan ------------------------------------------------------------------------------------------

@@ -35,8 +35,10 @@
 namespace pm {
 namespace {
 
+using sm100::cluster_arrive_diverged;
 using sm100::cluster_rank;
 using sm100::cluster_sync;
+using sm100::cluster_wait_diverged;
 using sm100::map_to_rank;
 using sm100::smem_u32;
 
@@ -201,6 +203,7 @@ struct LogprobShared {
   Sums warp_sums[32];
   alignas(16) Sums part;  // this CTA's sums, read by rank 0
   Entry best[kMaxTop];    // this CTA's n best in order, read by rank 0
+  Entry merged[kMaxTop];  // the row's; 0 to begin with
   float seg[32];          // largest value of each group of threads so far
   int count, n_hot;
   int32_t hot[kCap];   // 16-byte vectors that held a value that reached the floor
@@ -275,6 +278,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   T at_target{};
   if (tid == 0 && rank == 0 && a.logp != nullptr) target = a.targets[row];
   if (tid == 0) sh.count = sh.n_hot = 0;
+  if (tid < kMaxTop) sh.merged[tid] = 0;
   __syncthreads();
   auto push = [&](Entry e) {
     const int at = atomicAdd(&sh.count, 1);
@@ -477,22 +481,21 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
                        : "r"(map_to_rank(smem_u32(&sh.part), lane)));
         join_lanes(t, 8);
         __syncwarp();
-        if (lane == 0) {
-          sh.part = t;
-          sh.count = 0;
-        }
+        if (lane == 0) sh.part = t;
       }
-      __syncthreads();
-      for (int i = tid; i < parts * n; i += THREADS) {
-        Entry e;
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(e) : "r"(map_to_rank(smem_u32(&sh.best[i % n]), i / n)));
-        if (e != 0) push(e);
-      }
+      // the parts' best, which fill the list whether there are that many or not (0 ranks behind every entry)
+      for (int i = tid; i < parts * n; i += THREADS)
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(sh.list[i]) : "r"(map_to_rank(smem_u32(&sh.best[i % n]), i / n)));
     }
-    cluster_sync();  // nobody leaves before its part was read
-    if (rank != 0) return;
-    if (n > 0) rank_list<THREADS>(sh.list, sh.count, sh.best, n);
+    cluster_arrive_diverged();  // the others leave once their parts were read, which the first one does not wait for
+    if (rank != 0) {
+      cluster_wait_diverged();
+      return;
+    }
+    __syncthreads();
+    if (n > 0) rank_list<THREADS>(sh.list, parts * n, sh.merged, n);
   }
+  const Entry* best = parts > 1 ? sh.merged : sh.best;
   __syncthreads();
 
   Sums t = sh.part;
@@ -549,6 +552,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     }
     if (bad) t.s = CUDART_NAN_F;
   }
+  if (parts > 1) cluster_wait_diverged();
   if (warp != 0) return;
   const bool dead = !(t.s > 0.f) || !(fabsf(t.m) < CUDART_INF_F);
   const float log_s = logf(t.s);
@@ -560,7 +564,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     if (a.entropy != nullptr) a.entropy[row] = dead ? CUDART_NAN_F : fmaf(-(float)kLn2, t.u / t.s, log_s);
   }
   if (lane < n) {
-    const Entry e = dead ? 0 : sh.best[lane];
+    const Entry e = dead ? 0 : best[lane];
     a.top_ids[(int64_t)row * n + lane] = e == 0 ? -1 : (int32_t)(0xffffffffu - (uint32_t)e);
     a.top_logp[(int64_t)row * n + lane] =
         dead ? CUDART_NAN_F : e == 0 ? -CUDART_INF_F : (float)((double)value_of((uint32_t)(e >> 32)) - lse);
