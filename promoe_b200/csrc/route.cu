@@ -1,5 +1,13 @@
 // Stateless router on given logits: the experts of every token and their weights (route_select.cuh has the rule).
 // One warp per token, the row in registers: lane i holds npl = ceil(E / 32) neighbouring experts.
+//
+// Bound by instructions, not by bytes: 16384 rows of 256 float32 logits are 16.8 MB, 2.6 us at the measured copy rate, and take
+// 11.9 us for 8 of softmax scores (570 instructions a row), 13.5 us
+// with sigmoid scores and a bias, 20 us with the best 4 of 8 groups as well (820 instructions a row). One token to 64 take
+// 3.1 us, launch included. What it took to get there (the last case): integer divisions and group geometry out of the loop over
+// rows, numbers ranked as numbers (redux.sync of floats) instead of as ordered integers: 28 -> 22 us; the exact ranking of a row
+// with close neighbours by its candidates alone, one lane each, instead of all its experts: 64 tokens, one of them such a
+// row, 9.7 -> 3.9 us.
 #include <algorithm>
 
 #include "route_select.cuh"
@@ -15,8 +23,13 @@ __device__ __forceinline__ float load_logit(const float* p) { return *p; }
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float load_logit(const __half* p) { return __half2float(*p); }
 
+// Resident blocks, each row of warps taking one token after the other. More of them with fewer registers: 256 experts in groups
+// 20.3 -> 22 us (8 blocks), 512 experts 10.9 -> 12.0 us (5); one block per four tokens instead, launched one after another:
+// 25 us.
+constexpr int blocks_per_sm(int npl) { return npl <= 8 ? 6 : npl <= 16 ? 4 : 3; }
+
 template <class T, int NPL>
-__global__ void __launch_bounds__(kRouteWarps * 32, NPL <= 8 ? 8 : 4)
+__global__ void __launch_bounds__(kRouteWarps * 32, blocks_per_sm(NPL))
 route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_constant__ RouteRule rule, int vector_loads,
              int32_t* __restrict__ topk_ids, float* __restrict__ topk_w) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -27,6 +40,7 @@ route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_c
 
   float b[NPL];
   const float bias_max = load_choice_bias<NPL>(rule, npl, lane, b);
+  const RouteGroups groups(rule, npl, lane);
   constexpr int kVec = 16 / sizeof(T);
   float l[NPL];
   auto load = [&](int64_t t) {
@@ -54,7 +68,7 @@ route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_c
   for (int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp; t < n_tok; t += step) {
     load(t);
     const T* row = logits + t * ld;
-    route_token<NPL>(l, npl, rule, b, bias_max, scratch, lane, [&](int e) { return load_logit(row + e); },
+    route_token<NPL>(l, npl, rule, b, bias_max, groups, scratch, lane, [&](int e) { return load_logit(row + e); },
                      [&](int j, int id, float w) {
                        topk_ids[t * rule.k + j] = id;
                        topk_w[t * rule.k + j] = w;
@@ -71,8 +85,8 @@ cudaError_t launch(const T* logits, int64_t ld, int n_tok, const RouteRule& rule
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-  // One row after the other per warp once every SM has its 48 warps; at most 34 KB of shared memory per block.
-  const int blocks = std::min((n_tok + kRouteWarps - 1) / kRouteWarps, sms * 48 / kRouteWarps);
+  // One row after the other per warp once every SM has its blocks; at most 35 KB of shared memory per block.
+  const int blocks = std::min((n_tok + kRouteWarps - 1) / kRouteWarps, sms * blocks_per_sm(NPL));
   return launch_behind(route_kernel<T, NPL>, blocks, kRouteWarps * 32, kRouteWarps * route_scratch_bytes(rule.E), s, logits, ld,
                        n_tok, rule, vector_loads, ids, w);
 }
@@ -80,8 +94,10 @@ cudaError_t launch(const T* logits, int64_t ld, int n_tok, const RouteRule& rule
 template <class T>
 cudaError_t pick(const T* logits, int64_t ld, int n_tok, const RouteRule& rule, int32_t* ids, float* w, cudaStream_t s) {
   const int npl = (rule.E + 31) / 32;
+  // Registers of a lane: the next size up. 4096 rows of 512 experts in 16 registers 10.9 us, in 32 of them 18.8 us.
   if (npl <= 2) return launch<T, 2>(logits, ld, n_tok, rule, ids, w, s);
   if (npl <= 8) return launch<T, 8>(logits, ld, n_tok, rule, ids, w, s);
+  if (npl <= 16) return launch<T, 16>(logits, ld, n_tok, rule, ids, w, s);
   return launch<T, 32>(logits, ld, n_tok, rule, ids, w, s);
 }
 

@@ -21,16 +21,33 @@
 
 namespace pm {
 
-// Numbers as integers in the same order; the key of -inf, kNone, stands for what cannot be chosen.
-constexpr uint32_t kNone = 0x007fffffu;
-__device__ __forceinline__ uint32_t order_key(float v) {  // not for -0
+// The choice of what cannot be chosen is -inf.
+
+// The largest of a warp's numbers, in one instruction; no NaN among them.
+__device__ __forceinline__ float warp_top(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ uint32_t order_key(float v) {  // integers in the order of the numbers; not for -0
   const uint32_t b = __float_as_uint(v);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// Lanes that share a group: the same power of two for each of G <= 32 groups.
-__device__ __forceinline__ int lanes_per_group(int G) { return 1 << (31 - __clz(32 / G)); }
+// A lane's place in the rule's groups.
+struct RouteGroups {
+  int lanes;     // that share the valuation of a group: the same power of two for each of at most 32 groups
+  int per;       // experts of a group
+  int group;     // this lane's, n_group and more without one
+  bool aligned;  // lane i's own experts all belong to its group
+  __device__ __forceinline__ RouteGroups(const RouteRule& r, int npl, int lane) {
+    const int shift = 31 - __clz(32 / r.n_group);
+    lanes = 1 << shift;
+    per = r.E / r.n_group;
+    group = lane >> shift;
+    aligned = npl * 32 == r.E && 32 % r.n_group == 0;
+  }
+};
 
 // ---- the same ranking in 64 bits; c[E] is shared memory of the warp ------------------------------------------
 // Logits in c become choices.
@@ -53,6 +70,27 @@ static __device__ __noinline__ void exact_choices(double* c, const RouteRule* ru
     c[e] = l == -CUDART_INF || v != v ? -CUDART_INF : v;
   }
   __syncwarp();
+}
+
+// The sum behind the softmax scores; c holds the logits.
+static __device__ __noinline__ double exact_sum(const double* c, int E, double top, int lane) {
+  double sum = 0.0;
+  __syncwarp();
+  for (int e = lane; e < E; e += 32) sum += exp(c[e] - top);
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  return sum;
+}
+
+// Rank of each of the n <= 32 candidates, one per lane in the order of their ids, by a choice that `sum` (softmax) makes exact.
+static __device__ __noinline__ int exact_candidates(double logit, float bias, double top, double sum, int sigmoid, int n, int lane) {
+  const double v = (sigmoid ? 1.0 / (1.0 + exp(-logit)) : exp(logit - top) / sum) + (double)bias;
+  int rank = 0;
+  for (int i = 0; i < n; ++i) {
+    const double o = __shfl_sync(0xffffffffu, v, i);
+    rank += o > v || (o == v && i < lane);
+  }
+  return lane < n ? rank : 32;
 }
 
 // The groups that stay, as bits.
@@ -115,14 +153,17 @@ static __device__ __noinline__ int exact_rank(double* c, const RouteRule* rule, 
 // their ids, and each counts how many rank before it. Where more than 32 experts reach the floor (many equal logits,
 // large k) there are k rounds of arg-max over all experts instead.
 struct alignas(16) RouteScratch {  // shared memory of one warp, followed by E doubles
-  uint32_t key[36];                // candidates; then their values in rank order
-  uint32_t id[36];
+  uint32_t key[36];                // candidates as ordered integers; then their choices in rank order
+  float2 candidate[32];            // choice and id
 };
 __host__ __device__ __forceinline__ size_t route_scratch_bytes(int E) { return sizeof(RouteScratch) + 8 * (size_t)((E + 1) / 2 * 2); }
 
-__device__ __forceinline__ float fast_sigmoid(float l) {  // off by 2e-7; 0 for -inf, 1 for +inf
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + exp2f(l * -1.4426950408889634f)));
+// Off by less than 3e-7: the exponential by 2^-22 of itself and by what half a step of its argument makes of it, which moves
+// the quotient by a quarter of that at most; the sum by half a step, the reciprocal by one. 0 for -inf, 1 for +inf.
+__device__ __forceinline__ float fast_sigmoid(float l) {
+  float t, y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(l * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.f + t));
   return y;
 }
 
@@ -142,17 +183,18 @@ __device__ __forceinline__ float load_choice_bias(const RouteRule& r, int npl, i
 }
 
 // Row of a token: experts lane * npl .. lane * npl + npl - 1 are l[0 .. npl) of this lane (-inf beyond E; npl <= NPL), b and
-// bias_max from load_choice_bias. logit(e) reads the row again. write(j, id, weight) is called once for each j < k, by any lane.
+// bias_max from load_choice_bias, groups of this lane. logit(e) reads the row again. write(j, id, weight) is called once for each j < k, by any lane.
 template <int NPL, class Logit, class Write>
 __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, const RouteRule& r, const float (&b)[NPL], float bias_max,
-                                            RouteScratch* scratch, int lane, const Logit& logit, const Write& write) {
+                                            const RouteGroups& groups, RouteScratch* scratch, int lane, const Logit& logit, const Write& write) {
   const int E = r.E, e0 = lane * npl;
   double* work = reinterpret_cast<double*>(scratch + 1);
   const bool by_logit = r.bias == nullptr, grouped = r.n_group > 1 && r.topk_group < r.n_group, sums = grouped && r.group_top2 != 0;
   bool odd = false;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) odd |= !(l[j] < CUDART_INF_F);
-  if (__any_sync(0xffffffffu, odd)) {
+  for (int j = 0; j < NPL; ++j) odd |= !(fabsf(l[j]) < CUDART_INF_F);
+  odd = __any_sync(0xffffffffu, odd);
+  if (odd) {
     bool dead = false;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) dead |= l[j] != l[j] || (!r.sigmoid && l[j] == CUDART_INF_F);
@@ -161,124 +203,121 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       return;
     }
   }
-  // A float32 score is off by at most 1e-6 of the largest (the exponential's argument is off by half a step, the
-  // exponential and the division by about two), a choice by that and half a step of its own.
+  // How far apart two float32 choices have to be for their order to be certain: twice the error of one. A sigmoid score is
+  // off by 3e-7, a softmax score by 1.5e-6 of the largest (the sum of up to 37 roundings, the exponential and the division by
+  // two or three), a choice by that and half a step of its own.
   float sum = 0.f, top = 0.f, margin = 0.f;
-  uint32_t key[NPL];  // ordered choices
+  float c[NPL];  // choices
   if (!r.sigmoid) {
     top = -CUDART_INF_F;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) top = fmaxf(top, l[j]);
-    top = key_value(__reduce_max_sync(0xffffffffu, order_key(top)));
+    top = warp_top(top);
     if (top == -CUDART_INF_F) top = 0.f;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
-      const float e = __expf(l[j] - top);
-      key[j] = __float_as_uint(e);
-      sum += e;
+      c[j] = __expf(l[j] - top);
+      sum += c[j];
     }
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   }
   if (!by_logit || sums) {
     const float inv = r.sigmoid ? 1.f : 1.f / sum;
-    margin = 4e-6f * (inv + bias_max);
+    margin = (r.sigmoid ? 1e-6f : 4e-6f * inv) + 1e-6f * bias_max;
     if (r.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = __float_as_uint(fast_sigmoid(l[j]) + b[j]);
+      for (int j = 0; j < NPL; ++j) c[j] = fast_sigmoid(l[j]) + b[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = __float_as_uint(fmaf(__uint_as_float(key[j]), inv, b[j]));
+      for (int j = 0; j < NPL; ++j) c[j] = fmaf(c[j], inv, b[j]);
     }
+    if (odd) {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) key[j] = l[j] > -CUDART_INF_F ? order_key(__uint_as_float(key[j])) : kNone;
+      for (int j = 0; j < NPL; ++j) c[j] = l[j] > -CUDART_INF_F ? c[j] : -CUDART_INF_F;
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) key[j] = order_key(l[j] + 0.f);
+    for (int j = 0; j < NPL; ++j) c[j] = l[j] + 0.f;  // no -0
   }
-  auto stage_exact = [&]() {
+  auto stage_logits = [&]() {
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
       if (j < npl && e0 + j < E) work[e0 + j] = (double)l[j];
-    exact_choices(work, &r, lane);
   };
-  bool staged = false;
-  uint32_t kept = 0xffffffffu;
+  uint32_t lanes_in = 0xffffffffu;  // lanes whose group stays
+  auto kept_groups = [&]() {        // the same as bits of groups
+    uint32_t kept = 0u;
+    for (int g = 0; g < r.n_group; ++g) kept |= ((lanes_in >> (g * groups.lanes)) & 1u) << g;
+    return kept;
+  };
   if (grouped) {
-    const int G = r.n_group, per = E / G, L = lanes_per_group(G);
-    const bool aligned = npl * 32 == E && 32 % G == 0;  // lane i's experts all belong to group i / L
-    const int group = lane / L;                         // this lane's share of the valuation, and with `aligned` its experts'
-    uint32_t a = kNone, a2 = kNone;                     // the two best of it
-    auto take = [&](uint32_t v) {
-      a2 = max(a2, min(a, v));
-      a = max(a, v);
+    const int G = r.n_group, per = groups.per, L = groups.lanes, group = groups.group;
+    const bool aligned = groups.aligned;
+    float a = -CUDART_INF_F, a2 = -CUDART_INF_F;  // the two best of this lane's share of its group
+    auto take = [&](float v) {
+      a2 = fmaxf(a2, fminf(a, v));
+      a = fmaxf(a, v);
     };
     if (aligned) {
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) take(key[j]);
+      for (int j = 0; j < NPL; ++j) take(c[j]);
     } else {
-      uint32_t* all = reinterpret_cast<uint32_t*>(work);
+      float* all = reinterpret_cast<float*>(work);
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < NPL; ++j)
-        if (j < npl && e0 + j < E) all[e0 + j] = key[j];
+        if (j < npl && e0 + j < E) all[e0 + j] = c[j];
       __syncwarp();
-      const int q = lane % L, steps = (per + L - 1) / L;
+      const int q = lane & (L - 1), steps = (per + L - 1) / L;
       if (group < G) {
         int x = group % steps;  // groups start at different steps, so that they meet different banks
         for (int i = 0; i < steps; ++i) {
           const int at = q + L * x;
-          take(at < per ? all[group * per + at] : kNone);
+          take(at < per ? all[group * per + at] : -CUDART_INF_F);
           if (++x == steps) x = 0;
         }
       }
     }
     for (int m = L >> 1; m >= 1; m >>= 1) {
-      const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, m), ob = __shfl_xor_sync(0xffffffffu, a2, m);
-      a2 = max(max(a2, ob), min(a, oa));
-      a = max(a, oa);
+      const float oa = __shfl_xor_sync(0xffffffffu, a, m), ob = __shfl_xor_sync(0xffffffffu, a2, m);
+      a2 = fmaxf(fmaxf(a2, ob), fminf(a, oa));
+      a = fmaxf(a, oa);
     }
-    uint32_t value = a;  // the same in every lane of a group; kNone in lanes without one
-    if (sums && a2 != kNone) value = order_key(key_value(a) + key_value(a2) + 0.f);
-    bool in = false;
-    float last = 0.f;
-    for (int i = 0; i < r.topk_group; ++i) {
-      const uint32_t m = __reduce_max_sync(0xffffffffu, value);
-      if (m == kNone) break;
-      bool mine = value == m;
-      const unsigned who = __ballot_sync(0xffffffffu, mine);
-      if (__popc(who) != L) mine = group == (__ffs(who) - 1) / L;  // equal groups: the lowest
-      in |= mine;
-      if (mine) value = kNone;
-      last = key_value(m);
+    float value = a;  // the same in every lane of a group; -CUDART_INF_F in lanes without one
+    if (sums && a2 > -CUDART_INF_F) value = a + a2;
+    int before = 0;  // groups that rank before this one
+    for (int g = 0; g < G; ++g) {
+      const float o = __shfl_sync(0xffffffffu, value, g * L);
+      before += g < group ? o >= value : o > value;
     }
-    kept = __ballot_sync(0xffffffffu, in);
-    const uint32_t next = __reduce_max_sync(0xffffffffu, value);
-    const bool close = (!by_logit || sums) && next != kNone && last - key_value(next) < 2.f * margin;  // sums of two choices
-    if (L > 1) {  // from bits of lanes to bits of groups
-      uint32_t of_groups = 0u;
-      for (int g = 0; g < G; ++g) of_groups |= ((kept >> (g * L)) & 1u) << g;
-      kept = of_groups;
+    bool in = before < r.topk_group && value > -CUDART_INF_F;
+    bool close = false;
+    if (!by_logit || sums) {  // sums of two choices
+      const float next = warp_top(in ? -CUDART_INF_F : value), last = -warp_top(in ? -value : -CUDART_INF_F);
+      close = next > -CUDART_INF_F && last - next < 2.f * margin;
     }
     if (close) {
-      stage_exact();
-      staged = true;
-      kept = exact_groups(work, &r, lane);
+      stage_logits();
+      exact_choices(work, &r, lane);
+      const uint32_t kept = exact_groups(work, &r, lane);
       in = (kept >> group) & 1u;
     }
+    lanes_in = __ballot_sync(0xffffffffu, in);
     if (by_logit && sums) {  // from here on by the logits
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = order_key(l[j] + 0.f);
+      for (int j = 0; j < NPL; ++j) c[j] = l[j] + 0.f;
     }
     if (aligned) {
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = in ? key[j] : kNone;
+      for (int j = 0; j < NPL; ++j) c[j] = in ? c[j] : -CUDART_INF_F;
     } else {
+      const uint32_t kept = kept_groups();
       int g = e0 / per, rem = e0 - g * per;
 #pragma unroll
       for (int j = 0; j < NPL; ++j) {
-        if (!((kept >> (g & 31)) & 1u)) key[j] = kNone;
+        if (!((kept >> (g & 31)) & 1u)) c[j] = -CUDART_INF_F;
         if (++rem == per) {
           rem = 0;
           ++g;
@@ -287,21 +326,22 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
     }
   }
   const int want = by_logit ? r.k : r.k + 1;  // one more to compare the last with
-  uint32_t floor_key = kNone;
+  float floor = -CUDART_INF_F;
   {
-    uint32_t best = kNone;
+    float best = -CUDART_INF_F;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) best = max(best, key[j]);
+    for (int j = 0; j < NPL; ++j) best = fmaxf(best, c[j]);
     for (int i = 0; i < want; ++i) {  // equal maxima leave together, which only lowers the floor
-      floor_key = __reduce_max_sync(0xffffffffu, best);
-      if (floor_key == kNone) break;
-      if (best == floor_key) best = kNone;
+      floor = warp_top(best);
+      if (best == floor) best = -CUDART_INF_F;
     }
   }
-  floor_key = max(floor_key, kNone + 1u);  // fewer lanes than that: everything that can be chosen
+  // Fewer lanes than that: everything that can be chosen. Else also what float32 may have put below the floor.
+  if (!by_logit) floor -= margin;
+  floor = fmaxf(floor, -3.402823466e38f);
   int mine = 0;
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) mine += key[j] >= floor_key;
+  for (int j = 0; j < NPL; ++j) mine += c[j] >= floor;
   int before = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -310,21 +350,23 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   }
   const int n = __shfl_sync(0xffffffffu, before, 31);
   before -= mine;
-  bool close = false;
   int rank = 32, id = -1;
+  float v_id = 0.f;  // the logit of id
   __syncwarp();
   if (n <= 32) {
-    scratch->key[lane] = 0u;
+    scratch->candidate[lane].x = -CUDART_INF_F;
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < NPL; ++j)
-      if (key[j] >= floor_key) {
-        scratch->key[before] = key[j];
-        scratch->id[before] = (uint32_t)(e0 + j);
+      if (c[j] >= floor) {
+        scratch->candidate[before] = make_float2(c[j], __int_as_float(e0 + j));
         ++before;
       }
     __syncwarp();
-    const uint32_t v = scratch->key[lane];
+    const float choice = scratch->candidate[lane].x;
+    const uint32_t v = order_key(choice);
+    scratch->key[lane] = v;
+    __syncwarp();
     const uint4* four = reinterpret_cast<const uint4*>(scratch->key);
     rank = 0;
     for (int i = 0; i < n; i += 4) {  // of equals the one in the lower lane, with the lower id, ranks first
@@ -332,61 +374,70 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       rank += (o.x + (i < lane ? 1u : 0u) > v) + (o.y + (i + 1 < lane ? 1u : 0u) > v) + (o.z + (i + 2 < lane ? 1u : 0u) > v) +
               (o.w + (i + 3 < lane ? 1u : 0u) > v);
     }
-    if (lane < n) id = (int)scratch->id[lane];
-    else rank = 32;
+    if (lane < n) {
+      id = __float_as_int(scratch->candidate[lane].y);
+      v_id = logit(id);
+    } else {
+      rank = 32;
+    }
     if (!by_logit) {
       __syncwarp();
-      if (lane < n) scratch->key[rank] = v;
+      if (lane < n) scratch->key[rank] = __float_as_uint(choice);
       __syncwarp();
-      const uint32_t next = lane < n && rank + 1 < n ? scratch->key[rank + 1] : 0u;
-      close = __any_sync(0xffffffffu, rank < r.k && next != 0u && key_value(v) - key_value(next) < margin);
+      const bool close = rank < r.k && rank + 1 < n && choice - __uint_as_float(scratch->key[rank + 1]) < margin;
+      if (__any_sync(0xffffffffu, close)) {
+        double sum64 = 1.0;
+        if (!r.sigmoid) {
+          stage_logits();
+          sum64 = exact_sum(work, E, (double)top, lane);
+        }
+        rank = exact_candidates((double)v_id, lane < n ? r.bias[id] : 0.f, (double)top, sum64, r.sigmoid, n, lane);
+      }
     }
   } else {
     // k rounds: the best of every lane, the warp's best of those; a lane keeps the first of equals
-    uint32_t best = kNone;
+    float best = -CUDART_INF_F;
     int at = 0;
     auto scan = [&]() {
-      best = kNone;
+      best = -CUDART_INF_F;
 #pragma unroll
       for (int j = 0; j < NPL; ++j)
-        if (key[j] > best) {
-          best = key[j];
+        if (c[j] > best) {
+          best = c[j];
           at = j;
         }
     };
     scan();
     float last = 0.f;
+    bool close = false;
     for (int i = 0; i < want && !close; ++i) {
-      const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-      if (m == kNone) break;
+      const float m = warp_top(best);
+      if (m == -CUDART_INF_F) break;
       const int win = __ffs(__ballot_sync(0xffffffffu, best == m)) - 1;
       const int e = __shfl_sync(0xffffffffu, e0 + at, win);
       if (!by_logit) {
-        const float v = key_value(m);
-        if (i > 0) close = last - v < margin;
-        last = v;
+        if (i > 0) close = last - m < margin;
+        last = m;
       }
       if (i < r.k && lane == i) id = e;
       if (lane == win) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-          if (j == at) key[j] = kNone;
+          if (j == at) c[j] = -CUDART_INF_F;
         scan();
       }
     }
+    if (close) {
+      stage_logits();
+      exact_choices(work, &r, lane);
+      id = exact_rank(work, &r, kept_groups(), lane);
+    }
     rank = lane;
-  }
-  if (close) {
-    if (!staged) stage_exact();
-    id = exact_rank(work, &r, kept, lane);
-    rank = lane;
+    if (id >= 0) v_id = logit(id);
   }
   const bool chosen = id >= 0 && rank < r.k;
   float w = 0.f;
-  if (chosen) {
-    const float v = logit(id);
-    w = r.sigmoid ? __fdividef(1.f, 1.f + expf(-v)) : __fdividef(expf(v - top), sum);
-  }
+  if (chosen) w = r.sigmoid ? __fdividef(1.f, 1.f + expf(-v_id)) : __fdividef(expf(v_id - top), sum);
   if (r.norm) {
     float all = w;
 #pragma unroll
