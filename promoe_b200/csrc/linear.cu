@@ -42,6 +42,7 @@ struct LinearTc {
   int32_t atoms, stage_bytes, n_stages;  // 64-k atoms of a step; k_tiles counts steps
   int32_t chunk;                         // steps that one accumulator takes
   int32_t split, part_offset, shared_bytes;  // CTAs (pairs) on a tile; their partial sums behind the ring; all of these bytes
+  int32_t part_cols;                         // columns that each of them finishes, a multiple of 4
   int32_t tmem_cols;
   int32_t* err;
 };
@@ -164,37 +165,47 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   const int first = blockIdx.x / per_tile, step = gridDim.x / per_tile;
   const int n_tiles = a.w_tiles * a.tok_tiles, n_stages = a.n_stages;
   const bool split = a.split > 1;
-  const int k0 = split ? (int)((long long)a.k_tiles * part_rank / a.split) : 0;
-  const int k1 = split ? (int)((long long)a.k_tiles * (part_rank + 1) / a.split) : a.k_tiles;
+  const int k0 = split ? a.k_tiles * (int)part_rank / a.split : 0;  // k_tiles <= 2^25, split <= 8
+  const int k1 = split ? a.k_tiles * ((int)part_rank + 1) / a.split : a.k_tiles;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < n_stages; ++s) {
-      mbar_init(&sh.full[s], 2);  // the two producers
-      mbar_init(&sh.empty[s], 1);
+  if (warp == 0) {
+    if (lane == 0) prefetch_tensor_map(&map_w);
+    if (lane < n_stages) {
+      mbar_init(&sh.full[lane], 2);  // the two producers
+      mbar_init(&sh.empty[lane], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.acc_full[i], 1);
-      mbar_init(&sh.acc_empty[i], CG * kEpiWarps);
+    if (lane < 2) {
+      mbar_init(&sh.acc_full[lane], 1);
+      mbar_init(&sh.acc_empty[lane], CG * kEpiWarps);
     }
-    sh.abort = 0;
+    if (lane == 0) sh.abort = 0;
     fence_barrier_init();
+    __syncwarp();
   }
+  if (warp == 3 && lane == 0) prefetch_tensor_map(&map_x);
   if (warp == 2) {
     if (CG == 2) tmem_alloc(&sh.tmem_base, a.tmem_cols);
     else tmem_alloc_single(&sh.tmem_base, a.tmem_cols);
   }
   tc_fence_before();
-  __syncthreads();
-  if (CG == 2) cluster_sync_diverged();
-  else if (split) cluster_arrive_diverged();  // waited for before the partial sums are sent
+  if (CG == 2) {
+    __syncthreads();
+    cluster_sync_diverged();
+  } else {
+    // The weights' producer needs nothing but its own barriers: it goes ahead, by some 500 ns.
+    if (warp == 0) asm volatile("barrier.cta.arrive 1, %0;" ::"n"(kTcThreads) : "memory");
+    else asm volatile("barrier.cta.sync 1, %0;" ::"n"(kTcThreads) : "memory");
+    if (split) cluster_arrive_diverged();  // waited for before the partial sums are sent
+  }
   tc_fence_after();
-  const uint32_t tmem_base = sh.tmem_base;
+  const uint32_t tmem_base = sh.tmem_base;    // not yet there for warp 0, which does not use it
   const uint32_t acc_cols = a.tmem_cols / 2;  // distance of the two accumulators
-  let_successor_start();
+  if (CG == 2 || warp != 0) let_successor_start();  // not before the tensor memory is allocated
   wait_for_predecessor();
 
   const uint32_t full0 = smem_u32(&sh.full[0]), empty0 = smem_u32(&sh.empty[0]), stage0 = smem_u32(stages);
   const int lead = CG == 2 ? (int)(cta & ~1u) : 0;  // the pair's first CTA
+  float bias = 0.f;
   if ((warp == 0 || warp == 3) && lane == 0) {
     // ---- producers: one thread for this CTA's 128 weight rows, one for its share of the token rows ------------------
     const bool tokens = warp == 3;
@@ -270,7 +281,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         if (ok) umma_commit_at<CG>(smem_u32(&sh.acc_full[acc]), both);
       }
     if (!ok) sh.abort = 1;
-  } else if (warp >= 4) {
+  } else if (warp >= 4) {  // `bias` of this lane's row stays for the joining of partial sums
     // ---- epilogue: warp w drains accumulator rows 32w .. 32w+31, two warps of a quadrant share the columns ------
     const int w = warp & 3, half = (warp - 4) >> 2;
     const float nan = __int_as_float(0x7fffffff);
@@ -282,26 +293,28 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       tile_at(a, tile, wt, tt);
       const int n = (wt * CG + (int)rank) * 128 + 32 * w + lane;
       const int m0 = tt * a.width, cols = min(a.width, a.M - m0);
-      const float b = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
+      bias = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
       auto give = [&](float (&o)[16], int c0) {
         if (!ok) {
 #pragma unroll
           for (int c = 0; c < 16; ++c) o[c] = nan;
         }
         if (!split) {
-          finish<OT, 16>(a, o, b, m0 + c0, n, n < a.N ? cols - c0 : 0);
+          finish<OT, 16>(a, o, bias, m0 + c0, n, n < a.N ? cols - c0 : 0);
         } else {
-          // column c0 + c to the CTA that finishes it, which keeps [source][its columns][128 rows]
-          const int per = (a.width + a.split - 1) / a.split;
-          const uint32_t mine = stage0 + a.part_offset + 4u * (uint32_t)((int)part_rank * per * 128 + 32 * w + lane);
+          // four columns at a time to the CTA that finishes them, which keeps [source][its fours of columns][128 rows][4]
+          const int per = a.part_cols;
+          const uint32_t mine = stage0 + a.part_offset + 16u * (uint32_t)((int)part_rank * (per >> 2) * 128 + 32 * w + lane);
           int owner = c0 / per, at = c0 - owner * per;
           uint32_t dst = map_to_rank(mine, CG * owner + rank) + 512u * (uint32_t)at;
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
+          for (int c = 0; c < 16; c += 4)
             if (c0 + c < cols) {
-              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(o[c]) : "memory");
-              dst += 512;
-              if (++at == per) {
+              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(o[c]), "f"(o[c + 1]), "f"(o[c + 2]),
+                           "f"(o[c + 3]) : "memory");
+              dst += 2048;
+              at += 4;
+              if (at == per) {
                 at = 0;
                 ++owner;
                 if (owner < a.split) dst = map_to_rank(mine, CG * owner + rank);
@@ -364,19 +377,18 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     if (warp >= 4) {
       int wt, tt;
       tile_at(a, first, wt, tt);
-      const int per = (a.width + a.split - 1) / a.split, c_first = (int)part_rank * per;
+      const int per = a.part_cols, c_first = (int)part_rank * per;
       const int m0 = tt * a.width, mine = min(per, min(a.width, a.M - m0) - c_first);
-      const float* part = reinterpret_cast<const float*>(stages + a.part_offset);
       const int row = (warp & 3) * 32 + lane, n = (wt * CG + (int)rank) * 128 + row;
-      const float b = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
       for (int c0 = ((warp - 4) >> 2) * 8; c0 < mine; c0 += 16) {
         float o[8] = {};
-        for (int r = 0; r < a.split; ++r) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            if (c0 + c < mine) o[c] += part[(r * per + c0 + c) * 128 + row];
+        const float4* part = reinterpret_cast<const float4*>(stages + a.part_offset) + (c0 >> 2) * 128 + row;
+        for (int r = 0; r < a.split; ++r, part += (per >> 2) * 128) {
+          const float4 u = part[0], v = c0 + 4 < per ? part[128] : make_float4(0.f, 0.f, 0.f, 0.f);
+          o[0] += u.x, o[1] += u.y, o[2] += u.z, o[3] += u.w;
+          o[4] += v.x, o[5] += v.y, o[6] += v.z, o[7] += v.w;
         }
-        finish<OT, 8>(a, o, b, m0 + c_first + c0, n, n < a.N ? mine - c0 : 0);
+        finish<OT, 8>(a, o, bias, m0 + c_first + c0, n, n < a.N ? mine - c0 : 0);
       }
     }
   }
@@ -388,7 +400,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
-  if (CG == 2 || split) cluster_sync_diverged();
+  if (CG == 2) cluster_sync_diverged();
   tc_fence_after();
   if (warp == 2) {
     if (CG == 2) tmem_dealloc(tmem_base, a.tmem_cols);
@@ -737,7 +749,8 @@ int launch_linear(const LinearCall& a, cudaStream_t s) {
   t.chunk = promote ? kPromoteK / 64 / c.atoms : t.k_tiles;
   t.split = c.split; t.err = a.err;
   t.stage_bytes = c.atoms * (kWBytes + c.width / c.cg * 128);
-  const int part_bytes = c.split > 1 ? (c.width + c.split - 1) / c.split * c.split * 512 : 0;
+  t.part_cols = ((c.width + c.split - 1) / c.split + 3) & ~3;
+  const int part_bytes = c.split > 1 ? t.part_cols * c.split * 512 : 0;
   const int room = kSmemMost - 1024 - (int)sizeof(LinShared) - part_bytes, steps = (t.k_tiles + c.split - 1) / c.split;
   const long long n_tiles = (long long)t.w_tiles * t.tok_tiles, units = cap[c.cg * c.split];
   const long long tiles_each = c.split > 1 ? 1 : (n_tiles + units - 1) / units;
