@@ -599,6 +599,171 @@ cudaError_t launch_plain(const LinearCall& a, cudaStream_t s) {
   return a.out_type == PM_F32 ? launch_plain_for<T, float>(a, s) : launch_plain_for<T, T>(a, s);
 }
 
+// ---- few tokens -----------------------------------------------------------------------------------------
+// 16 RT weight rows per CTA, its warps on one step of 64 k after the other in turn (mma.sync; weight rows are its M operand, MT
+// tiles of eight tokens its N operand). A lane loads 16 bytes of a row, eight neighbouring k, and gives them to two MMAs as
+// the k it has there: both operands come in the same order, so that neither goes through shared memory. Weights pass the L1
+// by, two steps of a warp are under way at a time. The warps' sums are added in order through shared memory.
+// Bound by the weights' way from HBM, once a launch has started: 8 x 3584 -> 4608 (33 MB) takes 7.4 us, of which 5.0 are the
+// bytes at the measured copy rate. The tensor-core kernel needs 3 us more for its setup, the joining of partial sums and the
+// longer way of the operands.
+
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+// Eight values from `at` on of which `left` lie inside the row; the others are zero.
+template <class T>
+__device__ __forceinline__ uint4 load_end(const T* row, int left) {
+  if (left >= 8) return *reinterpret_cast<const uint4*>(row);
+  uint4 v = make_uint4(0, 0, 0, 0);
+  const unsigned short* src = reinterpret_cast<const unsigned short*>(row);
+  if (left > 0) v.x = src[0];
+  if (left > 1) v.x |= (uint32_t)src[1] << 16;
+  if (left > 2) v.y = src[2];
+  if (left > 3) v.y |= (uint32_t)src[3] << 16;
+  if (left > 4) v.z = src[4];
+  if (left > 5) v.z |= (uint32_t)src[5] << 16;
+  if (left > 6) v.w = src[6];
+  return v;
+}
+
+template <class T, class OT, int RT, int MT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(const __grid_constant__ LinearCall a) {
+  __shared__ float part[WARPS][MT * 8][16 * RT + 4];  // the lanes of a store meet different banks
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16 * RT, steps = a.K / 64;
+  let_successor_start();
+  wait_for_predecessor();
+  const T *w[2 * RT], *x[MT];  // rows beyond the last are the last again, their sums are not used
+#pragma unroll
+  for (int i = 0; i < 2 * RT; ++i) w[i] = static_cast<const T*>(a.w) + (int64_t)min(n0 + g + 8 * i, a.N - 1) * a.ldw + 8 * t;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) x[i] = static_cast<const T*>(a.x) + (int64_t)min(g + 8 * i, a.M - 1) * a.ldx + 8 * t;
+
+  struct Step {
+    uint4 w[2 * RT][2], x[MT][2];
+  };
+  auto load = [&](Step& s, int step) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) s.w[i][h] = load_once(w[i] + step * 64 + 32 * h);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) s.x[i][h] = *reinterpret_cast<const uint4*>(x[i] + step * 64 + 32 * h);
+    }
+  };
+  float acc[RT][MT][4] = {}, sum[RT][MT][4] = {};
+  auto multiply = [&](const Step& s) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const uint4 lo = s.w[2 * r][h], hi = s.w[2 * r + 1][h];
+        const uint32_t first[4] = {lo.x, hi.x, lo.y, hi.y}, second[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          mma_16x8x16<T>(acc[r][i], first, s.x[i][h].x, s.x[i][h].y);
+          mma_16x8x16<T>(acc[r][i], second, s.x[i][h].z, s.x[i][h].w);
+        }
+      }
+  };
+  auto promote = [&]() {  // the tensor cores cut their running sums off
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          sum[r][i][c] += acc[r][i][c];
+          acc[r][i][c] = 0.f;
+        }
+  };
+  Step even, odd;
+  int s = warp;
+  if (s < steps) load(even, s);
+  for (int n = 1; s < steps; s += 2 * WARPS, ++n) {
+    if (s + WARPS < steps) load(odd, s + WARPS);
+    multiply(even);
+    if (s + 2 * WARPS < steps) load(even, s + 2 * WARPS);
+    if (s + WARPS < steps) multiply(odd);
+    if (n % (kPromoteK / 128) == 0) promote();
+  }
+  if (steps * 64 < a.K && warp == steps % WARPS) {  // the rest of the rows, less than a step
+    Step end;
+    const int left = a.K - steps * 64 - 8 * t;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) end.w[i][h] = load_end(w[i] + steps * 64 + 32 * h, left - 32 * h);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) end.x[i][h] = load_end(x[i] + steps * 64 + 32 * h, left - 32 * h);
+    }
+    multiply(end);
+  }
+  promote();
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) part[warp][8 * i + 2 * t + (c & 1)][16 * r + g + 8 * (c >> 1)] = sum[r][i][c];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * RT * 8 * MT; i += WARPS * 32) {
+    const int row = i % (16 * RT), m = i / (16 * RT), n = n0 + row;
+    if (m >= a.M || n >= a.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) v += part[k][m][row];
+    v = activate_one(v + load_bias(a.bias, a.bias_type, n), a.act);
+    if (a.res != nullptr) v += to_float<OT>(static_cast<const OT*>(a.res)[(int64_t)m * a.ldr + n]);
+    static_cast<OT*>(a.y)[(int64_t)m * a.ldy + n] = from_float<OT>(v);
+  }
+}
+
+// Which of them a product of M tokens takes, none (false) for the tensor-core kernel. All blocks should be resident at once, 16
+// warps per SM; 32 weight rows a block halve the fetches of x, but only for one tile of tokens have they the registers.
+// Cold weights, the others of {16, 32 rows} x {4, 8, 16 warps} and the tensor-core kernel in turn: 8 x 2048 -> 2048 16x16 3.7 us, 16x8
+// 4.7, tensor cores 6.5; 8 x 3584 -> 4608 32x16 7.4, 16x8 7.6, 10.3; 8 x 2048 -> 8192 32x8 7.4, 16x4 7.5, 10.2; 8 x 1024 -> 30000 32x8
+// 12.3, 16x4 12.8, 14.0; 8 x 4096 -> 128000 32x8 170, tensor cores 166. 16 x 3584 -> 4608 16x8 8.1, 32x16 9.7, 10.4; 16 x 2048 -> 6000
+// 16x4 7.3, 16x8 8.7, 9.5; 16 x 7168 -> 18432 16x4 44.6, tensor cores 43.3. 32 tokens (four tiles): 2048 -> 512 6.0 against 5.3.
+struct FewShape {
+  int rows, warps;
+};
+bool few_shape(int M, int N, int sms, FewShape& f) {
+  const int narrow = (N + 15) / 16, wide = (N + 31) / 32;
+  if (M > 16) return false;
+  f = {16, 16};
+  if (narrow <= sms) return true;
+  if (M <= 8) {
+    f = {32, wide <= sms ? 16 : 8};
+    return wide <= 8 * sms;
+  }
+  f = {16, narrow <= 2 * sms ? 8 : 4};
+  return narrow <= 4 * sms;
+}
+
+template <class T, class OT>
+cudaError_t launch_few_for(const LinearCall& a, FewShape f, cudaStream_t s) {
+  const unsigned blocks = (unsigned)((a.N + f.rows - 1) / f.rows), threads = (unsigned)f.warps * 32;
+  if (a.M <= 8) {
+    if (f.rows == 16) return launch_behind(linear_few_kernel<T, OT, 1, 1, 16>, blocks, threads, 0, s, a);
+    if (f.warps == 16) return launch_behind(linear_few_kernel<T, OT, 2, 1, 16>, blocks, threads, 0, s, a);
+    return launch_behind(linear_few_kernel<T, OT, 2, 1, 8>, blocks, threads, 0, s, a);
+  }
+  if (f.warps == 16) return launch_behind(linear_few_kernel<T, OT, 1, 2, 16>, blocks, threads, 0, s, a);
+  if (f.warps == 8) return launch_behind(linear_few_kernel<T, OT, 1, 2, 8>, blocks, threads, 0, s, a);
+  return launch_behind(linear_few_kernel<T, OT, 1, 2, 4>, blocks, threads, 0, s, a);
+}
+template <class T>
+cudaError_t launch_few(const LinearCall& a, FewShape f, cudaStream_t s) {
+  return a.out_type == PM_F32 ? launch_few_for<T, float>(a, f, s) : launch_few_for<T, T>(a, f, s);
+}
+
 // ---- launch plan ------------------------------------------------------------------------------------------
 struct LinearShape {
   int cg = 1, split = 1, tok_tiles = 1, width = 16, atoms = 1;
@@ -729,6 +894,11 @@ int launch_linear(const LinearCall& a, cudaStream_t s) {
   int dev = 0, cap[kMaxCluster + 1];
   PM_CUDA(cudaGetDevice(&dev));
   PM_CUDA(cluster_capacity(dev, cap));
+  FewShape few;
+  if (few_shape(a.M, a.N, cap[1], few)) {
+    PM_CUDA(a.type == PM_BF16 ? launch_few<__nv_bfloat16>(a, few, s) : launch_few<__half>(a, few, s));
+    return PM_OK;
+  }
   // The shape follows from the sizes alone; a thread remembers the last few.
   const bool promote = a.out_type == PM_F32;
   const PlanKey key{a.M, a.N, a.K, promote, dev};
