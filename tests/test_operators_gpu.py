@@ -213,6 +213,16 @@ def test_linear_sizes(lib, M, K, N, dtype):
     check_linear(randn(g, M, K).to(dtype), (randn(g, N, K) * 0.05).to(dtype))
 
 
+@pytest.mark.parametrize("M", [1, 8, 9, 16])
+@pytest.mark.parametrize("K,N", [(8, 16), (200, 15), (64, 2368), (1160, 2369), (72, 4737), (520, 9000), (64, 9473), (128, 37889)])
+@pytest.mark.parametrize("out_dtype", [F16, F32])
+def test_linear_few_tokens(lib, M, K, N, out_dtype):
+    """Either side of where the kernels for few tokens take each other's place, with rows that end inside a step."""
+    g = gen(M + K + N)
+    x, w = randn(g, M, K).to(F16), (randn(g, N, K) * 0.05).to(F16)
+    check_linear(x, w, randn(g, N).to(F16), "gelu_tanh", randn(g, M, N).to(out_dtype), out_dtype)
+
+
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("M,K,N", [(1, 512, 640), (5, 4096, 200), (40, 256, 300), (600, 192, 2304)])
 @pytest.mark.parametrize("out_dtype", [BF16, F32])
