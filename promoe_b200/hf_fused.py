@@ -15,6 +15,9 @@ worth to the model.
 """
 from __future__ import annotations
 
+import types
+import weakref
+
 import torch
 
 from . import ops
@@ -109,52 +112,85 @@ def _replace_forward(block, cache: ExpertCache, layer: int):
     block.forward = fused_forward
 
 
+# The products of replaced modules, with what they were made from. Beside the modules, so that a copied model makes its own.
+_PRODUCTS: "weakref.WeakKeyDictionary[torch.nn.Module, tuple]" = weakref.WeakKeyDictionary()
+
+
+def _usable(m) -> bool:
+    return (isinstance(m, torch.nn.Linear) and m.weight.is_cuda and m.weight.dtype in (torch.bfloat16, torch.float16)
+            and m.weight.dim() == 2 and (m.bias is None or m.bias.dtype == m.weight.dtype))
+
+
+def _product(owner: torch.nn.Module, m: torch.nn.Linear, x: torch.Tensor, activation: str | None = None):
+    """The library's product with m's weights as they are now, or None where m's own forward has to do: other types or
+    devices, or a gradient to record."""
+    w, b = m.weight, m.bias
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+        return None
+    if x.dtype != w.dtype or x.device != w.device:
+        return None
+    key = (w.data_ptr(), w.dtype, w.shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
+    have = _PRODUCTS.get(owner)
+    if have is None or have[0] != key:
+        if not _usable(m):
+            return None
+        have = _PRODUCTS[owner] = (key, ops.Linear(w.detach(), None if b is None else b.detach(), activation))
+    return have[1]
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x as a matrix with dense rows, none over another."""
+    x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+
+
+def _linear_forward(self, x):
+    lin = _product(self, self, x)
+    if lin is None:
+        return type(self).forward(self, x)
+    return lin(_rows(x)).view(*x.shape[:-1], lin.N)
+
+
+def _gated_forward(self, x):
+    learns = torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
+    gate = None if self.training or learns else _product(self, self.gate_proj, x, "silu")
+    if gate is None:
+        return type(self).forward(self, x)
+    rows = _rows(x)
+    return self.down_proj(gate(rows).mul_(self.up_proj(rows))).view(*x.shape[:-1], self.down_proj.out_features)
+
+
 def install_linears(model: torch.nn.Module) -> int:
     """Replaces the forward of every torch.nn.Linear with bf16 or fp16 weights on a GPU by promoe_b200.ops.Linear (bias in the
-    product's epilogue), and of gated MLPs (`gate_proj`, `up_proj`, `down_proj` around a SiLU: dense layers between MoE blocks)
-    by three such products, SiLU in the first one's epilogue. For inference: calls with tensors that require a gradient
-    keep the module's own forward. Call it once the model is on its device; weights are used in place. MoE blocks that
-    inject_hf_fused_model replaced do not call theirs any more. Returns the number of replaced modules."""
-    def usable(m):
-        return (isinstance(m, torch.nn.Linear) and m.weight.is_cuda and m.weight.dtype in (torch.bfloat16, torch.float16)
-                and m.weight.dim() == 2 and (m.bias is None or m.bias.dtype == m.weight.dtype) and "_promoe_linear" not in vars(m))
-
-    def rows(x):
-        return x.reshape(-1, x.shape[-1])
-
-    def takes(x, lin):
-        return x.is_cuda and x.dtype == lin.weight.dtype and not (torch.is_grad_enabled() and x.requires_grad)
-
-    def replace_linear(m):
-        lin, own = ops.Linear(m.weight, m.bias), m.forward
-
-        def forward(x):
-            if not takes(x, lin):
-                return own(x)
-            return lin(rows(x)).view(*x.shape[:-1], lin.N)
-        m._promoe_linear, m.forward = lin, forward
-
-    def replace_mlp(m):
-        gate, up, down, own = ops.Linear(m.gate_proj.weight, m.gate_proj.bias, "silu"), m.up_proj, m.down_proj, m.forward
-
-        def forward(x):
-            if not takes(x, gate):
-                return own(x)
-            return down(gate(rows(x)).mul_(up(rows(x)))).view(*x.shape[:-1], -1)
-        m._promoe_linear, m.forward = gate, forward
-
+    product's epilogue), and of gated MLPs (`gate_proj`, `up_proj`, `down_proj` around a SiLU and nothing else: dense layers
+    between MoE blocks) by three such products, SiLU in the first one's epilogue. For inference, under torch.no_grad() or with
+    parameters that require no gradient: calls that a gradient is to be recorded for keep the module's own forward, a gated
+    MLP's also in training mode. Call it once the model is on its device. Weights are used in place; they may be changed or
+    exchanged afterwards, and a copied model works on its own. Modules of other classes than torch.nn.Linear itself, or with a forward of
+    their own (hooks of other libraries), stay as they are. MoE blocks that inject_hf_fused_model replaced do
+    not call theirs any more. Returns the number of replaced modules."""
     replaced = 0
     for m in list(model.modules()):
-        if usable(m):
-            replace_linear(m)
+        if type(m) is torch.nn.Linear and _usable(m) and "forward" not in vars(m):
+            m.forward = types.MethodType(_linear_forward, m)
             replaced += 1
+    mine = lambda m: getattr(vars(m).get("forward"), "__func__", None) is _linear_forward  # noqa: E731
     for m in list(model.modules()):
-        if "_promoe_linear" in vars(m):
+        parts = dict(m.named_children())
+        act = type(parts.pop("act_fn", None)).__name__.lower()
+        if (sorted(parts) != ["down_proj", "gate_proj", "up_proj"] or not all(mine(p) for p in parts.values())
+                or act not in ("silu", "siluactivation") or "forward" in vars(m)):
             continue
-        parts = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
-        act = type(getattr(m, "act_fn", None)).__name__.lower()
-        if all(isinstance(p, torch.nn.Linear) and "_promoe_linear" in vars(p) for p in parts) and act in ("silu", "siluactivation"):
-            replace_mlp(m)
+        with torch.no_grad():  # whether its forward is what the names say
+            w = m.gate_proj.weight
+            x = torch.randn(2, w.shape[1], generator=torch.Generator(w.device).manual_seed(0), device=w.device).to(w.dtype)
+            modes = [(c, c.training) for c in m.modules()]
+            m.eval()
+            own, fused = type(m).forward(m, x), _gated_forward(m, x)
+            for c, mode in modes:
+                c.training = mode
+        if own.shape == fused.shape and float((own - fused).float().norm()) <= 0.02 * float(own.float().norm()):
+            m.forward = types.MethodType(_gated_forward, m)
             replaced += 1
     return replaced
 

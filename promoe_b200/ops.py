@@ -108,6 +108,7 @@ class Linear:
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
                  out_dtype: torch.dtype | None = None):
+        self._learns = weight.requires_grad or (bias is not None and bias.requires_grad)
         weight = weight.detach()
         index, N, K, pitch = _matrix(weight, "weight", dtypes=(torch.bfloat16, torch.float16))
         if activation not in _ACTS:
@@ -124,15 +125,17 @@ class Linear:
         self.weight, self.bias, self.out_dtype, self.device_index, self.N, self.K = weight, bias, out_dtype, index, N, K
         self._x_dtypes, self._y_dtypes = (weight.dtype,), (out_dtype,)
         # what stays the same from call to call; a call works on a copy, so that two threads may call at once
-        self._call = bytes(_lib.pm_linear(w=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(), ld_w=pitch, N=N, K=K,
+        self._call = bytes(_lib.pm_linear(bias=None if bias is None else bias.data_ptr(), ld_w=pitch, N=N, K=K,
                                           dtype=_DTYPES[weight.dtype], out_dtype=_DTYPES[out_dtype],
                                           bias_dtype=0 if bias is None else _DTYPES[bias.dtype], act=_ACTS[activation]))
         self._fn = _lib.load().pm_k_linear
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [M, K] of the weight's type, residual [M, N] of out_dtype (dense rows, any pitch) -> y [M, N]. out may be the
-        residual itself; it must not overlap x, the weight or the bias."""
+        residual itself; otherwise it must not overlap it, nor ever x, the weight or the bias."""
         index = self.device_index
+        if self._learns and torch.is_grad_enabled():
+            raise ValueError("the weight or the bias requires a gradient: these operators have no backward pass")
         on, M, _, ld_x = _matrix(x, "x", self.K, self._x_dtypes)
         if out is None:
             out = torch.empty((M, self.N), dtype=self.out_dtype, device=x.device)
@@ -140,7 +143,7 @@ class Linear:
         if rows != M:
             raise ValueError(f"out must have {M} rows, not {rows}")
         a = _lib.pm_linear.from_buffer_copy(self._call)
-        a.x, a.y, a.ld_x, a.ld_y, a.M = x.data_ptr(), out.data_ptr(), ld_x, ld_y, M
+        a.x, a.w, a.y, a.ld_x, a.ld_y, a.M = x.data_ptr(), self.weight.data_ptr(), out.data_ptr(), ld_x, ld_y, M
         if residual is not None:
             on_r, rows, _, a.ld_residual = _matrix(residual, "residual", self.N, self._y_dtypes)
             if rows != M:
@@ -165,6 +168,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, 
     logits [T, V] float32 / bf16 / fp16, targets [T] int64; a negative target names no token (logp 0). Masked logits (-inf)
     have probability 0; pm_k_token_logprobs states what rows without a distribution give. out: the four results to fill."""
     index, T, V, pitch = _matrix(logits, "logits")
+    if top_n < 0:
+        raise ValueError("top_n must not be negative")
     if targets.shape != (T,) or targets.dtype != torch.int64 or targets.get_device() != index or not targets.is_contiguous():
         raise ValueError(f"targets must be a contiguous int64 tensor of shape [{T}] on cuda:{index}")
     logp, entropy, ids, best = out if out is not None else (None, None, None, None)

@@ -1,6 +1,9 @@
 """The operators around the experts (promoe_b200.ops: Router, Linear, token_logprobs) against plain 64-bit forms, at the sizes,
 masks, strides and streams where they can go wrong. half_step(t) is the largest relative error of one rounding to t."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -461,6 +464,36 @@ def test_captured_and_replayed_beside_an_eager_run(lib):
     torch.cuda.synchronize()
     for a, b in zip(got[:3], want[:3]):
         assert torch.equal(torch.flip(a, [0]), b)
+
+
+FIRST_CALLS = """
+import torch
+from promoe_b200 import ops
+torch.manual_seed(0)
+rand = lambda *s: torch.randn(s, device="cuda")
+l, b = rand(40, 64), rand(64)
+w, wo = rand(300, 128).bfloat16(), rand(300, 77).bfloat16()
+x, few, xo, v, t = rand(40, 128).bfloat16(), rand(3, 128).bfloat16(), rand(40, 77).bfloat16(), rand(2, 50000), torch.tensor([3, 4], device="cuda")
+many = rand(600, 128).bfloat16()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    r = ops.Router(64, 6, "sigmoid", b, 8, 3, "top2")(l)
+    y = [ops.Linear(w, out_dtype=torch.float32)(x), ops.Linear(w)(few), ops.Linear(wo)(xo), ops.Linear(w)(many)]
+    p = ops.token_logprobs(v, t, 5)
+for _ in range(2):
+    g.replay()
+torch.cuda.synchronize()
+assert torch.equal(r[0], ops.Router(64, 6, "sigmoid", b, 8, 3, "top2")(l)[0])
+for have, rows, weight in zip(y, (x, few, xo, many), (w, w, wo, w)):
+    want = rows.double() @ weight.double().T
+    assert float((have.double() - want).norm()) <= 2.0 ** -8 * float(want.norm())
+assert float((p[0].double() - torch.log_softmax(v.double(), -1)[torch.arange(2), t.cpu()]).abs().max()) < 1e-5
+"""
+
+
+def test_first_call_of_a_process_inside_a_capture(lib):
+    root = Path(__file__).resolve().parent.parent
+    subprocess.run([sys.executable, "-c", FIRST_CALLS], check=True, timeout=300, cwd=root)
 
 
 def test_two_threads_on_two_streams(lib):

@@ -283,3 +283,63 @@ def test_install_linears_fuses_a_gated_mlp_and_steps_aside_for_gradients(lib):
     x.requires_grad_()
     m(x).sum().backward()
     assert x.grad is not None and float(x.grad.float().norm()) > 0
+
+
+def test_installed_linears_follow_their_modules(lib):
+    """Weights that are changed, exchanged or copied, inputs with strides, no rows at all, and parameters that learn."""
+    from promoe_b200.hf_fused import install_linears
+    torch.manual_seed(1)
+    m = torch.nn.Sequential(torch.nn.Linear(64, 96), torch.nn.ReLU(), torch.nn.Linear(96, 40, bias=False)).to(torch.bfloat16).cuda()
+    assert install_linears(m) == 2
+    x = torch.randn(5, 64, device="cuda").to(torch.bfloat16)
+
+    def same(model, y, rows=None):
+        first, last = model[0], model[2]
+        h = torch.nn.functional.linear((x if rows is None else rows).double(), first.weight.double(), first.bias.double()).relu()
+        assert rel_err(y, torch.nn.functional.linear(h, last.weight.double())) < 1e-2  # two roundings to bf16
+    with torch.no_grad():
+        same(m, m(x))
+        other = copy.deepcopy(m)
+        for p in other.parameters():
+            p.mul_(-2.0)
+        same(other, other(x))                                     # the copy's weights
+        same(m, m(x))
+        m[0].weight.mul_(3.0)                                     # changed in place
+        same(m, m(x))
+        m[2].weight = torch.nn.Parameter(torch.randn(40, 96, device="cuda").to(torch.bfloat16))  # exchanged
+        m[0].bias.data = torch.randn(96, device="cuda").to(torch.bfloat16)
+        same(m, m(x))
+        same(m, m(x[:1].expand(7, 64)), x[:1].expand(7, 64))      # rows over one another
+        wide = torch.randn(64, 9, device="cuda").to(torch.bfloat16).t()
+        same(m, m(wide), wide)                                    # rows that are not dense
+        assert m(x[:0]).shape == (0, 40) and m(x[0]).shape == (40,)
+    y = m(x)                                                      # the parameters require a gradient, the input does not
+    y.sum().backward()
+    assert float(m[0].weight.grad.float().norm()) > 0
+    m.requires_grad_(False)
+    same(m, m(x))
+    with pytest.raises(ValueError):
+        ops.Linear(torch.nn.Parameter(m[0].weight.data))(x)
+
+
+def test_mlps_of_another_kind_stay_as_they_are(lib):
+    from promoe_b200.hf_fused import install_linears
+
+    class Mlp(torch.nn.Module):
+        def __init__(self, scale):
+            super().__init__()
+            self.gate_proj, self.up_proj = torch.nn.Linear(64, 72, bias=False), torch.nn.Linear(64, 72, bias=False)
+            self.down_proj, self.act_fn, self.scale = torch.nn.Linear(72, 64), torch.nn.SiLU(), scale
+
+        def forward(self, x):
+            return self.down_proj(self.act_fn(self.gate_proj(x) * self.scale) * self.up_proj(x))
+
+    state = torch.cuda.get_rng_state()
+    plain, scaled = (Mlp(s).to(torch.bfloat16).cuda() for s in (1.0, 2.0))
+    assert install_linears(plain) == 4 and install_linears(scaled) == 3
+    assert torch.equal(state, torch.cuda.get_rng_state()) and plain.training and scaled.act_fn.training
+    x = torch.randn(3, 64, device="cuda").to(torch.bfloat16)
+    with torch.no_grad():
+        assert plain.eval()(x[:0]).shape == (0, 64)
+        for m in (plain, scaled):
+            assert rel_err(m(x), copy.deepcopy(m).double()(x.double())) < 1e-2
