@@ -27,21 +27,28 @@ combine_kernel(const float* __restrict__ yexp, const int32_t* __restrict__ pos,
     p_s[threadIdx.x] = pos[(size_t)t * k + threadIdx.x];
     w_s[threadIdx.x] = topk_w[(size_t)t * k + threadIdx.x];
   }
-  __syncthreads();
+  // Rows without some of their experts (a router rule's -1) take a loop that looks at each: the test in the common loop kept its
+  // loads from being issued together, 1 us of a pass of one token.
+  const bool holes = __syncthreads_or(threadIdx.x < k && p_s[threadIdx.x] < 0);
   const float ss = (shared_scale != nullptr) ? shared_scale[t] : 1.f;
   for (int h = threadIdx.x * 4; h < H; h += kCombineThreads * 4) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = 0; j < k; ++j) {
-      if (p_s[j] < 0) {  // no expert: a weight of 0, or NaN where the token has no routing at all
-        if (w_s[j] != 0.f) acc.x = acc.y = acc.z = acc.w = w_s[j];
-        continue;
-      }
+    auto add = [&](int j) {
       float4 v = *reinterpret_cast<const float4*>(yexp + (size_t)p_s[j] * H + h);
       float w = w_s[j];
       acc.x = fmaf(w, v.x, acc.x);
       acc.y = fmaf(w, v.y, acc.y);
       acc.z = fmaf(w, v.z, acc.z);
       acc.w = fmaf(w, v.w, acc.w);
+    };
+    if (!holes) {
+      for (int j = 0; j < k; ++j) add(j);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < k; ++j) {
+        if (p_s[j] >= 0) add(j);
+        else if (w_s[j] != 0.f) acc.x = acc.y = acc.z = acc.w = w_s[j];  // NaN, where the token has no routing at all
+      }
     }
     for (int s = 0; s < n_shared; ++s) {
       // Shared-expert rows follow the R routed rows: row R + s*T + t.
