@@ -151,9 +151,9 @@ class CudaBackend:
         has_gate = p["shared_gate_w"] is not None
         router, logits = p.get("router"), None
         if router is not None:
-            if "logits" not in b:
-                b["logits"] = torch.empty((T, E), dtype=torch.float32, device=self.device)
-            logits = b["logits"]
+            logits = b.get(("logits", E))
+            if logits is None:
+                logits = b["logits", E] = torch.empty((T, E), dtype=torch.float32, device=self.device)
         self._lib.call("pm_k_gate_topk", x.data_ptr(), p["gate_w"].data_ptr(), ptr(p["gate_bias"]),
                        ptr(p["shared_gate_w"]), T, H, E, k, int(p["norm_topk"]), float(p["routed_scale"]), None,
                        b["ids"].data_ptr(), b["w"].data_ptr(), None, b["ss"].data_ptr() if has_gate else None, ptr(logits),

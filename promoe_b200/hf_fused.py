@@ -201,13 +201,16 @@ def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask
     entropy of the model's prediction there and its top_n favourites. input_ids [B, S] -> {"logp": [B, S - 1], "entropy": [B, S - 1],
     "top_ids", "top_logp": [B, S - 1, top_n]}. Tokens outside attention_mask are not scored (logp 0). The vocabulary
     projection (bf16 or fp16, on the GPU) runs with float32 logits, for as many positions at a time as 64 Mi logits hold,
-    so a long text does not need all its logits at once."""
+    so a long text does not need all its logits at once. Models that cap or scale their logits afterwards are refused."""
+    for name in ("final_logit_softcapping", "logit_scale", "logits_scaling", "lm_head_multiplier"):
+        if getattr(model.config, name, None) not in (None, 1.0):
+            raise ValueError(f"this model changes its logits behind the vocabulary projection ({name})")
     head = model.get_output_embeddings()
     trunk = getattr(model, model.base_model_prefix)
     hidden = trunk(input_ids=input_ids, attention_mask=attention_mask).last_hidden_state
     lin = ops.Linear(head.weight, getattr(head, "bias", None), out_dtype=torch.float32)
     B, S = input_ids.shape
-    x = hidden[:, :-1].reshape(B * (S - 1), -1).to(head.weight.dtype)
+    x = hidden[:, :-1].reshape(B * (S - 1), hidden.shape[-1]).to(head.weight.dtype)
     targets = input_ids[:, 1:].to(torch.int64)
     if attention_mask is not None:
         targets = targets.masked_fill(attention_mask[:, 1:] == 0, -100)

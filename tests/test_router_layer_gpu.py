@@ -258,6 +258,11 @@ def test_install_linears_and_score_tokens_of_an_injected_model(lib):
     assert mine["top_ids"].shape == (2, 10, 3) and bool((mine["top_logp"][..., 0] >= mine["top_logp"][..., 1]).all())
     best = torch.gather(lp, 2, mine["top_ids"].long())
     assert float((best - mine["top_logp"].double()).abs().max()) < 4 * 2.0 ** -8 * 2
+    none = score_tokens(model, ids[:, :1], top_n=2)                # a text of one token has nothing to predict
+    assert none["logp"].shape == (2, 0) and none["top_ids"].shape == (2, 0, 2)
+    model.config.final_logit_softcapping = 30.0
+    with pytest.raises(ValueError):
+        score_tokens(model, ids)
     cache.close()
 
 
