@@ -517,7 +517,8 @@ linear_plain_kernel(const __grid_constant__ LinearCall a) {
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  float acc[kM][kN][4] = {};
+  constexpr bool kPromote = sizeof(OT) == 4;  // as in the tensor-memory kernel
+  float acc[kM][kN][4] = {}, sum[kPromote ? kM : 1][kPromote ? kN : 1][4] = {};
   const uint32_t base = smem_u32(tile);
   // ldmatrix: lanes 0-15 give the rows of the first 8 k, lanes 16-31 of the next
   const uint32_t x_at = base + 2u * (uint32_t)((wm + (lane & 15)) * P::kPitch + (lane >> 4) * 8);
@@ -554,6 +555,19 @@ linear_plain_kernel(const __grid_constant__ LinearCall a) {
         for (int i = 0; i < kM; ++i) mma_16x8x16<T>(acc[i][j], xf[i], w0, w1);
       }
     }
+    if constexpr (kPromote) {
+      if ((step + 1) % (kPromoteK / P::kK) == 0 || step + 1 == steps) {
+#pragma unroll
+        for (int i = 0; i < kM; ++i)
+#pragma unroll
+          for (int j = 0; j < kN; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              sum[i][j][c] += acc[i][j][c];
+              acc[i][j][c] = 0.f;
+            }
+      }
+    }
   }
 #pragma unroll
   for (int j = 0; j < kN; ++j)
@@ -568,7 +582,7 @@ linear_plain_kernel(const __grid_constant__ LinearCall a) {
         for (int h = 0; h < 2; ++h) {
           const int m = m0 + wm + 16 * i + (lane >> 2) + 8 * h;
           if (m >= a.M) continue;
-          float v = activate_one(acc[i][j][2 * h + e] + b, a.act);
+          float v = activate_one((kPromote ? sum[kPromote ? i : 0][kPromote ? j : 0] : acc[i][j])[2 * h + e] + b, a.act);
           if (a.res != nullptr) v += to_float<OT>(static_cast<const OT*>(a.res)[(int64_t)m * a.ldr + n]);
           static_cast<OT*>(a.y)[(int64_t)m * a.ldy + n] = from_float<OT>(v);
         }

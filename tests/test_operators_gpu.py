@@ -286,6 +286,19 @@ def test_linear_infinities_and_nan_stay_in_their_rows_and_columns(lib):
     assert torch.equal(torch.isnan(r), torch.isnan(ref))
 
 
+@pytest.mark.parametrize("M", [1, 12, 40, 300])
+@pytest.mark.parametrize("K", [4160, 4099])
+def test_linear_float32_results_keep_their_precision(lib, M, K):
+    """Tensor cores cut running sums off (by up to 2^-23 of them, half of that on average): 32 additions of 16 k of
+    terms with random signs, whose partial sums grow with the root of their number, shrink a sum by 2^-24 * 32 * 2/3 = 1.3e-6 of what it
+    is like. Nine such sums are added and the result is rounded: 2^-24 * (sqrt(9) + 1) at most. 4099 k in one sum: 1e-5."""
+    g = gen(M + K)
+    x, w = randn(g, M, K).to(BF16), randn(g, 700, K).to(BF16)
+    want = x.double() @ w.double().T
+    y = ops.Linear(w, out_dtype=F32)(x)
+    assert float((y.double() - want).norm()) <= 1.6e-6 * float(want.norm())
+
+
 def test_linear_is_reproducible_and_independent_of_other_rows(lib):
     g = gen(10)
     for M, K, N in ((1, 4096, 256), (24, 8192, 512), (500, 1024, 1000)):
