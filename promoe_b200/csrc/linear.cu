@@ -1,17 +1,24 @@
 // y = act(x w^T + bias) + residual: x [M, K] tokens, w [N, K] weights, bf16 or fp16, float32 sums, one rounding at the end.
 //
-// Tensor-core kernel (linear_tc_kernel): weight rows are the M operand of tcgen05.mma, token rows the N operand, because N
-// can be any multiple of 16: one token costs a 16-column tile, a prompt of 777 four tiles of 208. TMA brings both in steps
-// of 64 k into a ring, one thread issues the MMAs, eight warps drain the accumulators (double-buffered in
-// tensor memory) through bias, activation and residual. A lane holds one weight row, so the bias is one load per tile and
-// the lanes of a warp store 32 neighbouring outputs of a token, whatever the alignment of y.
-// Three shapes of it, chosen by launch_linear:
-//   pairs   CTA pairs (cta_group::2) on 256 weight rows x up to 256 tokens, persistent: many tokens
-//   single  one CTA on 128 weight rows, persistent: few tokens against many weight rows
+// More than 16 tokens: linear_tc_kernel. Weight rows are the M operand of tcgen05.mma, token rows the N operand, because N can
+// be any multiple of 16: 33 tokens cost 48 columns, a prompt of 777 seven tiles of 112. TMA brings both in steps of 64 or 128 k
+// into a ring, one thread issues the MMAs, eight warps drain the accumulators (double-buffered in tensor memory)
+// through bias, activation and residual. A lane holds one weight row, so the bias is one load per tile and the lanes of a
+// warp store 32 neighbouring outputs of a token, whatever the alignment of y. Three shapes of it, chosen by an estimate of
+// their time (shape_cost):
+//   pairs   CTA pairs (cta_group::2) on 256 weight rows x up to 256 tokens, persistent
+//   single  one CTA on 128 weight rows, persistent
 //   split   a cluster of up to 8 CTAs shares the k steps of one tile and adds its partial sums through distributed shared
 //           memory, in the order of the ranks: too few tiles for the GPU
+// What bounds it. Large products the tensor cores under the power limit: 8192 x 4096 -> 14336 takes 645 us in a burst = 1.49 PFLOP/s,
+// 0.92 of measured, and 742 us sustained. Few tokens against many weights HBM: 33 x 2048 -> 100003 68 us = 6.0 TB/s, 0.92 of measured. Between them an
+// SM's intake, 124 bytes per ns at most: 777 x 5632 -> 2048 (tiles of 256 x 112, 22 KB a step of 64 k and SM) 25 us where the
+// MMAs alone would take 12. And what comes before and after the k steps: setup and first load 1.5 us, a tile's epilogue
+// 0.3 us for each 16 columns and half (a warp's store or remote store of 16 columns takes 600 cycles), joining partial sums 0.7 us for the
+// cluster barrier and as much for the sums. 64 x 4096 -> 4096 11 us, 512 x 3584 -> 4608 18 us.
 //
-// Rows that do not start on 16-byte boundaries cannot be fetched by TMA: linear_plain_kernel (mma.sync, plain loads).
+// At most 16 tokens: linear_few_kernel (mma.sync), which streams the weights straight into registers. Rows that do not start on
+// 16-byte boundaries cannot be fetched by TMA: linear_plain_kernel (mma.sync, plain loads) for more tokens than that.
 //
 // Every mbarrier wait is bounded. On a give-up the outputs of the tile become NaN and *err (optional) a code.
 #include <algorithm>
@@ -413,8 +420,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 // the aligned 16-byte words that hold a step's values come into a ring of kRing steps (cp.async; each word holds at least one
 // of the row's bytes, so it is mapped memory), and a thread shifts its eight values out of two of them into the tile: 15
 // instructions instead of eight loads. What bounds it: the steps' two barriers and, with few tiles, the SMs that have none.
-// 86 rows of 2611 -> 15580 take 105 us (180 with two-byte loads straight into the tile), 4000 of 2001 -> 2001 295 us = 109
-// TFLOP/s, 125 of 1506 -> 111 20 us (36), one of 3001 -> 4001 28 us. Rows on 16-byte boundaries are five to ten times faster.
+// 86 rows of 2611 -> 15580 take 90 us (180 with two-byte loads straight into the tile), 4000 of 2001 -> 2001 295 us = 109
+// TFLOP/s, 125 of 1506 -> 111 20 us (36). Rows on 16-byte boundaries are three to eight times faster. Up to 16 tokens take
+// linear_few_kernel instead.
 constexpr int kPlainThreads = 256;
 
 template <class T>
@@ -600,24 +608,14 @@ cudaError_t launch_plain_tiles(const LinearCall& a, cudaStream_t s) {
   return launch_behind(kern, (unsigned)tiles, kPlainThreads, PlainTile<BM, BN>::bytes(), s, a);
 }
 
-template <class T, class OT>
-cudaError_t launch_plain_for(const LinearCall& a, cudaStream_t s) {
-  // Few tokens need few rows of the tile; narrow weight tiles where wide ones would leave SMs without any.
-  if (a.M <= 16) return launch_plain_tiles<T, OT, 16, 64>(a, s);
-  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) < 148) return launch_plain_tiles<T, OT, 32, 64>(a, s);
-  return launch_plain_tiles<T, OT, 64, 128>(a, s);
-}
-
-template <class T>
-cudaError_t launch_plain(const LinearCall& a, cudaStream_t s) {
-  return a.out_type == PM_F32 ? launch_plain_for<T, float>(a, s) : launch_plain_for<T, T>(a, s);
-}
-
 // ---- few tokens -----------------------------------------------------------------------------------------
 // 16 RT weight rows per CTA, its warps on one step of 64 k after the other in turn (mma.sync; weight rows are its M operand, MT
 // tiles of eight tokens its N operand). A lane loads 16 bytes of a row, eight neighbouring k, and gives them to two MMAs as
 // the k it has there: both operands come in the same order, so that neither goes through shared memory. Weights pass the L1
 // by, two steps of a warp are under way at a time. The warps' sums are added in order through shared memory.
+// Rows off 16-byte boundaries (ALIGNED = false): a lane's eight values are shifted out of two aligned words; their registers leave
+// room for one step per warp, more warps make up for it. 1 x 3001 -> 4001 8.6 us, 7 x 1628 -> 80637 60 us = 4.4 TB/s, where
+// tiles through shared memory took 28 and 90.
 // Bound by the weights' way from HBM, once a launch has started: 8 x 3584 -> 4608 (33 MB) takes 7.4 us, of which 5.0 are the
 // bytes at the measured copy rate. The tensor-core kernel needs 3 us more for its setup, the joining of partial sums and the
 // longer way of the operands.
@@ -643,8 +641,8 @@ __device__ __forceinline__ uint4 load_end(const T* row, int left) {
   return v;
 }
 
-template <class T, class OT, int RT, int MT, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(const __grid_constant__ LinearCall a) {
+template <class T, class OT, int RT, int MT, int WARPS, bool ALIGNED = true>
+__global__ void __launch_bounds__(WARPS * 32, (ALIGNED ? 16 : 24) / WARPS) linear_few_kernel(const __grid_constant__ LinearCall a) {
   __shared__ float part[WARPS][MT * 8][16 * RT + 4];  // the lanes of a store meet different banks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16 * RT, steps = a.K / 64;
@@ -658,6 +656,26 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(cons
 
   struct Step {
     uint4 w[2 * RT][2], x[MT][2];
+  };
+  // Rows that start anywhere: the two 16-byte words that hold a lane's eight values, if they hold any of the row's `left` values
+  // from the step's start on (else they may lie in memory that is not there), and the values shifted out of them.
+  auto load_shifted = [&](Step& s, int step, int left) {
+    auto two = [&](const T* row, uint4& v) {
+      const uintptr_t at = (uintptr_t)(row + step * 64), word = at & ~(uintptr_t)15;
+      const int shift = (int)(at & 15), valid = left - 8 * t;
+      const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int in = valid - 32 * h;
+        const uint4* p = reinterpret_cast<const uint4*>(word + 64 * h);
+        const uint4 lo = in > 0 ? p[0] : none, hi = 2 * in + shift > 16 && shift > 0 ? p[1] : none;
+        (&v)[h] = eight_from(lo, hi, shift, in < 8 ? in : 8);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) two(w[i], s.w[i][0]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) two(x[i], s.x[i][0]);
   };
   auto load = [&](Step& s, int step) {
 #pragma unroll
@@ -697,27 +715,40 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(cons
           acc[r][i][c] = 0.f;
         }
   };
-  Step even, odd;
-  int s = warp;
-  if (s < steps) load(even, s);
-  for (int n = 1; s < steps; s += 2 * WARPS, ++n) {
-    if (s + WARPS < steps) load(odd, s + WARPS);
-    multiply(even);
-    if (s + 2 * WARPS < steps) load(even, s + 2 * WARPS);
-    if (s + WARPS < steps) multiply(odd);
-    if (n % (kPromoteK / 128) == 0) promote();
-  }
-  if (steps * 64 < a.K && warp == steps % WARPS) {  // the rest of the rows, less than a step
-    Step end;
-    const int left = a.K - steps * 64 - 8 * t;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 2 * RT; ++i) end.w[i][h] = load_end(w[i] + steps * 64 + 32 * h, left - 32 * h);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) end.x[i][h] = load_end(x[i] + steps * 64 + 32 * h, left - 32 * h);
+  if constexpr (!ALIGNED) {
+    Step one;  // the other blocks' warps have theirs under way meanwhile
+    for (int s = warp, n = 1; s < steps; s += WARPS, ++n) {
+      load_shifted(one, s, 64);
+      multiply(one);
+      if (n % (kPromoteK / 64) == 0) promote();
     }
-    multiply(end);
+    if (steps * 64 < a.K && warp == steps % WARPS) {
+      load_shifted(one, steps, a.K - steps * 64);
+      multiply(one);
+    }
+  } else {
+    Step even, odd;
+    int s = warp;
+    if (s < steps) load(even, s);
+    for (int n = 1; s < steps; s += 2 * WARPS, ++n) {
+      if (s + WARPS < steps) load(odd, s + WARPS);
+      multiply(even);
+      if (s + 2 * WARPS < steps) load(even, s + 2 * WARPS);
+      if (s + WARPS < steps) multiply(odd);
+      if (n % (kPromoteK / 128) == 0) promote();
+    }
+    if (steps * 64 < a.K && warp == steps % WARPS) {  // the rest of the rows, less than a step
+      Step end;
+      const int left = a.K - steps * 64 - 8 * t;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i) end.w[i][h] = load_end(w[i] + steps * 64 + 32 * h, left - 32 * h);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) end.x[i][h] = load_end(x[i] + steps * 64 + 32 * h, left - 32 * h);
+      }
+      multiply(end);
+    }
   }
   promote();
 #pragma unroll
@@ -773,9 +804,33 @@ cudaError_t launch_few_for(const LinearCall& a, FewShape f, cudaStream_t s) {
   if (f.warps == 8) return launch_behind(linear_few_kernel<T, OT, 1, 2, 8>, blocks, threads, 0, s, a);
   return launch_behind(linear_few_kernel<T, OT, 1, 2, 4>, blocks, threads, 0, s, a);
 }
+template <class T, class OT, int MT>
+cudaError_t launch_few_shifted_for(const LinearCall& a, int sms, cudaStream_t s) {
+  const int blocks = (a.N + 15) / 16;
+  if (blocks <= sms) return launch_behind(linear_few_kernel<T, OT, 1, MT, 16, false>, blocks, 512, 0, s, a);
+  if (blocks <= 3 * sms) return launch_behind(linear_few_kernel<T, OT, 1, MT, 8, false>, blocks, 256, 0, s, a);
+  return launch_behind(linear_few_kernel<T, OT, 1, MT, 4, false>, blocks, 128, 0, s, a);
+}
+template <class T, class OT>
+cudaError_t launch_few_shifted(const LinearCall& a, int sms, cudaStream_t s) {
+  return a.M <= 8 ? launch_few_shifted_for<T, OT, 1>(a, sms, s) : launch_few_shifted_for<T, OT, 2>(a, sms, s);
+}
 template <class T>
 cudaError_t launch_few(const LinearCall& a, FewShape f, cudaStream_t s) {
   return a.out_type == PM_F32 ? launch_few_for<T, float>(a, f, s) : launch_few_for<T, T>(a, f, s);
+}
+
+template <class T, class OT>
+cudaError_t launch_plain_for(const LinearCall& a, cudaStream_t s) {
+  // narrow weight tiles where wide ones would leave SMs without any
+  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) < 148) return launch_plain_tiles<T, OT, 32, 64>(a, s);
+  return launch_plain_tiles<T, OT, 64, 128>(a, s);
+}
+
+template <class T>
+cudaError_t launch_plain(const LinearCall& a, int sms, cudaStream_t s) {
+  if (a.M <= 16) return a.out_type == PM_F32 ? launch_few_shifted<T, float>(a, sms, s) : launch_few_shifted<T, T>(a, sms, s);
+  return a.out_type == PM_F32 ? launch_plain_for<T, float>(a, s) : launch_plain_for<T, T>(a, s);
 }
 
 // ---- launch plan ------------------------------------------------------------------------------------------
@@ -903,13 +958,13 @@ bool tma_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld
 }  // namespace
 
 int launch_linear(const LinearCall& a, cudaStream_t s) {
-  if (!tma_rows(a.x, a.ldx) || !tma_rows(a.w, a.ldw)) {
-    PM_CUDA(a.type == PM_BF16 ? launch_plain<__nv_bfloat16>(a, s) : launch_plain<__half>(a, s));
-    return PM_OK;
-  }
   int dev = 0, cap[kMaxCluster + 1];
   PM_CUDA(cudaGetDevice(&dev));
   PM_CUDA(cluster_capacity(dev, cap));
+  if (!tma_rows(a.x, a.ldx) || !tma_rows(a.w, a.ldw)) {
+    PM_CUDA(a.type == PM_BF16 ? launch_plain<__nv_bfloat16>(a, cap[1], s) : launch_plain<__half>(a, cap[1], s));
+    return PM_OK;
+  }
   FewShape few;
   if (few_shape(a.M, a.N, cap[1], few)) {
     PM_CUDA(a.type == PM_BF16 ? launch_few<__nv_bfloat16>(a, few, s) : launch_few<__half>(a, few, s));

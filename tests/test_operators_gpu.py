@@ -226,6 +226,21 @@ def test_linear_few_tokens(lib, M, K, N, out_dtype):
     check_linear(x, w, randn(g, N).to(F16), "gelu_tanh", randn(g, M, N).to(out_dtype), out_dtype)
 
 
+@pytest.mark.parametrize("M", [1, 8, 9, 16])
+@pytest.mark.parametrize("K,N", [(1, 17), (77, 40), (130, 2369), (1001, 2368), (67, 7105)])
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_linear_few_tokens_off_16_byte_boundaries(lib, M, K, N, out_dtype):
+    """Every offset of rows in a 16-byte word, with values around them that must not count."""
+    g = gen(M + K + N)
+    for lead, pitch in ((1, K + 1), (3, K + 12), (6, K + 7)):
+        xb = torch.full((M * pitch + 16,), float("nan"), dtype=BF16, device="cuda")
+        wb = torch.full((N * (pitch + 2) + 16,), float("nan"), dtype=BF16, device="cuda")
+        x, w = xb.as_strided((M, K), (pitch, 1), lead), wb.as_strided((N, K), (pitch + 2, 1), lead + 1)
+        x.copy_(randn(g, M, K))
+        w.copy_(randn(g, N, K) * 0.1)
+        check_linear(x, w, randn(g, N).to(BF16), "gelu", None, out_dtype)
+
+
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("M,K,N", [(1, 512, 640), (5, 4096, 200), (40, 256, 300), (600, 192, 2304)])
 @pytest.mark.parametrize("out_dtype", [BF16, F32])
