@@ -1,7 +1,7 @@
 // y = act(x w^T + bias) + residual: x [M, K] tokens, w [N, K] weights, bf16 or fp16, float32 sums, one rounding at the end.
 //
 // More than 16 tokens: linear_tc_kernel. Weight rows are the M operand of tcgen05.mma, token rows the N operand, because N can
-// be any multiple of 16: 33 tokens cost 48 columns, a prompt of 777 seven tiles of 112. TMA brings both in steps of 64 or 128 k
+// be any multiple of 16: 33 tokens cost 48 columns, a prompt of 777 nine tiles of 96. TMA brings both in steps of 64 or 128 k
 // into a ring, one thread issues the MMAs, eight warps drain the accumulators (double-buffered in tensor memory)
 // through bias, activation and residual. A lane holds one weight row, so the bias is one load per tile and the lanes of a
 // warp store 32 neighbouring outputs of a token, whatever the alignment of y. Three shapes of it, chosen by an estimate of
@@ -12,8 +12,8 @@
 //           memory, in the order of the ranks: too few tiles for the GPU
 // What bounds it. Large products the tensor cores under the power limit: 8192 x 4096 -> 14336 takes 645 us in a burst = 1.49 PFLOP/s,
 // 0.92 of measured, and 742 us sustained. Few tokens against many weights HBM: 33 x 2048 -> 100003 68 us = 6.0 TB/s, 0.92 of measured. Between them an
-// SM's intake, 124 bytes per ns at most: 777 x 5632 -> 2048 (tiles of 256 x 112, 22 KB a step of 64 k and SM) 25 us where the
-// MMAs alone would take 12. And what comes before and after the k steps: setup and first load 1.5 us, a tile's epilogue
+// SM's intake, 124 bytes per ns at most: 777 x 5632 -> 2048 (tiles of 256 x 96, 22 KB for 64 k and SM) 25 us where the
+// MMAs alone would take 9. And what comes before and after the k steps: setup and first load 1.5 us, a tile's epilogue
 // 0.3 us for each 16 columns and half (a warp's store or remote store of 16 columns takes 600 cycles), joining partial sums 0.7 us for the
 // cluster barrier and as much for the sums. 64 x 4096 -> 4096 11 us, 512 x 3584 -> 4608 18 us.
 //

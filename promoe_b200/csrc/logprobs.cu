@@ -9,7 +9,7 @@
 // A row is read by a cluster of CTAs (one where there are many rows); every thread keeps its own running maximum and
 // sums and rescales them when a batch of its values raises the maximum.
 //
-// The n best come out of the same pass. The first batch gives a floor (of 32 groups of threads the n-th best
+// The n best come out of the same pass. The first batch gives a floor (of 32 or 64 groups of threads the n-th best
 // maximum: n values reach it), later ones raise it; every 16-byte vector with a value that reaches the floor is noted, about
 // 1.5 n of them each time the part read doubles. At the end their values that reach the last floor go to a list, where a
 // value's place is the number of entries before it. Entries are (ordered value, reversed index), so ties go to the lower index and
@@ -17,12 +17,15 @@
 // equal values, ascending rows) finds its n-th best entry by radix selection over the row instead. (Sorting out the values of
 // a vector inside the loop costs registers and code there: 53 and, for n = 20, 90 us instead of 55 and 58 for 1024 rows of 131072.)
 //
-// What bounds it: long rows HBM. 4096 rows of 131072 bf16 take 166 us = 6.49 TB/s without alternatives, 194 us = 5.5 TB/s with
+// What bounds it: long rows HBM. 4096 rows of 131072 bf16 take 166 us = 6.49 TB/s without alternatives, 190 us = 5.65 TB/s with
 // five and 211 us with twenty: the end of a row (two rankings, the noted vectors' way from L2) is latency that four CTAs per SM
 // cover in part. That is at 1965 MHz; after some hundred passes the 1000 W limit takes the clock to 1680 MHz, and the same
-// passes take 197, 229 and about 250 us. Short rows that end too (4096 of 2048: 12 us without alternatives, 23 with five; one warp per row instead
-// of four changed that by less than a fifth). One row of 131072: 7 to 9 us, the chain of load, floor, sums, two cluster
-// barriers and ranking. First form, with scalar arithmetic and the lists sorted out in the loop: 281 us for 4096 rows, 11.5 for one.
+// passes take 197, 223 and about 250 us. Short rows that end too (4096 of 2048: 12 us without alternatives, 21 with five; one warp per row
+// instead of four changed that by less than a fifth). One row of 131072 takes 3.7 us without alternatives, 6 to 6.5 with five, 8
+// with twenty: a chain of load, floor, sums, cluster barrier and ranking, each of them 500 to 1500 cycles, most of which go into the
+// first fetch of its instructions. Hence few unrolled loops and one copy of the ranking. The parts of a row write their
+// sums and best into rank 0's shared memory before the only barrier that anyone waits for (reading them from there
+// behind it: 0.5 us more). First form, with scalar arithmetic and the lists sorted out in the loop: 281 us for 4096 rows, 11.5 for one.
 //
 // Masked logits: -inf has probability 0 and is never an alternative (id -1, log probability -inf where fewer than n are
 // left). A row that holds NaN or +inf, or whose logits are all -inf, is no distribution: NaN and id -1. A negative target names
@@ -37,13 +40,13 @@ namespace {
 
 using sm100::cluster_arrive_diverged;
 using sm100::cluster_rank;
-using sm100::cluster_sync;
 using sm100::cluster_wait_diverged;
 using sm100::map_to_rank;
 using sm100::smem_u32;
 
 constexpr int kCap = 1024;  // room in the lists
 constexpr int kMaxTop = 32;
+constexpr int kMaxParts = 8;  // CTAs of a row
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994531;
 constexpr int kUnroll = 4;  // 16-byte vectors per thread and batch
@@ -201,10 +204,12 @@ template <int THREADS>
 struct LogprobShared {
   alignas(16) Entry list[kCap];
   Sums warp_sums[32];
-  alignas(16) Sums part;  // this CTA's sums, read by rank 0
-  Entry best[kMaxTop];    // this CTA's n best in order, read by rank 0
-  Entry merged[kMaxTop];  // the row's; 0 to begin with
-  float seg[32];          // largest value of each group of threads so far
+  alignas(16) Sums part;  // the row's sums
+  Entry best[kMaxTop];    // the row's n best in order; 0 to begin with
+  // in rank 0, which the others write to: sums and n best of each part
+  alignas(16) Sums part_sums[kMaxParts];
+  alignas(16) Entry part_best[kMaxParts * kMaxTop];
+  float seg[64];          // largest value of each group of threads so far
   int count, n_hot;
   int32_t hot[kCap];   // 16-byte vectors that held a value that reached the floor
   uint32_t hist[256];
@@ -212,34 +217,52 @@ struct LogprobShared {
   int need;
 };
 
-// Entries of `list` in order: out[r] = the r-th largest, r < n; 0 where there are fewer.
+// Entries of `list` in order: the r-th largest to shared memory (of any CTA of the cluster) at out + 8 r, r < n; 0 where there
+// are fewer. Four neighbouring threads compare for one entry. All threads call it; `list` is aligned to 16 bytes. One
+// copy of the code for both rankings of a row: fetching it costs more than running it.
 template <int THREADS>
-__device__ __forceinline__ void rank_list(const Entry* list, int count, Entry* out, int n) {
-  const int tid = threadIdx.x;
-  for (int r = tid; r < n; r += THREADS)
-    if (r >= count) out[r] = 0;
-  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(list);
-  for (int i = tid; i < count; i += THREADS) {
-    const Entry mine = list[i];
-    int before = 0, j = 0;
-    for (; j + 8 <= count; j += 8) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const ulonglong2 o = pairs[j / 2 + k];
-        before += (o.x > mine) + (o.y > mine);
-      }
+__device__ __noinline__ void rank_list(const Entry* list, int count, int n, uint32_t out) {
+  const int tid = threadIdx.x, quarter = tid & 3;
+  auto put = [&](int r, Entry e) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(out + 8u * (uint32_t)r), "l"(e) : "memory"); };
+  for (int r = count + tid; r < n; r += THREADS) put(r, 0);
+  const uint32_t pairs = smem_u32(list);
+#pragma unroll 1
+  for (int i0 = 0; i0 < count; i0 += THREADS / 4) {
+    const int i = i0 + (tid >> 2);
+    const Entry mine = i < count ? list[i] : ~(Entry)0;
+    int before = 0;
+#pragma unroll 2
+    for (int j = quarter; 2 * j < count; j += 4) {
+      const uint4 o = sm100::lds128(pairs + 16u * (uint32_t)j);
+      before += (((Entry)o.y << 32 | o.x) > mine) + (2 * j + 1 < count && ((Entry)o.w << 32 | o.z) > mine);
     }
-    for (; j < count; ++j) before += list[j] > mine;
-    if (before < n) out[before] = mine;
+    before += __shfl_xor_sync(0xffffffffu, before, 1);
+    before += __shfl_xor_sync(0xffffffffu, before, 2);
+    if (i < count && before < n && quarter == 0) put(before, mine);
   }
 }
 
-// The n-th largest of 32 values, one per lane: the least of those that fewer than n exceed.
-__device__ __forceinline__ float nth_best(float mine, int n) {
+// The n-th largest of seg[0 .. 32 or 64): the least of those that fewer than n exceed. Read once: they may rise meanwhile.
+__device__ __forceinline__ float nth_best(const volatile float* seg, bool wide, int n) {
+  const int lane = threadIdx.x & 31;
+  const float a = seg[lane];
   int above = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) above += __shfl_sync(0xffffffffu, mine, i) > mine;
-  return value_of(__reduce_min_sync(0xffffffffu, above < n ? order_of(mine) : 0xffffffffu));
+  for (int i = 0; i < 32; ++i) above += __shfl_sync(0xffffffffu, a, i) > a;
+  uint32_t least = 0xffffffffu;
+  if (wide) {
+    const float b = seg[lane + 32];
+    int above_b = 0;
+#pragma unroll 4
+    for (int i = 0; i < 32; ++i) {
+      const float oa = __shfl_sync(0xffffffffu, a, i), ob = __shfl_sync(0xffffffffu, b, i);
+      above += ob > a;
+      above_b += (oa > b) + (ob > b);
+    }
+    if (above_b < n) least = order_of(b);
+  }
+  if (above < n) least = min(least, order_of(a));
+  return value_of(__reduce_min_sync(0xffffffffu, least));
 }
 
 template <class T, int THREADS>
@@ -251,12 +274,13 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank();
   const int row = blockIdx.x / parts, n = a.n;
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // waited for before rank 0's shared memory is written
   wait_for_predecessor();
 
   const T* l = static_cast<const T*>(a.logits) + (int64_t)row * a.ld;
   const int head = min(a.V, (int)(((16 - ((uintptr_t)l & 15)) & 15) / sizeof(T)));
   const int n_vec = (a.V - head) / N, tail0 = head + n_vec * N;
-  const int v0 = (int)((long long)n_vec * rank / parts), v1 = (int)((long long)n_vec * (rank + 1) / parts);
+  const int v0 = (int)((unsigned)n_vec * rank / (unsigned)parts), v1 = (int)((unsigned)n_vec * (rank + 1) / (unsigned)parts);  // n_vec < 2^29
   const uint4* body = reinterpret_cast<const uint4*>(l + head);
 
   uint4 cur[kUnroll], next[kUnroll];
@@ -278,7 +302,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   T at_target{};
   if (tid == 0 && rank == 0 && a.logp != nullptr) target = a.targets[row];
   if (tid == 0) sh.count = sh.n_hot = 0;
-  if (tid < kMaxTop) sh.merged[tid] = 0;
+  if (tid < kMaxTop) sh.best[tid] = 0;
   __syncthreads();
   auto push = [&](Entry e) {
     const int at = atomicAdd(&sh.count, 1);
@@ -315,12 +339,16 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   }
   const float above_low = __int_as_float(__float_as_int(V::kLow) - 1);  // the next number; raised values are not noted
   float floor_v = above_low;
+  // Many alternatives want more groups: the 32nd best of 32 maxima is their least, which some 130 values reach, and the lists of
+  // rows of 50000 overflowed (300 of them, n = 32: 220 to 490 us; of 64 groups 27 us). Ranking 64 values takes every warp
+  // three times as many shuffles (one row of 131072, n = 20, where 31 values reach the floor of 32 groups: 8.3 -> 9.6 us).
+  const bool wide = n > 24;
   auto group_best = [&]() {
-    constexpr int kGroup = THREADS / 32;
     float g = m;
 #pragma unroll
-    for (int d = kGroup / 2; d >= 1; d >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
-    if (tid % kGroup == 0) sh.seg[tid / kGroup] = g;
+    for (int d = 1; d < THREADS / 64; d <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, d));
+    if (!wide) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, THREADS / 64));
+    if (tid % (wide ? THREADS / 64 : THREADS / 32) == 0) sh.seg[tid / (wide ? THREADS / 64 : THREADS / 32)] = g;
   };
   int batch = 0;
   for (int base = v0; base < v1; base += kBatch, ++batch) {
@@ -347,13 +375,13 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
         add_pair(V::pair(cur[k], i + 1), minus_c, s3, u3);
       }
     if (n == 0) continue;
-    if ((batch & (batch + 1)) == 0) {  // batches 0, 1, 3, 7, ...
+    if ((batch & (batch + 1)) == 0 && (batch == 0 || base + kBatch < v1)) {  // batches 0, 1, 3, 7, ...
       group_best();
       // At first every group has to have its value there. Later a warp may see other groups' older, lower ones: they are
       // maxima of those groups all the same. (It takes them once: they may rise while it compares them.)
       if (batch == 0) __syncthreads();
       else __syncwarp();
-      floor_v = fmaxf(nth_best(*(volatile float*)&sh.seg[lane], n), above_low);
+      floor_v = fmaxf(nth_best(sh.seg, wide, n), above_low);
     }
     if (all >= floor_v) {
 #pragma unroll
@@ -381,10 +409,16 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   if (lane == 0) sh.warp_sums[warp] = a0;
   if (n > 0 && batch > 1) group_best();
   __syncthreads();
+  if (parts > 1) cluster_wait_diverged();
   if (warp == 0) {
     Sums t = lane < THREADS / 32 ? sh.warp_sums[lane] : no_sums<T>();
     join_lanes(t, THREADS / 32);
-    if (lane == 0) sh.part = t;
+    if (lane == 0) {
+      if (parts == 1) sh.part = t;
+      else
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(map_to_rank(smem_u32(&sh.part_sums[rank]), 0)),
+                     "f"(t.m), "f"(t.c), "f"(t.s), "f"(t.u) : "memory");
+    }
   }
   if (n > 0) {
     const bool all_hot = sh.n_hot <= kCap;
@@ -392,7 +426,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     if (all_hot) {
       // the noted vectors once more, against the last floor
       // (after a single batch the loop's is the last)
-      if (batch > 1) floor_v = fmaxf(nth_best(sh.seg[lane], n), above_low);
+      if (batch > 1) floor_v = fmaxf(nth_best(sh.seg, wide, n), above_low);
       const bool low = floor_v == above_low;
       for (int i = tid; i < sh.n_hot; i += THREADS) {
         const int at = head + sh.hot[i] * N;
@@ -468,34 +502,32 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
       __syncthreads();
       count = sh.count;
     }
-    rank_list<THREADS>(sh.list, count, sh.best, n);
+    rank_list<THREADS>(sh.list, count, n, parts == 1 ? smem_u32(sh.best) : map_to_rank(smem_u32(&sh.part_best[rank * n]), 0));
   }
   if (parts > 1) {
-    cluster_sync();
-    if (rank == 0) {
-      if (warp == 0) {
-        Sums t = no_sums<T>();
-        if (lane < parts)
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(t.m), "=f"(t.c), "=f"(t.s), "=f"(t.u)
-                       : "r"(map_to_rank(smem_u32(&sh.part), lane)));
-        join_lanes(t, 8);
-        __syncwarp();
-        if (lane == 0) sh.part = t;
-      }
-      // the parts' best, which fill the list whether there are that many or not (0 ranks behind every entry)
+    cluster_arrive_diverged();
+    if (rank != 0) return;
+    cluster_wait_diverged();  // the parts' sums and best are there
+    if (warp == 0) {
+      Sums t = lane < parts ? sh.part_sums[lane] : no_sums<T>();
+      join_lanes(t, kMaxParts);
+      if (lane == 0) sh.part = t;
+    }
+    // Entries of 0 rank behind every other. Of many, only those that reach the least of the parts' ceil(n / parts)-th best, at least
+    // n of them, are ranked (160 of 8 parts: 1.8 us all of them).
+    if (n > 0 && parts * n <= THREADS / 4) {
+      rank_list<THREADS>(sh.part_best, parts * n, n, smem_u32(sh.best));
+    } else if (n > 0) {
+      Entry least = ~(Entry)0;
+      for (int p = 0; p < parts; ++p) least = min(least, sh.part_best[p * n + (n - 1) / parts]);
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
       for (int i = tid; i < parts * n; i += THREADS)
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(sh.list[i]) : "r"(map_to_rank(smem_u32(&sh.best[i % n]), i / n)));
+        if (sh.part_best[i] >= least && sh.part_best[i] != 0) push(sh.part_best[i]);
+      __syncthreads();
+      rank_list<THREADS>(sh.list, sh.count, n, smem_u32(sh.best));
     }
-    cluster_arrive_diverged();  // the others leave once their parts were read, which the first one does not wait for
-    if (rank != 0) {
-      cluster_wait_diverged();
-      return;
-    }
-    __syncthreads();
-    if (n > 0) rank_list<THREADS>(sh.list, parts * n, sh.merged, n);
   }
-  const Entry* best = parts > 1 ? sh.merged : sh.best;
   __syncthreads();
 
   Sums t = sh.part;
@@ -552,7 +584,6 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     }
     if (bad) t.s = CUDART_NAN_F;
   }
-  if (parts > 1) cluster_wait_diverged();
   if (warp != 0) return;
   const bool dead = !(t.s > 0.f) || !(fabsf(t.m) < CUDART_INF_F);
   const float log_s = logf(t.s);
@@ -564,7 +595,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     if (a.entropy != nullptr) a.entropy[row] = dead ? CUDART_NAN_F : fmaf(-(float)kLn2, t.u / t.s, log_s);
   }
   if (lane < n) {
-    const Entry e = dead ? 0 : best[lane];
+    const Entry e = dead ? 0 : sh.best[lane];
     a.top_ids[(int64_t)row * n + lane] = e == 0 ? -1 : (int32_t)(0xffffffffu - (uint32_t)e);
     a.top_logp[(int64_t)row * n + lane] =
         dead ? CUDART_NAN_F : e == 0 ? -CUDART_INF_F : (float)((double)value_of((uint32_t)(e >> 32)) - lse);
@@ -591,7 +622,7 @@ template <class T>
 cudaError_t pick(const LogprobArgs& a, int sms, cudaStream_t s) {
   // a cluster per row while that fills the GPU no more than about twice and a part stays longer than a batch of 128 threads
   int parts = 1;
-  while (parts < 8 && (int64_t)a.T * parts * 2 <= 2 * sms && a.V / (2 * parts) >= 4096) parts *= 2;
+  while (parts < kMaxParts && (int64_t)a.T * parts * 2 <= 2 * sms && a.V / (2 * parts) >= 4096) parts *= 2;
   // Every thread should have half a batch, and each of the 32 groups of threads values for the floor. Parts of a row are
   // short: more threads finish sooner. Whole rows leave room for other rows' CTAs, which work while one row is finished.
   const int vectors = a.V / parts / Vec<T>::kN;

@@ -399,6 +399,19 @@ def test_logprobs_masks_and_rows_without_a_distribution(lib, V, dtype):
     check_logprobs(logits, targets, n)
 
 
+@pytest.mark.parametrize("T,V", [(1, 131072), (9, 40000), (200, 3000)])
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 24, 25, 32])
+def test_logprobs_every_number_of_alternatives(lib, T, V, n):
+    g = gen(T + n)
+    for order in ("random", "ascending", "descending", "equal"):
+        logits = 3 * randn(g, T, V)
+        if order in ("ascending", "descending"):  # lists that overflow; the best of one part of the row alone
+            logits = logits.sort(1, descending=order == "descending").values.contiguous()
+        elif order == "equal":
+            logits = logits.round()
+        check_logprobs(logits.to(BF16), torch.randint(0, V, (T,), generator=g, device="cuda"), n)
+
+
 def test_logprobs_strided_rows_off_boundaries(lib):
     g = gen(4)
     wide = 2 * randn(g, 11, 9100)
