@@ -123,27 +123,27 @@ __device__ __forceinline__ void tile_at(const LinearTc& a, int tile, int& wt, in
   wt = band * kBand + in - tt * high;
 }
 
-// C neighbouring tokens from token m on of weight row n (one row per lane), `left` of them inside y: bias, activation,
+// C neighbouring tokens from token m on of weight row n (one row per lane), `left` of them inside y: the residual there; bias, activation,
 // residual, rounding, store. A chunk that lies inside y as a whole takes a form without tests: those made 17 instructions of
 // the 6 per output, which bounds products with a short K.
 template <class OT, int C>
-__device__ __forceinline__ void finish(const LinearTc& a, float (&o)[C], float bias, int64_t m, int n, int left) {
-  const bool whole = __all_sync(0xffffffffu, left >= C), add = a.res != nullptr;
-  OT r[C];
-  if (add) {
-    const OT* src = static_cast<const OT*>(a.res) + m * a.ldr + n;
-    if (whole) {
+__device__ __forceinline__ void load_residual(const LinearTc& a, OT (&r)[C], int64_t m, int n, int left) {
+  const OT* src = static_cast<const OT*>(a.res) + m * a.ldr + n;
+  if (__all_sync(0xffffffffu, left >= C)) {
 #pragma unroll
-      for (int c = 0; c < C; ++c, src += a.ldr) r[c] = *src;
-    } else {
+    for (int c = 0; c < C; ++c, src += a.ldr) r[c] = *src;
+  } else {
 #pragma unroll
-      for (int c = 0; c < C; ++c, src += a.ldr) r[c] = c < left ? *src : from_float<OT>(0.f);
-    }
+    for (int c = 0; c < C; ++c, src += a.ldr) r[c] = c < left ? *src : from_float<OT>(0.f);
   }
+}
+template <class OT, int C, bool ADD>
+__device__ __forceinline__ void finish(const LinearTc& a, float (&o)[C], const OT (&r)[C], float bias, int64_t m, int n, int left) {
+  const bool whole = __all_sync(0xffffffffu, left >= C);
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] += bias;
   activate_all(o, a.act);
-  if (add) {
+  if (ADD) {
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] += to_float<OT>(r[c]);
   }
@@ -301,13 +301,29 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       const int n = (wt * CG + (int)rank) * 128 + 32 * w + lane;
       const int m0 = tt * a.width, cols = min(a.width, a.M - m0);
       bias = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
+      // The residual of a chunk is asked for one chunk ahead, the first one's while the tile is still being multiplied.
+      const bool add = a.res != nullptr && !split;
+      OT ahead[16] = {};
+      auto ask = [&](int c0) {
+        if (add && c0 < cols) load_residual<OT, 16>(a, ahead, m0 + c0, n, n < a.N ? cols - c0 : 0);
+      };
+      ask(half * 16);
       auto give = [&](float (&o)[16], int c0) {
         if (!ok) {
 #pragma unroll
           for (int c = 0; c < 16; ++c) o[c] = nan;
         }
         if (!split) {
-          finish<OT, 16>(a, o, bias, m0 + c0, n, n < a.N ? cols - c0 : 0);
+          const int left = n < a.N ? cols - c0 : 0;
+          if (!add) {
+            finish<OT, 16, false>(a, o, ahead, bias, m0 + c0, n, left);
+          } else {
+            OT r[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) r[c] = ahead[c];
+            ask(c0 + 32);
+            finish<OT, 16, true>(a, o, r, bias, m0 + c0, n, left);
+          }
         } else {
           // four columns at a time to the CTA that finishes them, which keeps [source][its fours of columns][128 rows][4]
           const int per = a.part_cols;
@@ -395,7 +411,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
           o[0] += u.x, o[1] += u.y, o[2] += u.z, o[3] += u.w;
           o[4] += v.x, o[5] += v.y, o[6] += v.z, o[7] += v.w;
         }
-        finish<OT, 8>(a, o, bias, m0 + c_first + c0, n, n < a.N ? mine - c0 : 0);
+        const int left = n < a.N ? mine - c0 : 0;
+        OT r[8] = {};
+        if (a.res != nullptr) load_residual<OT, 8>(a, r, m0 + c_first + c0, n, left);
+        finish<OT, 8, true>(a, o, r, bias, m0 + c_first + c0, n, left);
       }
     }
   }
