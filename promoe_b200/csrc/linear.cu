@@ -123,9 +123,9 @@ __device__ __forceinline__ void tile_at(const LinearTc& a, int tile, int& wt, in
   wt = band * kBand + in - tt * high;
 }
 
-// C neighbouring tokens from token m on of weight row n (one row per lane), `left` of them inside y: the residual there; bias, activation,
-// residual, rounding, store. A chunk that lies inside y as a whole takes a form without tests: those made 17 instructions of
-// the 6 per output, which bounds products with a short K.
+// C neighbouring tokens from token m on of weight row n (one row per lane), `left` of them inside y: their residual; and bias,
+// activation, residual, rounding, store. A chunk that lies inside y as a whole takes forms without tests: those made 17
+// instructions of the 6 per output, which bounds products with a short K.
 template <class OT, int C>
 __device__ __forceinline__ void load_residual(const LinearTc& a, OT (&r)[C], int64_t m, int n, int left) {
   const OT* src = static_cast<const OT*>(a.res) + m * a.ldr + n;
@@ -301,7 +301,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       const int n = (wt * CG + (int)rank) * 128 + 32 * w + lane;
       const int m0 = tt * a.width, cols = min(a.width, a.M - m0);
       bias = n < a.N ? load_bias(a.bias, a.bias_type, n) : 0.f;
-      // The residual of a chunk is asked for one chunk ahead, the first one's while the tile is still being multiplied.
+      // The residual of a chunk is asked for one chunk ahead, the first one's while the tile is still being multiplied (777 x
+      // 5632 -> 2048 27.6 -> 26.9 us, 8192 x 64 -> 8192 137 -> 128 us).
       const bool add = a.res != nullptr && !split;
       OT ahead[16] = {};
       auto ask = [&](int c0) {
