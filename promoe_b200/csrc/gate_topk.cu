@@ -177,7 +177,7 @@ __device__ __forceinline__ int finish_token_by_rule(const float* logit_s, int t,
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) l[i] = i < npl && lane * npl + i < E ? logit_s[lane * npl + i] : -CUDART_INF_F;
   const float bias_max = load_choice_bias<kPerLane>(rule, npl, lane, b);
-  route_token<kPerLane>(l, npl, rule, b, bias_max, RouteGroups(rule, npl, lane), scratch, lane, [&](int e) { return logit_s[e]; },
+  route_token<kPerLane, kAnyRule>(l, npl, rule, b, bias_max, RouteGroups(rule, npl, lane), scratch, lane, [&](int e) { return logit_s[e]; },
                         [&](int j, int id, float w) {
     topk_ids[(size_t)t * k + j] = id;
     topk_w[(size_t)t * k + j] = w;

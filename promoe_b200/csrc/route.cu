@@ -2,12 +2,11 @@
 // One warp per token, the row in registers: lane i holds npl = ceil(E / 32) neighbouring experts.
 //
 // Bound by instructions, not by bytes: 16384 rows of 256 float32 logits are 16.8 MB, 2.6 us at the measured copy rate, and take
-// 11.9 us for 8 of softmax scores (570 instructions a row), 13.5 us
-// with sigmoid scores and a bias, 20 us with the best 4 of 8 groups as well (820 instructions a row). One token to 64 take
-// 3.1 us, launch included. What it took to get there (the last case): integer divisions and group geometry out of the loop over
-// rows, numbers ranked as numbers (redux.sync of floats) instead of as ordered integers: 28 -> 22 us; the exact ranking of a row
-// with close neighbours by its candidates alone, one lane each, instead of all its experts: 64 tokens, one of them such a
-// row, 9.7 -> 3.9 us.
+// 10.5 us for 8 of softmax scores, 11.8 us with sigmoid scores and a bias, 18.8 us with the best 4 of 8 groups as well (some 750
+// instructions a row, 2.7 a cycle and SM). One token to 64 take 2.1 to 3.3 us, launch included. What it took to get there (the
+// last case): integer divisions and group geometry out of the loop over rows, numbers ranked as numbers (redux.sync of floats)
+// instead of as ordered integers: 28 -> 20 us; the exact ranking of a row with close neighbours by its candidates alone, one
+// lane each, instead of all its experts: 64 tokens, one of them such a row, 9.7 -> 3.9 us.
 #include <algorithm>
 
 #include "route_select.cuh"
@@ -28,7 +27,7 @@ __device__ __forceinline__ float load_logit(const __half* p) { return __half2flo
 // 25 us.
 constexpr int blocks_per_sm(int npl) { return npl <= 8 ? 6 : npl <= 16 ? 4 : 3; }
 
-template <class T, int NPL>
+template <class T, int NPL, int KIND>
 __global__ void __launch_bounds__(kRouteWarps * 32, blocks_per_sm(NPL))
 route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_constant__ RouteRule rule, int vector_loads,
              int32_t* __restrict__ topk_ids, float* __restrict__ topk_w) {
@@ -68,7 +67,7 @@ route_kernel(const T* __restrict__ logits, int64_t ld, int n_tok, const __grid_c
   for (int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp; t < n_tok; t += step) {
     load(t);
     const T* row = logits + t * ld;
-    route_token<NPL>(l, npl, rule, b, bias_max, groups, scratch, lane, [&](int e) { return load_logit(row + e); },
+    route_token<NPL, KIND>(l, npl, rule, b, bias_max, groups, scratch, lane, [&](int e) { return load_logit(row + e); },
                      [&](int j, int id, float w) {
                        topk_ids[t * rule.k + j] = id;
                        topk_w[t * rule.k + j] = w;
@@ -87,7 +86,18 @@ cudaError_t launch(const T* logits, int64_t ld, int n_tok, const RouteRule& rule
   if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
   // One row after the other per warp once every SM has its blocks; at most 35 KB of shared memory per block.
   const int blocks = std::min((n_tok + kRouteWarps - 1) / kRouteWarps, sms * blocks_per_sm(NPL));
-  return launch_behind(route_kernel<T, NPL>, blocks, kRouteWarps * 32, kRouteWarps * route_scratch_bytes(rule.E), s, logits, ld,
+  // Kernels of their own for the usual kinds of rules: 16384 tokens of 256 experts, softmax 11.8 -> 10.5 us, sigmoid and bias 13.5 ->
+  // 11.8, with groups 20.3 -> 18.8. Wider rows are too rare for that.
+  auto kern = route_kernel<T, NPL, kAnyRule>;
+  if constexpr (NPL <= 16) {
+    switch (route_kind(rule)) {
+      case 0: kern = route_kernel<T, NPL, 0>; break;
+      case kGrouped: kern = route_kernel<T, NPL, kGrouped>; break;
+      case kSigmoid | kHasBias: kern = route_kernel<T, NPL, kSigmoid | kHasBias>; break;
+      case kSigmoid | kHasBias | kGrouped: kern = route_kernel<T, NPL, kSigmoid | kHasBias | kGrouped>; break;
+    }
+  }
+  return launch_behind(kern, blocks, kRouteWarps * 32, kRouteWarps * route_scratch_bytes(rule.E), s, logits, ld,
                        n_tok, rule, vector_loads, ids, w);
 }
 

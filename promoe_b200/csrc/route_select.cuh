@@ -184,12 +184,19 @@ __device__ __forceinline__ float load_choice_bias(const RouteRule& r, int npl, i
 
 // Row of a token: experts lane * npl .. lane * npl + npl - 1 are l[0 .. npl) of this lane (-inf beyond E; npl <= NPL), b and
 // bias_max from load_choice_bias, groups of this lane. logit(e) reads the row again. write(j, id, weight) is called once for each j < k, by any lane.
-template <int NPL, class Logit, class Write>
+// KIND: what of the rule is fixed when the code is compiled (route_kind), or kAnyRule.
+constexpr int kAnyRule = -1, kHasBias = 1, kGrouped = 2, kSigmoid = 4;
+__host__ __device__ __forceinline__ int route_kind(const RouteRule& r) {
+  return (r.bias != nullptr ? kHasBias : 0) | (r.n_group > 1 && r.topk_group < r.n_group ? kGrouped : 0) | (r.sigmoid ? kSigmoid : 0);
+}
+template <int NPL, int KIND, class Logit, class Write>
 __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, const RouteRule& r, const float (&b)[NPL], float bias_max,
                                             const RouteGroups& groups, RouteScratch* scratch, int lane, const Logit& logit, const Write& write) {
   const int E = r.E, e0 = lane * npl;
   double* work = reinterpret_cast<double*>(scratch + 1);
-  const bool by_logit = r.bias == nullptr, grouped = r.n_group > 1 && r.topk_group < r.n_group, sums = grouped && r.group_top2 != 0;
+  const int kind = KIND == kAnyRule ? route_kind(r) : KIND;
+  const bool by_logit = !(kind & kHasBias), grouped = (kind & kGrouped) != 0, sigmoid = (kind & kSigmoid) != 0;
+  const bool sums = grouped && r.group_top2 != 0;
   bool odd = false;
 #pragma unroll
   for (int j = 0; j < NPL; ++j) odd |= !(fabsf(l[j]) < CUDART_INF_F);
@@ -197,7 +204,7 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   if (odd) {
     bool dead = false;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) dead |= l[j] != l[j] || (!r.sigmoid && l[j] == CUDART_INF_F);
+    for (int j = 0; j < NPL; ++j) dead |= l[j] != l[j] || (!sigmoid && l[j] == CUDART_INF_F);
     if (__any_sync(0xffffffffu, dead)) {
       if (lane < r.k) write(lane, -1, CUDART_NAN_F);
       return;
@@ -208,7 +215,7 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   // two or three), a choice by that and half a step of its own.
   float sum = 0.f, top = 0.f, margin = 0.f;
   float c[NPL];  // choices
-  if (!r.sigmoid) {
+  if (!sigmoid) {
     top = -CUDART_INF_F;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) top = fmaxf(top, l[j]);
@@ -223,9 +230,9 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
     for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   }
   if (!by_logit || sums) {
-    const float inv = r.sigmoid ? 1.f : 1.f / sum;
-    margin = (r.sigmoid ? 1e-6f : 4e-6f * inv) + 1e-6f * bias_max;
-    if (r.sigmoid) {
+    const float inv = sigmoid ? 1.f : 1.f / sum;
+    margin = (sigmoid ? 1e-6f : 4e-6f * inv) + 1e-6f * bias_max;
+    if (sigmoid) {
 #pragma unroll
       for (int j = 0; j < NPL; ++j) c[j] = fast_sigmoid(l[j]) + b[j];
     } else {
@@ -387,11 +394,11 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
       const bool close = rank < r.k && rank + 1 < n && choice - __uint_as_float(scratch->key[rank + 1]) < margin;
       if (__any_sync(0xffffffffu, close)) {
         double sum64 = 1.0;
-        if (!r.sigmoid) {
+        if (!sigmoid) {
           stage_logits();
           sum64 = exact_sum(work, E, (double)top, lane);
         }
-        rank = exact_candidates((double)v_id, lane < n ? r.bias[id] : 0.f, (double)top, sum64, r.sigmoid, n, lane);
+        rank = exact_candidates((double)v_id, lane < n ? r.bias[id] : 0.f, (double)top, sum64, sigmoid, n, lane);
       }
     }
   } else {
@@ -437,7 +444,7 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   }
   const bool chosen = id >= 0 && rank < r.k;
   float w = 0.f;
-  if (chosen) w = r.sigmoid ? __fdividef(1.f, 1.f + expf(-v_id)) : __fdividef(expf(v_id - top), sum);
+  if (chosen) w = sigmoid ? __fdividef(1.f, 1.f + expf(-v_id)) : __fdividef(expf(v_id - top), sum);
   if (r.norm) {
     float all = w;
 #pragma unroll
