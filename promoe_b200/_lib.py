@@ -135,7 +135,7 @@ SIGNATURES = {
     "pm_k_predictor_mlp": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp]),
     "pm_k_rank_topn": (_i, [_vp, _i, _i, _vp, _vp]),
     "pm_k_route": (_i, [C.POINTER(pm_router), _vp, _i, _i64, _i, _vp, _vp, _vp]),
-    "pm_k_linear": (_i, [C.POINTER(pm_linear), _vp]),
+    "pm_k_linear": (_i, [_vp, _vp]),  # a pm_linear by reference, or its bytes
     "pm_k_token_logprobs": (_i, [_vp, _i, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
 }
 _RAW = {"pm_version", "pm_last_error", "pm_k_swiglu_ffn_scratch_bytes", "pm_k_swiglu_ffn_static_capacity"}

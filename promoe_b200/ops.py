@@ -9,6 +9,7 @@ No gradients: tensors that require one are refused while autograd records.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -22,17 +23,14 @@ _GROUP_SCORE = {"max": 0, "top2": 1}
 
 # The stream as an integer, without the Stream object that torch.cuda.current_stream makes (1 us of a call that takes 5).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_I32, _F32 = torch.int32, torch.float32
 
 
-def _call(index: int, fn, *args) -> None:
+def _elsewhere(index: int, fn, *args) -> int:
     """fn(*args, stream) with device `index` current, on its current stream."""
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _lib.check(rc)
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
 def _matrix(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES) -> tuple[int, int, int, int]:
@@ -53,14 +51,6 @@ def _matrix(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient: these operators have no backward pass")
     return index, rows, n, pitch
-
-
-def _result(out, shape, dtype, index: int, what: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=torch.device("cuda", index))
-    if out.shape != shape or out.dtype != dtype or out.get_device() != index or not out.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index}")
-    return out
 
 
 class Router:
@@ -94,10 +84,25 @@ class Router:
         if self.device_index is not None and self.device_index != index:
             raise ValueError(f"logits must be on cuda:{self.device_index}, where the bias is")
         shape = (T, self.top_k)
-        ids, w = out if out is not None else (None, None)
-        ids, w = _result(ids, shape, torch.int32, index, "ids"), _result(w, shape, torch.float32, index, "weights")
-        _call(index, self._fn, self._ref, logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, ids.data_ptr(), w.data_ptr())
+        if out is None:
+            device = logits.device
+            ids, w = torch.empty(shape, dtype=_I32, device=device), torch.empty(shape, dtype=_F32, device=device)
+        else:
+            ids, w = out
+            if not (ids.shape == shape == w.shape and ids.dtype is _I32 and w.dtype is _F32 and ids.get_device() == index
+                    and w.get_device() == index and ids.is_contiguous() and w.is_contiguous()):
+                raise ValueError(f"out must be contiguous int32 and float32 tensors of shape {shape} on cuda:{index}")
+        if index == _current_device():
+            rc = self._fn(self._ref, logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, ids.data_ptr(), w.data_ptr(), _raw_stream(index))
+        else:
+            rc = _elsewhere(index, self._fn, self._ref, logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, ids.data_ptr(), w.data_ptr())
+        if rc:
+            _lib.check(rc)
         return ids, w
+
+
+# struct pm_linear as bytes, in one step: filling the ctypes structure takes 0.5 us more
+_PM_LINEAR = struct.Struct("@5P4q7iP").pack
 
 
 class Linear:
@@ -124,10 +129,8 @@ class Linear:
                 raise ValueError(f"bias must be on cuda:{index}, not on {bias.device}")
         self.weight, self.bias, self.out_dtype, self.device_index, self.N, self.K = weight, bias, out_dtype, index, N, K
         self._x_dtypes, self._y_dtypes = (weight.dtype,), (out_dtype,)
-        # what stays the same from call to call; a call works on a copy, so that two threads may call at once
-        self._call = bytes(_lib.pm_linear(bias=None if bias is None else bias.data_ptr(), ld_w=pitch, N=N, K=K,
-                                          dtype=_DTYPES[weight.dtype], out_dtype=_DTYPES[out_dtype],
-                                          bias_dtype=0 if bias is None else _DTYPES[bias.dtype], act=_ACTS[activation]))
+        self._bias_ptr, self._ld_w = 0 if bias is None else bias.data_ptr(), pitch
+        self._kind = (N, K, _DTYPES[weight.dtype], _DTYPES[out_dtype], 0 if bias is None else _DTYPES[bias.dtype], _ACTS[activation], 0)
         self._fn = _lib.load().pm_k_linear
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -142,23 +145,21 @@ class Linear:
         on_y, rows, _, ld_y = _matrix(out, "out", self.N, self._y_dtypes)
         if rows != M:
             raise ValueError(f"out must have {M} rows, not {rows}")
-        a = _lib.pm_linear.from_buffer_copy(self._call)
-        a.x, a.w, a.y, a.ld_x, a.ld_y, a.M = x.data_ptr(), self.weight.data_ptr(), out.data_ptr(), ld_x, ld_y, M
+        res, ld_r = 0, 0
         if residual is not None:
-            on_r, rows, _, a.ld_residual = _matrix(residual, "residual", self.N, self._y_dtypes)
+            on_r, rows, _, ld_r = _matrix(residual, "residual", self.N, self._y_dtypes)
             if rows != M:
                 raise ValueError(f"residual must have {M} rows, not {rows}")
             if on_r != index:
                 raise ValueError(f"residual must be on cuda:{index}, where the weight is")
-            a.residual = residual.data_ptr()
+            res = residual.data_ptr()
         if on != index or on_y != index:
             raise ValueError(f"x and out must be on cuda:{index}, where the weight is")
-        _call(index, self._fn, C.byref(a))
+        a = _PM_LINEAR(x.data_ptr(), self.weight.data_ptr(), self._bias_ptr, res, out.data_ptr(), ld_x, self._ld_w, ld_r, ld_y, M, *self._kind)
+        rc = self._fn(a, _raw_stream(index)) if index == _current_device() else _elsewhere(index, self._fn, a)
+        if rc:
+            _lib.check(rc)
         return out
-
-
-def _logprobs():
-    return _lib.load().pm_k_token_logprobs
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, out=None):
@@ -172,9 +173,21 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, 
         raise ValueError("top_n must not be negative")
     if targets.shape != (T,) or targets.dtype != torch.int64 or targets.get_device() != index or not targets.is_contiguous():
         raise ValueError(f"targets must be a contiguous int64 tensor of shape [{T}] on cuda:{index}")
-    logp, entropy, ids, best = out if out is not None else (None, None, None, None)
-    logp, entropy = _result(logp, (T,), torch.float32, index, "logp"), _result(entropy, (T,), torch.float32, index, "entropy")
-    ids, best = _result(ids, (T, top_n), torch.int32, index, "top_ids"), _result(best, (T, top_n), torch.float32, index, "top_logp")
-    _call(index, _logprobs(), logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, V, targets.data_ptr(), top_n, logp.data_ptr(),
-          entropy.data_ptr(), ids.data_ptr(), best.data_ptr())
+    if out is None:
+        new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=logits.device)  # noqa: E731
+        logp, entropy, ids, best = new((T,), _F32), new((T,), _F32), new((T, top_n), _I32), new((T, top_n), _F32)
+    else:
+        logp, entropy, ids, best = out
+        row, wide = (T,), (T, top_n)
+        if not (logp.shape == row == entropy.shape and ids.shape == wide == best.shape and ids.dtype is _I32
+                and logp.dtype is entropy.dtype is best.dtype is _F32 and logp.get_device() == index and entropy.get_device() == index
+                and ids.get_device() == index and best.get_device() == index and logp.is_contiguous() and entropy.is_contiguous()
+                and ids.is_contiguous() and best.is_contiguous()):
+            raise ValueError(f"out must be contiguous tensors on cuda:{index}: float32 {row} twice, int32 and float32 {wide}")
+    args = (logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, V, targets.data_ptr(), top_n, logp.data_ptr(), entropy.data_ptr(),
+            ids.data_ptr(), best.data_ptr())
+    fn = _lib.load().pm_k_token_logprobs
+    rc = fn(*args, _raw_stream(index)) if index == _current_device() else _elsewhere(index, fn, *args)
+    if rc:
+        _lib.check(rc)
     return logp, entropy, ids, best
