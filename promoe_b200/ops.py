@@ -21,9 +21,10 @@ _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
 
 
-# The stream as an integer, without the Stream object that torch.cuda.current_stream makes (1 us of a call that takes 5).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# The stream as an integer, without the Stream object that torch.cuda.current_stream makes (1 us of a call that takes 5). A torch
+# built without CUDA has neither; it has no CUDA tensors to call these operators with either.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 _I32, _F32 = torch.int32, torch.float32
 
 
@@ -39,6 +40,8 @@ def _matrix(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES
     if index < 0 or len(shape) != 2 or t.dtype not in dtypes:
         raise ValueError(f"{what} must be a 2-D CUDA tensor of {', '.join(str(d) for d in dtypes)}")
     rows, n = shape
+    if rows > 0x7fffffff or n > 0x7fffffff:  # ctypes would cut them off
+        raise ValueError(f"{what} has too many rows or columns")
     if width is not None and n != width:
         raise ValueError(f"{what} must have rows of {width} values, not {n}")
     pitch, inner = t.stride()
@@ -89,8 +92,12 @@ class Router:
             ids, w = torch.empty(shape, dtype=_I32, device=device), torch.empty(shape, dtype=_F32, device=device)
         else:
             ids, w = out
-            if not (ids.shape == shape == w.shape and ids.dtype is _I32 and w.dtype is _F32 and ids.get_device() == index
-                    and w.get_device() == index and ids.is_contiguous() and w.is_contiguous()):
+            try:
+                fits = (ids.shape == shape == w.shape and ids.dtype is _I32 and w.dtype is _F32 and ids.get_device() == index
+                        and w.get_device() == index and ids.is_contiguous() and w.is_contiguous())
+            except AttributeError:  # no tensors
+                fits = False
+            if not fits:
                 raise ValueError(f"out must be contiguous int32 and float32 tensors of shape {shape} on cuda:{index}")
         if index == _current_device():
             rc = self._fn(self._ref, logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, ids.data_ptr(), w.data_ptr(), _raw_stream(index))
@@ -179,10 +186,14 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, 
     else:
         logp, entropy, ids, best = out
         row, wide = (T,), (T, top_n)
-        if not (logp.shape == row == entropy.shape and ids.shape == wide == best.shape and ids.dtype is _I32
-                and logp.dtype is entropy.dtype is best.dtype is _F32 and logp.get_device() == index and entropy.get_device() == index
-                and ids.get_device() == index and best.get_device() == index and logp.is_contiguous() and entropy.is_contiguous()
-                and ids.is_contiguous() and best.is_contiguous()):
+        try:
+            fits = (logp.shape == row == entropy.shape and ids.shape == wide == best.shape and ids.dtype is _I32
+                    and logp.dtype is entropy.dtype is best.dtype is _F32 and logp.get_device() == index and entropy.get_device() == index
+                    and ids.get_device() == index and best.get_device() == index and logp.is_contiguous() and entropy.is_contiguous()
+                    and ids.is_contiguous() and best.is_contiguous())
+        except AttributeError:  # no tensors
+            fits = False
+        if not fits:
             raise ValueError(f"out must be contiguous tensors on cuda:{index}: float32 {row} twice, int32 and float32 {wide}")
     args = (logits.data_ptr(), _DTYPES[logits.dtype], pitch, T, V, targets.data_ptr(), top_n, logp.data_ptr(), entropy.data_ptr(),
             ids.data_ptr(), best.data_ptr())

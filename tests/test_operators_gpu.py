@@ -578,7 +578,12 @@ def test_calls_that_are_refused(lib):
            lambda: router(torch.zeros((3, 64), device="cuda"), out=(torch.zeros((3, 6), device="cuda"),) * 2),
            lambda: ops.token_logprobs(head(x), targets.int(), 1), lambda: ops.token_logprobs(head(x), targets[:2], 1),
            lambda: ops.token_logprobs(head(x), targets.cpu(), 1),
-           lambda: ops.token_logprobs(head(x), targets, 1, out=(torch.empty(2, device="cuda"), None, None, None))]
+           lambda: ops.token_logprobs(head(x), targets, 1, out=(torch.empty(2, device="cuda"), None, None, None)),
+           lambda: ops.token_logprobs(head(x), targets, 1, out=(torch.empty(3, device="cuda"), None, None, None)),
+           lambda: ops.token_logprobs(head(x), targets, -1),
+           lambda: router(torch.zeros((3, 64), device="cuda"), out=(None, None)),
+           lambda: router(torch.zeros((3, 64), device="cuda"), out=(torch.zeros((3, 6), dtype=torch.int32), torch.zeros((3, 6), device="cuda"))),
+           lambda: ops.token_logprobs(torch.empty(1, device="cuda").expand(2 ** 32 + 1, 1), targets, 0)]
     for i, f in enumerate(bad):
         with pytest.raises(ValueError):
             f()
