@@ -335,7 +335,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
     if (raised > m) raise_to(raised);
     add_pair(pack2(raised, V::kLow), pack2(-c, -c), s2, u2);
     if (raised == V::kLow) s2 = u2 = 0;  // what a masked value and the filler would count for beside nothing else
-    if (n > 0 && v > -CUDART_INF_F) push(entry_of(v, (uint32_t)i));
+    if (n > 0 && v > V::kLow) push(entry_of(v, (uint32_t)i));  // lower ones below, with those of the body
   }
   const float above_low = __int_as_float(__float_as_int(V::kLow) - 1);  // the next number; raised values are not noted
   float floor_v = above_low;
@@ -442,6 +442,11 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
       if (low) __syncthreads();
       if (low && count < n) {  // finite values from kLow down, if there are any
         for (int i = head + v0 * N + tid; i < head + v1 * N; i += THREADS) {
+          const float x = widen_one(l[i]);
+          if (x > -CUDART_INF_F && x <= V::kLow) push(entry_of(x, (uint32_t)i));
+        }
+        if (rank == 0 && tid < head + a.V - tail0) {
+          const int i = tid < head ? tid : tail0 + tid - head;
           const float x = widen_one(l[i]);
           if (x > -CUDART_INF_F && x <= V::kLow) push(entry_of(x, (uint32_t)i));
         }

@@ -13,7 +13,7 @@
 //
 // Which expert is chosen must not depend on float32 rounding. Without a bias experts are ranked by their logits (scores are
 // monotonic in them). Choices with a bias and sums of two are ranked in float32, and a row in which two neighbours of a
-// ranking lie closer than the error bound of those numbers is ranked again in 64 bits (a few rows in a thousand).
+// ranking lie closer than the error bound of those numbers is ranked again in 64 bits (about one row in a thousand).
 #pragma once
 #include <math_constants.h>
 

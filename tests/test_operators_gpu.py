@@ -412,6 +412,21 @@ def test_logprobs_every_number_of_alternatives(lib, T, V, n):
         check_logprobs(logits.to(BF16), torch.randint(0, V, (T,), generator=g, device="cuda"), n)
 
 
+@pytest.mark.parametrize("V", [5, 14, 33, 250, 5003, 70001])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_logprobs_lowest_values_as_alternatives(lib, V, dtype):
+    """Fewer ordinary logits than alternatives: the lowest finite values take the remaining places, lower ids first, wherever the
+    16-byte boundaries of a row lie."""
+    g = gen(V)
+    n = min(V, 20)
+    for ordinary in (0, 1, n - 1):
+        logits = torch.full((9, V), torch.finfo(dtype).min, device="cuda")
+        for t in range(9):
+            logits[t, torch.randperm(V, generator=g, device="cuda")[:ordinary]] = randn(g, ordinary)
+        logits[4:, ::3] = -INF
+        check_logprobs(logits.to(dtype), torch.zeros(9, dtype=torch.long, device="cuda"), n)
+
+
 def test_logprobs_strided_rows_off_boundaries(lib):
     g = gen(4)
     wide = 2 * randn(g, 11, 9100)
