@@ -636,8 +636,8 @@ cudaError_t launch_plain_tiles(const LinearCall& a, cudaStream_t s) {
 // Rows off 16-byte boundaries (ALIGNED = false): a lane's eight values are shifted out of two aligned words; their registers leave
 // room for one step per warp, more warps make up for it. 1 x 3001 -> 4001 8.6 us, 7 x 1628 -> 80637 60 us = 4.4 TB/s, where
 // tiles through shared memory took 28 and 90.
-// Bound by the weights' way from HBM, once a launch has started: 8 x 3584 -> 4608 (33 MB) takes 7.4 us, of which 5.0 are the
-// bytes at the measured copy rate. The tensor-core kernel needs 3 us more for its setup, the joining of partial sums and the
+// Bound by the weights' way from HBM, once a launch has started: 8 x 3584 -> 4608 (33 MB) takes 6.2 us in a chain of products, of
+// which 5.0 are the bytes at the measured copy rate. The tensor-core kernel needs 3 us more for its setup, the joining of partial sums and the
 // longer way of the operands.
 
 __device__ __forceinline__ uint4 load_once(const void* p) {
@@ -666,6 +666,8 @@ __global__ void __launch_bounds__(WARPS * 32, (ALIGNED ? 16 : 24) / WARPS) linea
   __shared__ float part[WARPS][MT * 8][16 * RT + 4];  // the lanes of a store meet different banks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16 * RT, steps = a.K / 64;
+  if (ALIGNED && threadIdx.x < 16 * RT && n0 + (int)threadIdx.x < a.N && a.ahead > 0)
+    prefetch_to_l2(static_cast<const T*>(a.w) + (int64_t)(n0 + (int)threadIdx.x) * a.ldw, (uint32_t)a.ahead);
   let_successor_start();
   wait_for_predecessor();
   const T *w[2 * RT], *x[MT];  // rows beyond the last are the last again, their sums are not used
@@ -789,6 +791,12 @@ __global__ void __launch_bounds__(WARPS * 32, (ALIGNED ? 16 : 24) / WARPS) linea
     static_cast<OT*>(a.y)[(int64_t)m * a.ldy + n] = from_float<OT>(v);
   }
 }
+
+// What an SM's blocks ask L2 for before they wait for the kernel in front of them, where all blocks are resident at once: the fetch
+// overlaps that kernel's end. Cold weights in a chain of products, 0 / 64 / 128 / 192 KB: 8 x 3584 -> 4608 7.39 / 6.56 / 6.22 / 6.56 us, 1 x
+// 4096 -> 4096 7.6 / 6.7 / 6.3 / 6.2, 1 x 2048 -> 512 3.1 / 2.5 / 2.5 / 2.5, 1 x 14336 -> 4096 20.4 / 19.2 / 18.4 / 17.4. With more blocks than fit
+// it takes bandwidth from the rows that are being read (8 x 7168 -> 18432 42.0 -> 44.2). (The tensor-core kernel gained nothing.)
+constexpr int kAheadBytes = 131072;
 
 // Which of them a product of M tokens takes, none (false) for the tensor-core kernel. All blocks should be resident at once, 16
 // warps per SM; 32 weight rows a block halve the fetches of x, but only for one tile of tokens have they the registers.
@@ -987,7 +995,10 @@ int launch_linear(const LinearCall& a, cudaStream_t s) {
   }
   FewShape few;
   if (few_shape(a.M, a.N, cap[1], few)) {
-    PM_CUDA(a.type == PM_BF16 ? launch_few<__nv_bfloat16>(a, few, s) : launch_few<__half>(a, few, s));
+    LinearCall c = a;
+    const int blocks = (a.N + few.rows - 1) / few.rows, per_sm = 16 / few.warps;
+    if (blocks <= per_sm * cap[1]) c.ahead = std::min(std::min(a.K, kAheadBytes) / 8 * 16, kAheadBytes / (per_sm * few.rows) & ~15);
+    PM_CUDA(a.type == PM_BF16 ? launch_few<__nv_bfloat16>(c, few, s) : launch_few<__half>(c, few, s));
     return PM_OK;
   }
   // The shape follows from the sizes alone; a thread remembers the last few.

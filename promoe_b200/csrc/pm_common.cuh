@@ -324,6 +324,7 @@ struct LinearCall {
   int64_t ldx, ldw, ldr, ldy;
   int32_t M, N, K, type, out_type, bias_type, act;
   int32_t* err;
+  int32_t ahead;  // the launcher's: bytes of a weight row to ask for ahead
 };
 int launch_linear(const LinearCall& a, cudaStream_t s);
 

@@ -116,6 +116,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
+// Asks for data to come to L2 (16-byte boundaries and multiples): a hint that reads nothing, so it may precede the wait for a
+// predecessor that writes there.
+__device__ __forceinline__ void prefetch_to_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 // TMA: global (tensor map) -> this CTA's shared memory, completion counted in bytes on `bar`, a cluster
 // address that may lie in either CTA of the pair. No multicast.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {

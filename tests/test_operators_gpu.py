@@ -301,6 +301,28 @@ def test_linear_infinities_and_nan_stay_in_their_rows_and_columns(lib):
     assert torch.equal(torch.isnan(r), torch.isnan(ref))
 
 
+@pytest.mark.parametrize("M", [1, 12, 40])
+def test_linear_weights_written_by_the_kernel_before(lib, M):
+    """A call may begin before its predecessor in the stream ends; it reads weights and tokens only after that."""
+    g = gen(M)
+    K, N = 2048, 2304
+    x = randn(g, M, K).to(BF16)
+    w = torch.zeros((N, K), dtype=BF16, device="cuda")
+    lin, new = ops.Linear(w, out_dtype=F32), [randn(g, N, K).to(BF16) for _ in range(6)]
+    want = [x.double() @ n.double().T for n in new]
+    got = []
+    for n in new:
+        w.copy_(n)
+        got.append(lin(x))
+    for a, b in zip(got, want):
+        assert float((a.double() - b).norm()) <= 1.6e-6 * float(b.norm())
+    # and tokens written by a product itself
+    up, down = ops.Linear(new[0][:K].contiguous()), ops.Linear(new[1][:K].contiguous())
+    h = up(x)
+    y = down(h)
+    assert float((y.double() - h.double() @ new[1][:K].double().T).norm()) <= 2.0 ** -8 * float(y.double().norm())
+
+
 @pytest.mark.parametrize("M", [1, 12, 40, 300])
 @pytest.mark.parametrize("K", [4160, 4099])
 def test_linear_float32_results_keep_their_precision(lib, M, K):
