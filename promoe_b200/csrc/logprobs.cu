@@ -441,9 +441,21 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
       count = sh.count;
       if (low) __syncthreads();
       if (low && count < n) {  // finite values from kLow down, if there are any
-        for (int i = head + v0 * N + tid; i < head + v1 * N; i += THREADS) {
-          const float x = widen_one(l[i]);
-          if (x > -CUDART_INF_F && x <= V::kLow) push(entry_of(x, (uint32_t)i));
+        for (int v = v0 + tid; v < v1; v += 4 * THREADS) {
+          uint4 w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (v + k * THREADS < v1) w[k] = body[v + k * THREADS];
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            if (v + k * THREADS >= v1) break;
+            const uint4 x4 = k == 0 ? w[0] : k == 1 ? w[1] : k == 2 ? w[2] : w[3];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              const float x = widen_one(reinterpret_cast<const T*>(&x4)[j]);
+              if (x > -CUDART_INF_F && x <= V::kLow) push(entry_of(x, (uint32_t)(head + (v + k * THREADS) * N + j)));
+            }
+          }
         }
         if (rank == 0 && tid < head + a.V - tail0) {
           const int i = tid < head ? tid : tail0 + tid - head;
@@ -536,7 +548,12 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   __syncthreads();
 
   Sums t = sh.part;
-  const bool again = !(t.m > V::kLow + kFar) || t.m > 1e37f;
+  bool again = !(t.m > V::kLow + kFar) || t.m > 1e37f;
+  // Neither NaN nor anything above -inf: no distribution, without a second look (33 x 50001 with one such row: 9.5 -> 6.0 us).
+  if (again && n > 0 && sh.best[0] == 0 && t.m == V::kLow && t.s == t.s) {
+    again = false;
+    t.s = 0.f;
+  }
   if (again) {
     // A row of the type's lowest values, or one so large that c overflows: its true maximum, and everything relative to it
     auto whole_row = [&](auto f) {
