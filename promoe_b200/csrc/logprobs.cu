@@ -1,7 +1,8 @@
 // Log probability of a given token, entropy and the best alternatives of every row of vocabulary logits, in one pass:
-//   M = max l, S = sum 2^(l log2e - c), U = sum 2^(l log2e - c) (l log2e - c), c = M log2e rounded
-//   lse = c ln2 + ln S,  logp = l_target - lse,  H = ln S - ln2 U / S,  top: l - lse of the n largest
-// c is rounded once and used everywhere, so its rounding cancels; two logits cost two exponentials and three packed
+//   M = max l, S = sum 2^(l k - c), U = sum 2^(l k - c) (l k - c), k = log2 e and c = M k, both rounded
+//   lse = c / k + ln S,  logp = l_target - lse,  H = ln S - ln2 U / S,  top: l - lse of the n largest
+// c is rounded once and used everywhere, so its rounding cancels. k's does where c is divided by the same k (times ln 2 it was
+// off by 1.3e-8 M); in the terms it leaves 1.3e-8 of (l - M). Two logits cost two exponentials and three packed
 // float32 instructions besides the widening and the maximum. Logits are raised to a value that has no probability beside any
 // other (kLow), which keeps 0 times infinity out of U; rows whose maximum is down there are summed again. (Raising only
 // once a thread has met a masked logit changed nothing.)
@@ -48,7 +49,8 @@ constexpr int kCap = 1024;  // room in the lists
 constexpr int kMaxTop = 32;
 constexpr int kMaxParts = 8;  // CTAs of a row
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr double kLn2 = 0.69314718055994531;
+constexpr double kPerC = 1.0 / (double)kLog2e;
+constexpr float kLn2 = 0.69314718f;
 constexpr int kUnroll = 4;  // 16-byte vectors per thread and batch
 
 using Entry = unsigned long long;  // ordered value above the reversed index
@@ -609,12 +611,12 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   if (warp != 0) return;
   const bool dead = !(t.s > 0.f) || !(fabsf(t.m) < CUDART_INF_F);
   const float log_s = logf(t.s);
-  const double lse = dead ? CUDART_NAN : (again ? (double)t.m : (double)t.c * kLn2) + (double)log_s;
+  const double lse = dead ? CUDART_NAN : (again ? (double)t.m : (double)t.c * kPerC) + (double)log_s;
   if (lane == 0) {
     if (a.logp != nullptr) {
       a.logp[row] = target < 0 ? 0.f : dead || target >= a.V ? CUDART_NAN_F : (float)((double)widen_one(at_target) - lse);
     }
-    if (a.entropy != nullptr) a.entropy[row] = dead ? CUDART_NAN_F : fmaf(-(float)kLn2, t.u / t.s, log_s);
+    if (a.entropy != nullptr) a.entropy[row] = dead ? CUDART_NAN_F : fmaf(-kLn2, t.u / t.s, log_s);
   }
   if (lane < n) {
     const Entry e = dead ? 0 : sh.best[lane];
