@@ -101,6 +101,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // register of it. raise(): all values at least kLow, NaN kept. top(): the larger (NaN ignored). pair(i): values 2i, 2i + 1. first(): the
 // lowest value of a 64-bit word.
 constexpr float kFar = 300.f;
+// Maxima whose c is off by at most 4, half a step of 1e8 log2 e: its rounding stays among the exponents that the sums can hold.
+// (Of 1e10 it is off by up to 512; from about 1e33 on the sums' rescaling meets infinity.) Rows beyond are summed again.
+constexpr float kPlain = 1e8f;
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int kN = 4;
@@ -550,14 +553,14 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   __syncthreads();
 
   Sums t = sh.part;
-  bool again = !(t.m > V::kLow + kFar) || t.m > 1e37f;
+  bool again = !(t.m > fmaxf(V::kLow + kFar, -kPlain)) || t.m > kPlain;
   // Neither NaN nor anything above -inf: no distribution, without a second look (33 x 50001 with one such row: 9.5 -> 6.0 us).
   if (again && n > 0 && sh.best[0] == 0 && t.m == V::kLow && t.s == t.s) {
     again = false;
     t.s = 0.f;
   }
   if (again) {
-    // A row of the type's lowest values, or one so large that c overflows: its true maximum, and everything relative to it
+    // A row of the type's lowest values, or of a size at which c is too coarse: its true maximum, and everything relative to it
     auto whole_row = [&](auto f) {
       if (tid < head + a.V - tail0) f(widen_one(l[tid < head ? tid : tail0 + tid - head]));
       for (int v = tid; v < n_vec; v += 4 * THREADS) {

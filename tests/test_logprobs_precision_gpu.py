@@ -43,3 +43,34 @@ def test_one_allowed_token_is_certain(lib, V, dtype):
     assert ids.flatten().tolist() == [V // 2] * len(levels)
     for r in (logp, entropy, best):
         assert float(r.abs().max()) <= 2.0 ** -21, r.tolist()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [9, 5000, 131072])
+@pytest.mark.parametrize("rest", [0.0, -INF])
+def test_one_logit_far_above_the_others(lib, V, dtype, rest):
+    """Certain, whatever its size: log probability and entropy 0."""
+    levels = torch.tensor([9e7, 1.1e8, 2e9, 1e10, 3e15, 1e20, 1e33, 1e34, 1e35, 9e36, 1.1e37, 3e38], device="cuda").to(dtype)
+    logits = torch.full((len(levels), V), rest, dtype=dtype, device="cuda")
+    logits[:, V - 2] = levels
+    targets = torch.full((len(levels),), V - 2, dtype=torch.int64, device="cuda")
+    logp, entropy, ids, best = ops.token_logprobs(logits, targets, 2)
+    assert ids[:, 0].tolist() == [V - 2] * len(levels)
+    for r in (logp, entropy, best[:, 0]):
+        assert float(r.abs().max()) <= 2.0 ** -21, r.tolist()
+
+
+@pytest.mark.parametrize("V", [33, 4099, 131072])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_large_logits_a_few_steps_apart(lib, V, sign):
+    """Rows around a size at which neighbouring float32 numbers differ by 1/16 to thousands."""
+    g = gen(V)
+    sizes = [1e6, 9e6, 9e7, 1.1e8, 5e8, 2e9, 1e10, 1e12, 1e18, 1e19, 1e25]
+    logits = torch.stack([sign * (s + float(2.0 ** -23 * 2.0 ** int(torch.tensor(s).log2().floor())) *
+                                  torch.randint(0, 3, (V,), generator=g, device="cuda").float()) for s in sizes])
+    targets = torch.randint(0, V, (len(sizes),), generator=g, device="cuda")
+    got, want = ops.token_logprobs(logits, targets, 4), logprob_oracle(logits, targets, 4)
+    assert torch.equal(got[2], want[2])
+    for i in (0, 3):
+        assert bool(((got[i].double() - want[i]).abs() <= tolerance(V, want[i].abs())).all()), i
+    assert bool(((got[1].double() - want[1]).abs() <= 20 * tolerance(V, want[1].abs())).all())
