@@ -358,7 +358,7 @@ int pm_k_ep_pack(const void* x, int hidden, const int32_t* counts, const int32_t
                  void* send, int32_t* pos_reply, void* stream);
 int pm_k_ep_unpack(const void* recv, int hidden, int n_ranks, int n_local, int max_block, int cap, int n_pred,
                    int num_expert, int32_t* row_expert, float* scores_sum, int32_t* err_flag, void* stream);
-/* pos = -1: no expert there; its weight is 0 (or NaN, which the token's row then takes over). */
+/* pos = -1: no expert there; its weight does not count, whatever it is, but for a NaN, which the token's row takes over. */
 int pm_k_combine(const float* yexp, const int32_t* pos, const float* topk_w, int T, int H, int k, int R,
                  int n_shared, const float* shared_scale, void* y, void* stream);
 /* scores[e] = sum_b (W2 relu(W1 x_b + b1) + b2)[e]; hidden_scratch is f32 [B, d] device scratch. */

@@ -47,7 +47,7 @@ combine_kernel(const float* __restrict__ yexp, const int32_t* __restrict__ pos,
 #pragma unroll 1
       for (int j = 0; j < k; ++j) {
         if (p_s[j] >= 0) add(j);
-        else if (w_s[j] != 0.f) acc.x = acc.y = acc.z = acc.w = w_s[j];  // NaN, where the token has no routing at all
+        else if (w_s[j] != w_s[j]) acc.x = acc.y = acc.z = acc.w = w_s[j];  // NaN: the token has no routing at all
       }
     }
     for (int s = 0; s < n_shared; ++s) {
