@@ -30,8 +30,9 @@ def _bf16_dev(t: torch.Tensor, device) -> torch.Tensor:
 def describe_router(block: torch.nn.Module, config=None) -> dict | None:
     """Arguments of the promoe_b200.ops.Router that the block's routing needs, besides num_expert, top_k, norm_topk and
     routed_scale; None for softmax with greedy top-k. Blocks whose gate carries a correction bias (`e_score_correction_bias`)
-    rank sigmoid scores + bias and value groups by their two best; `topk_method="group_limited_greedy"` ranks softmax
-    probabilities and values groups by their best."""
+    rank scores + bias and value groups by their two best; `topk_method="group_limited_greedy"` values groups by their best.
+    Scores are what `scoring_func` of the gate, the block or the configuration says, softmax or sigmoid; without it sigmoid where
+    there is a correction bias and softmax elsewhere."""
     gate = block.gate
     cfg = config if config is not None else getattr(block, "config", None)
 
@@ -47,13 +48,15 @@ def describe_router(block: torch.nn.Module, config=None) -> dict | None:
         groups["topk_group"] = 1
     bias = getattr(gate, "e_score_correction_bias", None)
     method = getattr(gate, "topk_method", getattr(block, "topk_method", None))
+    scoring = attr("scoring_func") or ("softmax" if bias is None else "sigmoid")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"the router scores by softmax or sigmoid; this block uses {scoring!r}")
     if bias is not None and method in (None, "noaux_tc"):
-        scoring = getattr(gate, "scoring_func", getattr(block, "scoring_func", "sigmoid"))
         return dict(scoring=scoring, bias=bias, group_score="top2", **groups)
     if method == "group_limited_greedy":
-        return dict(scoring="softmax", group_score="max", **groups)
+        return dict(scoring=scoring, group_score="max", **groups)
     if method in (None, "greedy"):
-        return None
+        return None if scoring == "softmax" else dict(scoring=scoring)
     raise ValueError(f"the router selects greedily, by groups or with a correction bias; this block uses {method!r}")
 
 
