@@ -22,7 +22,7 @@ import torch
 
 from . import ops
 from .engine import ExpertCache
-from .moe_block import describe_router, set_router
+from .moe_block import confirm_router, describe_router, set_router
 
 
 def find_moe_blocks(model: torch.nn.Module) -> list[tuple[str, torch.nn.Module]]:
@@ -47,10 +47,12 @@ def _describe(block) -> dict:
         norm = True
     else:
         norm = bool(getattr(gate, "norm_topk_prob", getattr(block, "norm_topk_prob", False)))
-    return dict(router=describe_router(block), E=E, H=H, I=two_i // 2, top_k=int(top_k), norm_topk=norm,
-                routed_scale=float(getattr(block, "routed_scaling_factor", 1.0) or 1.0),
-                shared=getattr(block, "shared_expert", None) or getattr(block, "shared_experts", None),
-                shared_gate=getattr(block, "shared_expert_gate", None))
+    d = dict(router=describe_router(block), E=E, H=H, I=two_i // 2, top_k=int(top_k), norm_topk=norm,
+             routed_scale=float(getattr(block, "routed_scaling_factor", 1.0) or 1.0),
+             shared=getattr(block, "shared_expert", None) or getattr(block, "shared_experts", None),
+             shared_gate=getattr(block, "shared_expert_gate", None))
+    confirm_router(block, d, gate.weight)
+    return d
 
 
 def inject_hf_fused_model(model: torch.nn.Module, cache_rate: float = 0.375, cache_policy: str = "lru",
@@ -61,22 +63,20 @@ def inject_hf_fused_model(model: torch.nn.Module, cache_rate: float = 0.375, cac
     blocks = find_moe_blocks(model)
     if not blocks:
         raise ValueError("no MoE block with fused expert tensors found")
-    d0 = _describe(blocks[0][1])
+    descs = [_describe(block) for _, block in blocks]  # what is refused is refused before anything is moved
+    d0 = descs[0]
     model_id = getattr(getattr(model, "config", None), "_name_or_path", "") or type(model).__name__
     cache = ExpertCache(len(blocks), d0["E"], num_expert_per_token=d0["top_k"], cache_rate=repr(float(cache_rate)),
                         cache_policy=cache_policy, num_predict_expert_per_layer=num_predict_expert_per_layer,
                         model_arch_string=model_id, **config)
     cache.set_param_list(["gate_proj.weight", "up_proj.weight", "down_proj.weight"])
-    descs = []
-    for layer, (name, block) in enumerate(blocks):
-        d = _describe(block)
+    for layer, ((name, block), d) in enumerate(zip(blocks, descs)):
         if (d["E"], d["H"], d["I"], d["top_k"]) != (d0["E"], d0["H"], d0["I"], d0["top_k"]):
             raise ValueError(f"MoE block {name} has a different shape than the first one")
         gu = block.experts.gate_up_proj.detach().to("cpu", torch.bfloat16)
         dn = block.experts.down_proj.detach().to("cpu", torch.bfloat16)
         for e in range(d["E"]):
             cache.register_expert(layer, e, [gu[e, : d["I"]].contiguous(), gu[e, d["I"]:].contiguous(), dn[e].contiguous()])
-        descs.append(d)
     cache.pin_all()
     cache.build_slab()
     dev = torch.device(device)

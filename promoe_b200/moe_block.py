@@ -55,9 +55,138 @@ def describe_router(block: torch.nn.Module, config=None) -> dict | None:
         return dict(scoring=scoring, bias=bias, group_score="top2", **groups)
     if method == "group_limited_greedy":
         return dict(scoring=scoring, group_score="max", **groups)
+    if method is None and groups["n_group"] > groups["topk_group"]:
+        raise ValueError("the block has groups of experts, but does not say how they are valued")
     if method in (None, "greedy"):
         return None if scoring == "softmax" else dict(scoring=scoring)
     raise ValueError(f"the router selects greedily, by groups or with a correction bias; this block uses {method!r}")
+
+
+class _NoExpert(torch.nn.Module):
+    """Stands in for what a block computes besides its routed experts."""
+
+    def forward(self, x, *args, **kwargs):
+        return torch.zeros_like(x)
+
+
+class _Expert(torch.nn.Module):
+    """Stands in for expert e: a one in column e, so that a block's output shows the expert's weight there."""
+
+    def __init__(self, e: int):
+        super().__init__()
+        self.e = e
+
+    def forward(self, x, *args, **kwargs):
+        y = torch.zeros_like(x)
+        y[..., self.e] = 1
+        return y
+
+
+class _Experts(torch.nn.Module):
+    """The same for all experts in one module, which is given hidden rows, ids and weights."""
+
+    def __init__(self, num_expert: int):
+        super().__init__()
+        self.num_expert, self.weights = num_expert, None
+
+    def forward(self, x, *args, **kwargs):
+        given = [t for t in (*args, *kwargs.values()) if torch.is_tensor(t) and t.dim() == 2]
+        ids = next(t for t in given if not t.is_floating_point())
+        w = next(t for t in given if t.is_floating_point() and t.shape == ids.shape)
+        self.weights = torch.zeros(ids.shape[0], self.num_expert, dtype=w.dtype).scatter_add_(1, ids.long(), w)
+        return torch.zeros_like(x)
+
+
+def _bare(m: torch.nn.Module, instead: dict) -> torch.nn.Module:
+    """A float32 copy of m on the CPU, in eval mode, without hooks and forwards of its instances; instead[id(child)] takes a
+    child's place."""
+    if id(m) in instead:
+        return instead[id(m)]
+    b = object.__new__(type(m))
+    b.__dict__.update({k: type(v)() if "hooks" in k and isinstance(v, dict) else v for k, v in vars(m).items() if k != "forward"})
+    if "report_experts" in vars(b):  # what tells the cache of a block's experts
+        b.__dict__["report_experts"] = lambda ids: ids
+    plain = lambda t: t.detach().to("cpu", torch.float32 if t.is_floating_point() else t.dtype, copy=True)  # noqa: E731
+    b.__dict__["_parameters"] = {n: None if t is None else torch.nn.Parameter(plain(t), requires_grad=False) for n, t in m._parameters.items()}
+    b.__dict__["_buffers"] = {n: None if t is None else plain(t) for n, t in m._buffers.items()}
+    b.__dict__["_modules"] = {n: None if c is None else _bare(c, instead) for n, c in m._modules.items()}
+    b.__dict__["training"] = False
+    return b
+
+
+def _observe(block: torch.nn.Module, gate_w: torch.Tensor):
+    """Routes some tokens through a copy of the block with random numbers in its gate: (logits [T, E] float64,
+    the weight of every expert [T, E], the copy). None where the block cannot be run like that."""
+    E, H = gate_w.shape
+    try:
+        experts = block.experts
+        one_each = isinstance(experts, torch.nn.ModuleList)
+        if one_each and E > H:
+            return None
+        instead = {id(c): _NoExpert() for c in block.children() if c is not block.gate and c is not experts}
+        if one_each:
+            instead.update({id(c): _Expert(e) for e, c in enumerate(experts)})
+        else:
+            instead[id(experts)] = _Experts(E)
+        probe = _bare(block, instead)
+        rng = torch.Generator().manual_seed(0)
+        T = 64
+        x = torch.randn(1, T, H, generator=rng)
+        with torch.no_grad():
+            for owner, deep in ((probe.gate, True), (probe, False)):
+                for t in (*owner.parameters(deep), *owner.buffers(deep)):
+                    if t.is_floating_point():  # corrections of the choice are positive here
+                        t.copy_(torch.randn(t.shape, generator=rng) * 2 / H ** 0.5 if t.dim() == 2 else
+                                0.1 + 0.5 * torch.rand(t.shape, generator=rng))
+            y = probe(x)
+        y = y[0] if isinstance(y, tuple) else y
+        seen = y.reshape(T, H)[:, :E] if one_each else probe.experts.weights
+        return x[0].double() @ probe.gate.weight.double().T, seen.double(), probe
+    except Exception:  # noqa: BLE001 - whatever a block of unknown make says to being run here
+        return None
+
+
+def _weights_by_rule(logits: torch.Tensor, d: dict, bias: torch.Tensor | None) -> torch.Tensor:
+    """The weight of every expert [T, E] as the layer will choose them, in 64 bits (logits float64)."""
+    r = d["router"] or {}
+    T, E = logits.shape
+    s = torch.sigmoid(logits) if r.get("scoring") == "sigmoid" else torch.softmax(logits, 1)
+    c = s if bias is None else s + bias.double()
+    G, kept = r.get("n_group", 1), r.get("topk_group", 1)
+    if G > kept:
+        groups = c.view(T, G, E // G)
+        best = groups.topk(2 if r.get("group_score") == "top2" and E // G > 1 else 1, 2).values.sum(2)
+        out = torch.ones(T, G, dtype=torch.bool).scatter_(1, best.topk(kept, 1).indices, False)
+        c = groups.masked_fill(out[..., None], -float("inf")).view(T, E)
+    ids = c.topk(d["top_k"], 1).indices
+    w = s.gather(1, ids)
+    if d["norm_topk"]:
+        w = w / (w.sum(1, keepdim=True) + 1e-20)
+    return torch.zeros_like(s).scatter_(1, ids, w * d["routed_scale"])
+
+
+def confirm_router(block: torch.nn.Module, d: dict, gate_w: torch.Tensor) -> None:
+    """Compares the description with how a copy of the block routes. Blocks that renormalise their weights without an attribute
+    that says so, or the other way round, are followed (d["norm_topk"]); one that routes by another rule is refused (ValueError).
+    Of a block that cannot be run like that, a gate that holds more than the description knows is refused."""
+    what = f"{type(block).__name__} chooses or weighs its experts in a way that this library does not know"
+    seen = _observe(block, gate_w)
+    if seen is not None:
+        logits, weights, probe = seen
+        has_bias = d["router"] is not None and d["router"].get("bias") is not None
+        bias = probe.gate.e_score_correction_bias if has_bias else None
+        for norm in (d["norm_topk"], not d["norm_topk"]):
+            want = _weights_by_rule(logits, {**d, "norm_topk": norm}, bias)
+            same = ((weights - want).abs() <= 1e-4 * (weights.abs() + want.abs()) + 1e-6).all(1)
+            if float(same.double().mean()) >= 0.95:  # a few rows for choices that float32 rounds into another order
+                d["norm_topk"] = norm
+                return
+        raise ValueError(what)
+    known = {"weight", "e_score_correction_bias"} if d["router"] is not None else {"weight"}
+    held = {n for n, _ in (*block.gate.named_parameters(), *block.gate.named_buffers())}
+    held |= {n for n, _ in (*block.named_parameters(recurse=False), *block.named_buffers(recurse=False))}
+    if held - known:
+        raise ValueError(f"{what} ({', '.join(sorted(held - known))})")
 
 
 def set_router(cache, layer: int, d: dict, num_expert: int, device) -> None:
@@ -96,8 +225,10 @@ def describe_block(block: torch.nn.Module, config=None) -> dict:
     else:
         norm = bool(getattr(block, "norm_topk_prob", getattr(gate, "norm_topk_prob", getattr(cfg, "norm_topk_prob", False))))
     scale = float(getattr(block, "routed_scaling_factor", getattr(gate, "routed_scaling_factor", 1.0)) or 1.0)
-    return dict(gate_w=gate_w, inter=inter, top_k=int(top_k), norm_topk=norm, routed_scale=scale,
-                shared=shared, shared_gate=shared_gate, quant4=quant4, router=router)
+    d = dict(gate_w=gate_w, inter=inter, top_k=int(top_k), norm_topk=norm, routed_scale=scale,
+             shared=shared, shared_gate=shared_gate, quant4=quant4, router=router)
+    confirm_router(block, d, gate_w)
+    return d
 
 
 def install_fused_forward(block: torch.nn.Module, cache, layer_id: int, device="cuda", config=None,

@@ -4,7 +4,8 @@ import types
 import pytest
 import torch
 
-from promoe_b200.moe_block import describe_router
+from promoe_b200.hf_fused import _describe
+from promoe_b200.moe_block import describe_block, describe_router
 
 
 def block(config=None, bias=None, gate=None, **attrs):
@@ -64,3 +65,111 @@ def test_scores_beside_a_correction_bias(scoring):
 def test_other_rules_are_refused(attrs):
     with pytest.raises(ValueError):
         describe_router(block(**attrs))
+
+
+# ---- blocks of the installed transformers: routed as the class does, or refused ----------------------------------
+def installed(family, block_name, config_name, **config):
+    import importlib
+    m = importlib.import_module(f"transformers.models.{family}.modeling_{family}")
+    c = importlib.import_module(f"transformers.models.{family}.configuration_{family}")
+    b = getattr(m, block_name)(getattr(c, config_name)(hidden_size=64, num_attention_heads=4, num_key_value_heads=2, **config))
+    with torch.no_grad():
+        for p in b.parameters():
+            p.normal_(0, 0.1)
+    return b
+
+
+V3 = dict(moe_intermediate_size=32, n_routed_experts=16, num_experts_per_tok=4, n_group=4, topk_group=2, n_shared_experts=1, norm_topk_prob=True)
+
+
+@pytest.mark.parametrize("case,norm", [
+    (("deepseek_v3", "DeepseekV3MoE", "DeepseekV3Config", V3), True),
+    (("deepseek_v3", "DeepseekV3MoE", "DeepseekV3Config", V3 | dict(norm_topk_prob=False)), False),
+    (("glm4_moe", "Glm4MoeMoE", "Glm4MoeConfig", V3), True),
+    (("mixtral", "MixtralSparseMoeBlock", "MixtralConfig", dict(num_local_experts=8, num_experts_per_tok=2)), True),
+    (("qwen2_moe", "Qwen2MoeSparseMoeBlock", "Qwen2MoeConfig", dict(num_experts=16, num_experts_per_tok=4, norm_topk_prob=False)), False),
+    # no attribute says that these renormalise
+    (("qwen3_vl_moe", "Qwen3VLMoeTextSparseMoeBlock", "Qwen3VLMoeTextConfig", dict(num_experts=16, num_experts_per_tok=4)), True),
+    (("minimax", "MiniMaxSparseMoeBlock", "MiniMaxConfig", dict(num_local_experts=8, num_experts_per_tok=2)), True)],
+    ids=lambda v: v[1] + str(v[3].get("norm_topk_prob", "")) if isinstance(v, tuple) else None)
+def test_installed_blocks_are_described_as_they_route(case, norm):
+    family, name, config, kw = case
+    b = installed(family, name, config, **kw)
+    before = {k: v.clone() for k, v in b.state_dict().items()}
+    d = _describe(b)
+    assert d["norm_topk"] is norm and d["top_k"] == kw["num_experts_per_tok"]
+    assert all(torch.equal(v, before[k]) for k, v in b.state_dict().items()) and b.training
+
+
+@pytest.mark.parametrize("case", [
+    ("minimax_m2", "MiniMaxM2SparseMoeBlock", "MiniMaxM2Config", dict(num_local_experts=16, num_experts_per_tok=4)),
+    ("ernie4_5_moe", "Ernie4_5_MoeSparseMoeBlock", "Ernie4_5_MoeConfig", dict(moe_num_experts=16, moe_k=4)),
+    ("lfm2_moe", "Lfm2MoeSparseMoeBlock", "Lfm2MoeConfig", dict(num_experts=16, num_experts_per_tok=4))], ids=lambda c: c[1])
+def test_installed_blocks_that_route_by_other_rules_are_refused(case):
+    """Corrections held elsewhere than on the gate, or under another name."""
+    family, name, config, kw = case
+    with pytest.raises(ValueError, match=name):
+        _describe(installed(family, name, config, **kw))
+
+
+class OneByOne(torch.nn.Module):
+    """A block with a module for each expert, as transformers 4.x has them."""
+
+    def __init__(self, score, H=32, E=8, I=16, gate_bias=False):
+        super().__init__()
+        self.score, self.top_k, self.norm_topk_prob = score, 2, False
+        self.gate = torch.nn.Linear(H, E, bias=gate_bias)
+
+        class Expert(torch.nn.Module):
+            def __init__(self):
+                super().__init__()
+                self.gate_proj, self.up_proj, self.down_proj = (torch.nn.Linear(*s, bias=False) for s in ((H, I), (H, I), (I, H)))
+
+            def forward(self, x):
+                return self.down_proj(torch.nn.functional.silu(self.gate_proj(x)) * self.up_proj(x))
+        self.experts = torch.nn.ModuleList(Expert() for _ in range(E))
+        self.shared_expert = Expert()
+
+    def forward(self, hidden_states):
+        x = hidden_states.reshape(-1, hidden_states.shape[-1])
+        logits = self.gate(x)
+        w, ids = self.score(logits).topk(self.top_k, -1)
+        y = self.shared_expert(x)
+        for e, expert in enumerate(self.experts):
+            tok, slot = torch.where(ids == e)
+            y = y.index_add(0, tok, expert(x[tok]) * w[tok, slot, None])
+        return y.view(hidden_states.shape), logits
+
+
+def softmax(l):
+    return torch.softmax(l, -1)
+
+
+def test_blocks_with_a_module_for_each_expert():
+    assert describe_block(OneByOne(softmax))["norm_topk"] is False
+    for other in (OneByOne(torch.sigmoid), OneByOne(softmax, gate_bias=True), OneByOne(lambda l: torch.softmax(l, -1).square())):
+        with pytest.raises(ValueError, match="OneByOne"):
+            describe_block(other)
+
+
+def test_blocks_that_cannot_be_run_alone():
+    class Needs(OneByOne):
+        def forward(self, hidden_states, more):
+            raise AssertionError
+    assert describe_block(Needs(softmax))["router"] is None
+    with pytest.raises(ValueError, match="bias"):
+        describe_block(Needs(softmax, gate_bias=True))
+
+
+def test_describing_a_block_runs_none_of_its_hooks():
+    b = OneByOne(softmax)
+
+    def never(*args):
+        raise AssertionError
+    for m in (b, b.gate, b.experts[0]):
+        m.register_forward_hook(never)
+        m.register_forward_pre_hook(never)
+    b.gate.forward = never
+    assert describe_block(b)["router"] is None
+    with pytest.raises(ValueError):
+        describe_block(OneByOne(torch.sigmoid))
