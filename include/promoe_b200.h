@@ -380,7 +380,9 @@ int pm_k_rank_topn(const float* scores, int width, int n, int32_t* out, void* st
  *   score   softmax(l)_e, or 1 / (1 + exp(-l_e))
  *   choice  score + choice_bias[e]; an expert whose logit or choice is -inf cannot be chosen
  *   groups  of num_expert / n_group neighbouring experts, valued by their largest choice or by the sum of their two
- *           largest (a missing second counts as nothing); the topk_group best stay, ties to the lower group
+ *           largest (a missing second counts as nothing); the topk_group best stay, ties to the lower group. Experts of the others
+ *           cannot be chosen; with PM_GROUP_DROPPED_ZERO (routers with a choice_bias) their choice is 0 instead, so that they
+ *           pass by experts of the best groups whose choice is negative
  *   ids     the top_k largest choices among them, descending, ties to the lower id; -1 where there are fewer
  *   weight  the score (not the choice), with norm_topk divided by the sum of the selected ones + 1e-20, times routed_scale;
  *           0 for id -1
@@ -392,12 +394,13 @@ int pm_k_rank_topn(const float* scores, int width, int n, int32_t* out, void* st
 #define PM_SCORE_SIGMOID 1
 #define PM_GROUP_MAX 0
 #define PM_GROUP_TOP2 1
+#define PM_GROUP_DROPPED_ZERO 16 /* to be added to one of them */
 typedef struct pm_router {
   int32_t num_expert, top_k;
   int32_t scoring;          /* PM_SCORE_* */
   int32_t n_group;          /* 1 = no groups */
   int32_t topk_group;       /* groups that stay */
-  int32_t group_score;      /* PM_GROUP_* */
+  int32_t group_score;      /* PM_GROUP_MAX or PM_GROUP_TOP2, + PM_GROUP_DROPPED_ZERO */
   int32_t norm_topk;
   float routed_scale;
   const float* choice_bias; /* device f32 [num_expert] or NULL */

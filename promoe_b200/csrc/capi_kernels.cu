@@ -100,9 +100,10 @@ int router_rule(const pm_router* r, const char* who, RouteRule* rule) {
   const std::string name(who);
   if (!r) return fail(PM_ERR_INVALID, name + ": null router");
   if (r->scoring != PM_SCORE_SOFTMAX && r->scoring != PM_SCORE_SIGMOID) return fail(PM_ERR_INVALID, name + ": unknown scoring");
-  if (r->group_score != PM_GROUP_MAX && r->group_score != PM_GROUP_TOP2) return fail(PM_ERR_INVALID, name + ": unknown group_score");
+  const int value = r->group_score & ~PM_GROUP_DROPPED_ZERO;
+  if (value != PM_GROUP_MAX && value != PM_GROUP_TOP2) return fail(PM_ERR_INVALID, name + ": unknown group_score");
   *rule = RouteRule{r->num_expert, r->top_k, r->scoring == PM_SCORE_SIGMOID, r->n_group, r->topk_group,
-                    r->group_score == PM_GROUP_TOP2, r->norm_topk != 0, r->routed_scale, r->choice_bias};
+                    value == PM_GROUP_TOP2, r->group_score != value, r->norm_topk != 0, r->routed_scale, r->choice_bias};
   return check_route_rule(*rule, who);
 }
 

@@ -114,7 +114,7 @@ cudaError_t launch_behind(void (*kern)(P...), dim3 grid, dim3 block, size_t smem
 
 // How a router turns logits into experts (route_select.cuh). E = 0: softmax, greedy top-k.
 struct RouteRule {
-  int32_t E, k, sigmoid, n_group, topk_group, group_top2, norm;
+  int32_t E, k, sigmoid, n_group, topk_group, group_top2, drop_zero, norm;
   float scale;
   const float* bias;  // device [E] or nullptr
 };

@@ -90,7 +90,7 @@ cudaError_t launch(const T* logits, int64_t ld, int n_tok, const RouteRule& rule
   // 11.8, with groups 20.3 -> 18.8. Wider rows are too rare for that.
   auto kern = route_kernel<T, NPL, kAnyRule>;
   if constexpr (NPL <= 16) {
-    switch (route_kind(rule)) {
+    switch (rule.drop_zero ? (int)kAnyRule : route_kind(rule)) {
       case 0: kern = route_kernel<T, NPL, 0>; break;
       case kGrouped: kern = route_kernel<T, NPL, kGrouped>; break;
       case kSigmoid | kHasBias: kern = route_kernel<T, NPL, kSigmoid | kHasBias>; break;
@@ -122,6 +122,7 @@ int check_route_rule(const RouteRule& r, const char* who) {
   if (r.topk_group < 1 || r.topk_group > r.n_group) return fail(PM_ERR_INVALID, name + ": topk_group must be in [1, n_group]");
   if (r.k > r.topk_group * (r.E / r.n_group))
     return fail(PM_ERR_INVALID, name + ": topk_group groups hold fewer than top_k experts");
+  if (r.drop_zero && r.bias == nullptr) return fail(PM_ERR_INVALID, name + ": PM_GROUP_DROPPED_ZERO is for routers with a choice_bias");
   return PM_OK;
 }
 

@@ -6,7 +6,8 @@
 //   score   s_e = softmax(l)_e  or  1 / (1 + exp(-l_e))
 //   choice  c_e = s_e + b_e; an expert whose logit or choice is -inf cannot be chosen
 //   group   max of its choices, or the sum of its two largest (a missing second counts as nothing);
-//           the topk_group best groups stay, ties to the lower group
+//           the topk_group best groups stay, ties to the lower group; the others' experts leave, or (drop_zero) their
+//           choices become 0
 //   ids     the k largest choices among them, descending, ties to the lower id; -1 where there are fewer
 //   weight  s_id, divided by (sum of the k + 1e-20) if asked for, times the scale; 0 for id -1
 // A row that holds a NaN (softmax: or +inf) has no scores: its ids are -1 and its weights NaN.
@@ -82,9 +83,11 @@ static __device__ __noinline__ double exact_sum(const double* c, int E, double t
   return sum;
 }
 
-// Rank of each of the n <= 32 candidates, one per lane in the order of their ids, by a choice that `sum` (softmax) makes exact.
-static __device__ __noinline__ int exact_candidates(double logit, float bias, double top, double sum, int sigmoid, int n, int lane) {
-  const double v = (sigmoid ? 1.0 / (1.0 + exp(-logit)) : exp(logit - top) / sum) + (double)bias;
+// Rank of each of the n <= 32 candidates, one per lane in the order of their ids, by a choice that `sum` (softmax) makes exact; 0
+// for one of a dropped group.
+static __device__ __noinline__ int exact_candidates(double logit, float bias, double top, double sum, int sigmoid, bool dropped, int n,
+                                                    int lane) {
+  const double v = dropped ? 0.0 : (sigmoid ? 1.0 / (1.0 + exp(-logit)) : exp(logit - top) / sum) + (double)bias;
   int rank = 0;
   for (int i = 0; i < n; ++i) {
     const double o = __shfl_sync(0xffffffffu, v, i);
@@ -118,11 +121,11 @@ static __device__ __noinline__ uint32_t exact_groups(const double* c, const Rout
   return __ballot_sync(0xffffffffu, lane < rule->n_group && before < rule->topk_group && value > -CUDART_INF);
 }
 
-// Lane j < k returns the j-th of the experts in the groups `kept`, -1 if there are fewer. Uses c up.
+// Lane j < k returns the j-th of the experts in the groups `kept` (drop_zero: of all), -1 if there are fewer. Uses c up.
 static __device__ __noinline__ int exact_rank(double* c, const RouteRule* rule, uint32_t kept, int lane) {
   const int E = rule->E, per = E / rule->n_group;
   for (int e = lane; e < E; e += 32)
-    if (!((kept >> (e / per)) & 1u)) c[e] = -CUDART_INF;
+    if (!((kept >> (e / per)) & 1u)) c[e] = rule->drop_zero && c[e] > -CUDART_INF ? 0.0 : -CUDART_INF;
   int mine = -1;
   for (int j = 0; j < rule->k; ++j) {
     double best = -CUDART_INF;
@@ -197,6 +200,7 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   const int kind = KIND == kAnyRule ? route_kind(r) : KIND;
   const bool by_logit = !(kind & kHasBias), grouped = (kind & kGrouped) != 0, sigmoid = (kind & kSigmoid) != 0;
   const bool sums = grouped && r.group_top2 != 0;
+  const bool zero = KIND == kAnyRule && grouped && r.drop_zero != 0;  // the fixed kinds let the experts of dropped groups leave
   bool odd = false;
 #pragma unroll
   for (int j = 0; j < NPL; ++j) odd |= !(fabsf(l[j]) < CUDART_INF_F);
@@ -318,13 +322,13 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
     }
     if (aligned) {
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) c[j] = in ? c[j] : -CUDART_INF_F;
+      for (int j = 0; j < NPL; ++j) c[j] = in ? c[j] : zero && c[j] > -CUDART_INF_F ? 0.f : -CUDART_INF_F;
     } else {
       const uint32_t kept = kept_groups();
       int g = e0 / per, rem = e0 - g * per;
 #pragma unroll
       for (int j = 0; j < NPL; ++j) {
-        if (!((kept >> (g & 31)) & 1u)) c[j] = -CUDART_INF_F;
+        if (!((kept >> (g & 31)) & 1u)) c[j] = zero && c[j] > -CUDART_INF_F ? 0.f : -CUDART_INF_F;
         if (++rem == per) {
           rem = 0;
           ++g;
@@ -398,7 +402,8 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
           stage_logits();
           sum64 = exact_sum(work, E, (double)top, lane);
         }
-        rank = exact_candidates((double)v_id, lane < n ? r.bias[id] : 0.f, (double)top, sum64, sigmoid, n, lane);
+        const bool dropped = zero && lane < n && !((kept_groups() >> (id / groups.per)) & 1u);
+        rank = exact_candidates((double)v_id, lane < n ? r.bias[id] : 0.f, (double)top, sum64, sigmoid, dropped, n, lane);
       }
     }
   } else {

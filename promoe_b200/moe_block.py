@@ -135,9 +135,9 @@ def _observe(block: torch.nn.Module, gate_w: torch.Tensor):
         with torch.no_grad():
             for owner, deep in ((probe.gate, True), (probe, False)):
                 for t in (*owner.parameters(deep), *owner.buffers(deep)):
-                    if t.is_floating_point():  # corrections of the choice are positive here
+                    if t.is_floating_point():  # corrections leave some choices negative
                         t.copy_(torch.randn(t.shape, generator=rng) * 2 / H ** 0.5 if t.dim() == 2 else
-                                0.1 + 0.5 * torch.rand(t.shape, generator=rng))
+                                -0.3 - 0.7 * torch.rand(t.shape, generator=rng))
             y = probe(x)
         y = y[0] if isinstance(y, tuple) else y
         seen = y.reshape(T, H)[:, :E] if one_each else probe.experts.weights
@@ -157,7 +157,7 @@ def _weights_by_rule(logits: torch.Tensor, d: dict, bias: torch.Tensor | None) -
         groups = c.view(T, G, E // G)
         best = groups.topk(2 if r.get("group_score") == "top2" and E // G > 1 else 1, 2).values.sum(2)
         out = torch.ones(T, G, dtype=torch.bool).scatter_(1, best.topk(kept, 1).indices, False)
-        c = groups.masked_fill(out[..., None], -float("inf")).view(T, E)
+        c = groups.masked_fill(out[..., None], 0.0 if r.get("dropped") == "zero" else -float("inf")).view(T, E)
     ids = c.topk(d["top_k"], 1).indices
     w = s.gather(1, ids)
     if d["norm_topk"]:
@@ -167,19 +167,22 @@ def _weights_by_rule(logits: torch.Tensor, d: dict, bias: torch.Tensor | None) -
 
 def confirm_router(block: torch.nn.Module, d: dict, gate_w: torch.Tensor) -> None:
     """Compares the description with how a copy of the block routes. Blocks that renormalise their weights without an attribute
-    that says so, or the other way round, are followed (d["norm_topk"]); one that routes by another rule is refused (ValueError).
-    Of a block that cannot be run like that, a gate that holds more than the description knows is refused."""
+    that says so, or the other way round, are followed (d["norm_topk"]), and so are those that count the choices of dropped groups as 0
+    beside a correction bias (d["router"]["dropped"]); one that routes by another rule is refused (ValueError). Of a block that cannot be run like that, a gate that holds more than the description knows is refused."""
     what = f"{type(block).__name__} chooses or weighs its experts in a way that this library does not know"
     seen = _observe(block, gate_w)
     if seen is not None:
         logits, weights, probe = seen
         has_bias = d["router"] is not None and d["router"].get("bias") is not None
         bias = probe.gate.e_score_correction_bias if has_bias else None
-        for norm in (d["norm_topk"], not d["norm_topk"]):
-            want = _weights_by_rule(logits, {**d, "norm_topk": norm}, bias)
+        rules = [d["router"]]
+        if has_bias and d["router"]["n_group"] > d["router"]["topk_group"]:
+            rules.append({**d["router"], "dropped": "zero"})
+        for norm, rule in ((n, r) for n in (d["norm_topk"], not d["norm_topk"]) for r in rules):
+            want = _weights_by_rule(logits, {**d, "norm_topk": norm, "router": rule}, bias)
             same = ((weights - want).abs() <= 1e-4 * (weights.abs() + want.abs()) + 1e-6).all(1)
             if float(same.double().mean()) >= 0.95:  # a few rows for choices that float32 rounds into another order
-                d["norm_topk"] = norm
+                d["norm_topk"], d["router"] = norm, rule
                 return
         raise ValueError(what)
     known = {"weight", "e_score_correction_bias"} if d["router"] is not None else {"weight"}

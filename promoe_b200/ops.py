@@ -19,6 +19,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
+_DROPPED = {"out": 0, "zero": 16}
 
 
 # The stream as an integer, without the Stream object that torch.cuda.current_stream makes (1 us of a call that takes 5). A torch
@@ -61,20 +62,24 @@ class Router:
 
     scoring: "softmax" or "sigmoid". bias: [num_expert] float32 on the device, added to the scores for the choice only (a
     load-balancing correction). n_group / topk_group / group_score ("max" or "top2"): choose among the best groups
-    only. norm_topk: weights divided by their sum. routed_scale: multiplies the weights."""
+    only; dropped: what becomes of the others' experts, "out" (they cannot be chosen) or, with a bias, "zero" (their score + bias
+    counts as 0, which passes by negative ones). norm_topk: weights divided by their sum. routed_scale: multiplies the weights."""
 
     def __init__(self, num_expert: int, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
-                 topk_group: int = 1, group_score: str = "max", norm_topk: bool = False, routed_scale: float = 1.0):
+                 topk_group: int = 1, group_score: str = "max", norm_topk: bool = False, routed_scale: float = 1.0,
+                 dropped: str = "out"):
         if scoring not in _SCORING:
             raise ValueError(f"scoring must be one of {sorted(_SCORING)}")
         if group_score not in _GROUP_SCORE:
             raise ValueError(f"group_score must be one of {sorted(_GROUP_SCORE)}")
+        if dropped not in _DROPPED:
+            raise ValueError(f"dropped must be one of {sorted(_DROPPED)}")
         if bias is not None:
             if not bias.is_cuda or bias.dtype != torch.float32 or bias.shape != (num_expert,) or not bias.is_contiguous():
                 raise ValueError("bias must be a contiguous float32 CUDA tensor of shape [num_expert]")
         self.num_expert, self.top_k, self.bias = num_expert, top_k, bias
         self.device_index = None if bias is None else bias.get_device()
-        self.rule = _lib.pm_router(num_expert, top_k, _SCORING[scoring], n_group, topk_group, _GROUP_SCORE[group_score],
+        self.rule = _lib.pm_router(num_expert, top_k, _SCORING[scoring], n_group, topk_group, _GROUP_SCORE[group_score] + _DROPPED[dropped],
                                    int(norm_topk), routed_scale, None if bias is None else bias.data_ptr())
         self._ref = C.byref(self.rule)
         self._fn = _lib.load().pm_k_route

@@ -173,3 +173,35 @@ def test_describing_a_block_runs_none_of_its_hooks():
     assert describe_block(b)["router"] is None
     with pytest.raises(ValueError):
         describe_block(OneByOne(torch.sigmoid))
+
+
+@pytest.mark.parametrize("fill", [0.0, -float("inf")])
+@pytest.mark.parametrize("bias", [0.3, -0.9])
+def test_dropped_groups_are_treated_as_the_block_does(fill, bias):
+    """Whatever its present correction is: with a positive one there is no difference."""
+    b = installed("deepseek_v3", "DeepseekV3MoE", "DeepseekV3Config", **V3)
+    b.gate.e_score_correction_bias.fill_(bias)
+    if fill != 0.0:  # the installed class fills with 0
+        class Out(type(b)):
+            def route_tokens_to_experts(self, logits):
+                s = logits.sigmoid()
+                c = s + self.gate.e_score_correction_bias
+                best = c.view(-1, self.n_group, 4).topk(2, -1)[0].sum(-1).topk(self.topk_group, -1)[1]
+                keep = torch.zeros(len(c), self.n_group).scatter_(1, best, 1.0).repeat_interleave(4, 1).bool()
+                ids = c.masked_fill(~keep, fill).topk(self.top_k, -1)[1]
+                w = s.gather(1, ids)
+                return ids, w / (w.sum(-1, keepdim=True) + 1e-20) * self.routed_scaling_factor
+        b.__class__ = Out
+    assert _describe(b)["router"].get("dropped", "out") == ("zero" if fill == 0.0 else "out")
+
+
+def test_dropped_groups_as_zero_need_a_correction_bias(lib):
+    from promoe_b200 import _lib
+    from tests.test_operators_refusals import PTR, route
+    for value in (16, 17):
+        with pytest.raises(_lib.PromoeError):
+            route(group_score=value, n_group=4, topk_group=2)
+        route(group_score=value, n_group=4, topk_group=2, choice_bias=PTR)
+    for value in (18, 32, 48, -16):
+        with pytest.raises(_lib.PromoeError):
+            route(group_score=value, n_group=4, topk_group=2, choice_bias=PTR)
