@@ -15,8 +15,7 @@ worth to the model.
 """
 from __future__ import annotations
 
-import types
-import weakref
+import copy
 
 import torch
 
@@ -112,30 +111,9 @@ def _replace_forward(block, cache: ExpertCache, layer: int):
     block.forward = fused_forward
 
 
-# The products of replaced modules, with what they were made from. Beside the modules, so that a copied model makes its own.
-_PRODUCTS: "weakref.WeakKeyDictionary[torch.nn.Module, tuple]" = weakref.WeakKeyDictionary()
-
-
 def _usable(m) -> bool:
     return (isinstance(m, torch.nn.Linear) and m.weight.is_cuda and m.weight.dtype in (torch.bfloat16, torch.float16)
             and m.weight.dim() == 2 and (m.bias is None or m.bias.dtype == m.weight.dtype))
-
-
-def _product(owner: torch.nn.Module, m: torch.nn.Linear, x: torch.Tensor, activation: str | None = None):
-    """The library's product with m's weights as they are now, or None where m's own forward has to do: other types or
-    devices, or a gradient to record."""
-    w, b = m.weight, m.bias
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
-        return None
-    if x.dtype != w.dtype or x.device != w.device:
-        return None
-    key = (w.data_ptr(), w.dtype, w.shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
-    have = _PRODUCTS.get(owner)
-    if have is None or have[0] != key:
-        if not _usable(m):
-            return None
-        have = _PRODUCTS[owner] = (key, ops.Linear(w.detach(), None if b is None else b.detach(), activation))
-    return have[1]
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -144,20 +122,61 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
 
 
-def _linear_forward(self, x):
-    lin = _product(self, self, x)
-    if lin is None:
-        return type(self).forward(self, x)
-    return lin(_rows(x)).view(*x.shape[:-1], lin.N)
+class _Product:
+    """The library's product with a module's weights as they are now, kept while they stay where they are."""
+
+    def __init__(self, activation: str | None = None):
+        self.activation, self.key, self.made = activation, None, None
+
+    def of(self, m: torch.nn.Linear, x: torch.Tensor):
+        """None where m's own forward has to do: other types or devices, or a gradient to record."""
+        w, b = m.weight, m.bias
+        if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+            return None
+        if x.dtype != w.dtype or x.device != w.device:
+            return None
+        key = (w.data_ptr(), w.dtype, w.shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
+        if self.key != key:
+            if not _usable(m):
+                return None
+            self.key, self.made = key, ops.Linear(w.detach(), None if b is None else b.detach(), self.activation)
+        return self.made
 
 
-def _gated_forward(self, x):
-    learns = torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
-    gate = None if self.training or learns else _product(self, self.gate_proj, x, "silu")
-    if gate is None:
-        return type(self).forward(self, x)
-    rows = _rows(x)
-    return self.down_proj(gate(rows).mul_(self.up_proj(rows))).view(*x.shape[:-1], self.down_proj.out_features)
+class _Forward:
+    """The forward of a replaced module. A copied or unpickled module gets one of its own, which makes its own product."""
+
+    activation = None
+
+    def __init__(self, m: torch.nn.Module):
+        self.m, self.product = m, _Product(self.activation)
+
+    def __deepcopy__(self, memo):
+        return type(self)(copy.deepcopy(self.m, memo))
+
+    def __reduce__(self):
+        return type(self), (self.m,)
+
+
+class _LinearForward(_Forward):
+    def __call__(self, input):  # noqa: A002 - torch.nn.Linear's own name for it
+        lin = self.product.of(self.m, input)
+        if lin is None:
+            return type(self.m).forward(self.m, input)
+        return lin(_rows(input)).view(*input.shape[:-1], lin.N)
+
+
+class _GatedForward(_Forward):
+    activation = "silu"
+
+    def __call__(self, x):
+        m = self.m
+        learns = torch.is_grad_enabled() and any(p.requires_grad for p in m.parameters())
+        gate = None if m.training or learns else self.product.of(m.gate_proj, x)
+        if gate is None:
+            return type(m).forward(m, x)
+        rows = _rows(x)
+        return m.down_proj(gate(rows).mul_(m.up_proj(rows))).view(*x.shape[:-1], m.down_proj.out_features)
 
 
 def install_linears(model: torch.nn.Module) -> int:
@@ -172,9 +191,9 @@ def install_linears(model: torch.nn.Module) -> int:
     replaced = 0
     for m in list(model.modules()):
         if type(m) is torch.nn.Linear and _usable(m) and "forward" not in vars(m):
-            m.forward = types.MethodType(_linear_forward, m)
+            m.forward = _LinearForward(m)
             replaced += 1
-    mine = lambda m: getattr(vars(m).get("forward"), "__func__", None) is _linear_forward  # noqa: E731
+    mine = lambda m: isinstance(vars(m).get("forward"), _LinearForward)  # noqa: E731
     for m in list(model.modules()):
         parts = dict(m.named_children())
         act = type(parts.pop("act_fn", None)).__name__.lower()
@@ -186,11 +205,11 @@ def install_linears(model: torch.nn.Module) -> int:
             x = torch.randn(2, w.shape[1], generator=torch.Generator(w.device).manual_seed(0), device=w.device).to(w.dtype)
             modes = [(c, c.training) for c in m.modules()]
             m.eval()
-            own, fused = type(m).forward(m, x), _gated_forward(m, x)
+            own, fused = type(m).forward(m, x), _GatedForward(m)(x)
             for c, mode in modes:
                 c.training = mode
         if own.shape == fused.shape and float((own - fused).float().norm()) <= 0.02 * float(own.float().norm()):
-            m.forward = types.MethodType(_gated_forward, m)
+            m.forward = _GatedForward(m)
             replaced += 1
     return replaced
 
