@@ -166,17 +166,42 @@ class _LinearForward(_Forward):
         return lin(_rows(input)).view(*input.shape[:-1], lin.N)
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+_EVERYWHERE = [getattr(torch.nn.modules.module, "_global" + h) for h in _HOOKS]
+
+
+def _untouched(m: torch.nn.Module, kinds) -> bool:
+    """Whether calling m is what its class does and nothing else; a torch.nn.Linear's forward may be the installed one."""
+    own = vars(m)
+    forward = own.get("forward")
+    return (type(m) in kinds and not any(own[h] for h in _HOOKS) and not any(_EVERYWHERE)
+            and (forward is None or (isinstance(forward, _LinearForward) and forward.m is m)))
+
+
+def _silu(m: torch.nn.Module) -> bool:
+    kind = type(m)
+    return _untouched(m, (torch.nn.SiLU,) if kind.__name__ != "SiLUActivation" or not kind.__module__.startswith("transformers.") else (kind,))
+
+
 class _GatedForward(_Forward):
+    """Three products, SiLU in the first one's epilogue. gate_proj and act_fn are passed by, so only while there is nothing else to them
+    (hooks, adapters around them, another activation); the other two are called as ever."""
+
     activation = "silu"
 
     def __call__(self, x):
         m = self.m
+        gate_proj, act_fn = m._modules.get("gate_proj"), m._modules.get("act_fn")
         learns = torch.is_grad_enabled() and any(p.requires_grad for p in m.parameters())
-        gate = None if m.training or learns else self.product.of(m.gate_proj, x)
+        gate = None
+        if not (m.training or learns) and gate_proj is not None and act_fn is not None:
+            if _untouched(gate_proj, (torch.nn.Linear,)) and _silu(act_fn):
+                gate = self.product.of(gate_proj, x)
         if gate is None:
             return type(m).forward(m, x)
-        rows = _rows(x)
-        return m.down_proj(gate(rows).mul_(m.up_proj(rows))).view(*x.shape[:-1], m.down_proj.out_features)
+        up = m.up_proj(x)
+        y = gate(_rows(x)).view(*x.shape[:-1], gate.N)
+        return m.down_proj(y.mul_(up) if up.dtype == y.dtype and up.shape == y.shape else y * up)
 
 
 def install_linears(model: torch.nn.Module) -> int:
@@ -196,9 +221,9 @@ def install_linears(model: torch.nn.Module) -> int:
     mine = lambda m: isinstance(vars(m).get("forward"), _LinearForward)  # noqa: E731
     for m in list(model.modules()):
         parts = dict(m.named_children())
-        act = type(parts.pop("act_fn", None)).__name__.lower()
+        act = parts.pop("act_fn", None)
         if (sorted(parts) != ["down_proj", "gate_proj", "up_proj"] or not all(mine(p) for p in parts.values())
-                or act not in ("silu", "siluactivation") or "forward" in vars(m)):
+                or act is None or not _silu(act) or "forward" in vars(m)):
             continue
         with torch.no_grad():  # whether its forward is what the names say
             w = m.gate_proj.weight

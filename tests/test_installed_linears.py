@@ -80,3 +80,105 @@ def test_the_name_of_the_argument_stays(stand_in):
     m, own = installed(torch.nn.Linear(32, 48))
     x = torch.randn(5, 32).to(BF16)
     assert close(m(input=x), own(input=x))
+
+
+class Adapter(torch.nn.Module):
+    """A low-rank addition around a layer, which shows the layer's weight as its own."""
+
+    def __init__(self, base, rank=4):
+        super().__init__()
+        self.base = base
+        self.a = torch.nn.Parameter(torch.randn(rank, base.in_features).to(BF16) * 0.3)
+        self.b = torch.nn.Parameter(torch.randn(base.out_features, rank).to(BF16) * 0.3)
+        self.requires_grad_(False)
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return self.base(x) + x @ self.a.T @ self.b.T
+
+
+@pytest.mark.parametrize("part", ["gate_proj", "up_proj", "down_proj"])
+def test_adapters_around_the_parts_of_a_gated_mlp(stand_in, part):
+    torch.manual_seed(1)
+    m, own = installed(Mlp())
+    x = torch.randn(2, 3, 32).to(BF16)
+    plain = m(x)
+    adapter = Adapter(getattr(m, part))
+    theirs = copy.deepcopy(adapter)
+    theirs.base = getattr(own, part)
+    setattr(m, part, adapter)
+    setattr(own, part, theirs)
+    assert close(m(x), own(x)) and not close(m(x), plain)
+
+
+@pytest.mark.parametrize("part", ["gate_proj", "up_proj", "down_proj", "act_fn"])
+@pytest.mark.parametrize("kind", ["after", "before", "with kwargs"])
+def test_hooks_on_the_parts_run_and_see_what_they_always_saw(stand_in, part, kind):
+    torch.manual_seed(2)
+    m, own = installed(Mlp())
+    x = torch.randn(2, 3, 32).to(BF16)
+    m(x)
+
+    def hook_into(model):
+        seen = []
+
+        def after(mod, args, out):
+            seen.append((args[0].shape, out.shape))
+            return out * 2
+
+        def before(mod, args):
+            seen.append(args[0].shape)
+            return (args[0] + 1,)
+        child = getattr(model, part)
+        if kind == "after":
+            child.register_forward_hook(after)
+        elif kind == "before":
+            child.register_forward_pre_hook(before)
+        else:
+            child.register_forward_pre_hook(lambda mod, args, kwargs: (seen.append(args[0].shape), (args, kwargs))[1], with_kwargs=True)
+        return seen
+    mine, theirs = hook_into(m), hook_into(own)
+    assert close(m(x), own(x)) and mine == theirs and len(mine) == 1
+
+
+def test_hooks_on_every_module(stand_in):
+    m, own = installed(Mlp())
+    x = torch.randn(3, 32).to(BF16)
+    seen = []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda mod, args, out: seen.append(type(mod).__name__))
+    try:
+        m(x)
+        mine, seen[:] = list(seen), []
+        own(x)
+    finally:
+        handle.remove()
+    assert mine == seen and len(mine) == 5
+
+
+def test_parts_exchanged_afterwards(stand_in):
+    torch.manual_seed(3)
+    m, own = installed(Mlp())
+    x = torch.randn(3, 32).to(BF16)
+    for model in (m, own):
+        model.act_fn = torch.nn.GELU()
+    assert close(m(x), own(x))
+    for model in (m, own):
+        model.act_fn = torch.nn.SiLU()
+        model.gate_proj.forward = lambda v, g=model.gate_proj: torch.nn.functional.linear(v, g.weight) * 3
+    assert close(m(x), own(x))
+    m, own = installed(Mlp())
+    wide = torch.nn.Linear(32, 48, bias=False).to(BF16).requires_grad_(False)
+    m.up_proj, own.up_proj = wide.float(), wide.float()
+    for model in (m, own):
+        model.up_proj.register_forward_pre_hook(lambda mod, args: (args[0].float(),))
+        model.down_proj.register_forward_pre_hook(lambda mod, args: (args[0].to(BF16),))
+    assert close(m(x), own(x))
+
+
+def test_a_gated_mlp_takes_three_products(stand_in):
+    m, own = installed(Mlp())
+    x = torch.randn(2, 3, 32).to(BF16)
+    stand_in.calls = 0
+    assert close(m(x), own(x)) and stand_in.calls == 3
