@@ -16,8 +16,12 @@ worth to the model.
 from __future__ import annotations
 
 import copy
+import operator
+import types
+import weakref
 
 import torch
+import torch.fx
 
 from . import ops
 from .engine import ExpertCache
@@ -183,18 +187,87 @@ def _silu(m: torch.nn.Module) -> bool:
     return _untouched(m, (torch.nn.SiLU,) if kind.__name__ != "SiLUActivation" or not kind.__module__.startswith("transformers.") else (kind,))
 
 
+class _Whole(torch.fx.Tracer):
+    def is_leaf_module(self, m, qualified_name):
+        return True
+
+
+# Classes whose forward has been read, with that forward.
+_READ: "weakref.WeakKeyDictionary[type, types.FunctionType]" = weakref.WeakKeyDictionary()
+
+
+def _settings(m: torch.nn.Module):
+    """The numbers that m's forward takes from m besides its parts gate_proj, up_proj, down_proj and act_fn; None where it takes anything
+    else (or is wrapped), so that it is not known from m alone."""
+    forward = type(m).forward
+    code = getattr(forward, "__code__", None)
+    if (code is None or code.co_freevars or forward.__defaults__ or forward.__kwdefaults__ or type(m).__getattr__ is not torch.nn.Module.__getattr__
+            or any(isinstance(c, types.CodeType) for c in code.co_consts)):
+        return None
+    names = set(code.co_names) - {"gate_proj", "up_proj", "down_proj", "act_fn"}
+    if any(hasattr(type(m), n) or type(vars(m).get(n, m)) not in (int, float, bool) for n in names):
+        return None
+    return {n: vars(m)[n] for n in names}
+
+
+def _is_gated(m: torch.nn.Module) -> bool:
+    """Whether m's forward is down_proj(act_fn(gate_proj(x)) * up_proj(x)) and nothing else: it is traced, not tried."""
+    if _settings(m) is None:
+        return False
+    still = object.__new__(type(m))  # m in eval mode
+    still.__dict__.update(vars(m), training=False)
+    try:
+        nodes = list(_Whole().trace(still).nodes)
+    except Exception:  # noqa: BLE001 - a forward that looks at its input's values or sizes
+        return False
+    met = []
+
+    def is_times(n):
+        return n.op == "call_function" and n.target in (operator.mul, operator.imul, torch.mul) and len(n.args) == 2 and not n.kwargs
+
+    def behind(n):  # n without factors of 1
+        met.append(n)
+        if is_times(n) and any(type(a) in (int, float) and a == 1 for a in n.args):
+            return behind(next(a for a in n.args if isinstance(a, torch.fx.Node)))
+        return n
+
+    def part(n, name):  # the argument of this part's call
+        n = behind(n) if isinstance(n, torch.fx.Node) else None
+        return n.args[0] if n is not None and n.op == "call_module" and n.target == name and len(n.args) == 1 and not n.kwargs else None
+
+    x, out = nodes[0], nodes[-1]
+    met += [x, out]
+    product = part(out.args[0], "down_proj")
+    product = behind(product) if isinstance(product, torch.fx.Node) else None
+    if x.op != "placeholder" or product is None or not is_times(product):
+        return False
+    for a, b in (product.args, product.args[::-1]):
+        seen = len(met)
+        gate = part(part(a, "act_fn"), "gate_proj")
+        up = part(b, "up_proj")
+        if gate is x and up is x:
+            return set(met) == set(nodes)
+        del met[seen:]
+    return False
+
+
 class _GatedForward(_Forward):
     """Three products, SiLU in the first one's epilogue. gate_proj and act_fn are passed by, so only while there is nothing else to them
     (hooks, adapters around them, another activation); the other two are called as ever."""
 
     activation = "silu"
 
+    def __init__(self, m: torch.nn.Module):
+        super().__init__(m)
+        self.settings = _settings(m)
+
     def __call__(self, x):
         m = self.m
         gate_proj, act_fn = m._modules.get("gate_proj"), m._modules.get("act_fn")
         learns = torch.is_grad_enabled() and any(p.requires_grad for p in m.parameters())
         gate = None
-        if not (m.training or learns) and gate_proj is not None and act_fn is not None:
+        same = _READ.get(type(m)) is type(m).forward and all(vars(m).get(n) == v for n, v in self.settings.items())
+        if same and not (m.training or learns) and gate_proj is not None and act_fn is not None:
             if _untouched(gate_proj, (torch.nn.Linear,)) and _silu(act_fn):
                 gate = self.product.of(gate_proj, x)
         if gate is None:
@@ -225,15 +298,8 @@ def install_linears(model: torch.nn.Module) -> int:
         if (sorted(parts) != ["down_proj", "gate_proj", "up_proj"] or not all(mine(p) for p in parts.values())
                 or act is None or not _silu(act) or "forward" in vars(m)):
             continue
-        with torch.no_grad():  # whether its forward is what the names say
-            w = m.gate_proj.weight
-            x = torch.randn(2, w.shape[1], generator=torch.Generator(w.device).manual_seed(0), device=w.device).to(w.dtype)
-            modes = [(c, c.training) for c in m.modules()]
-            m.eval()
-            own, fused = type(m).forward(m, x), _GatedForward(m)(x)
-            for c, mode in modes:
-                c.training = mode
-        if own.shape == fused.shape and float((own - fused).float().norm()) <= 0.02 * float(own.float().norm()):
+        if _is_gated(m):
+            _READ[type(m)] = type(m).forward
             m.forward = _GatedForward(m)
             replaced += 1
     return replaced

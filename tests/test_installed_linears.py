@@ -182,3 +182,85 @@ def test_a_gated_mlp_takes_three_products(stand_in):
     x = torch.randn(2, 3, 32).to(BF16)
     stand_in.calls = 0
     assert close(m(x), own(x)) and stand_in.calls == 3
+
+
+def gated(forward, **attrs):
+    """An Mlp of another class, whose forward is given; whether it is taken for a gated MLP."""
+    m = type("Other", (Mlp,), {"forward": forward})()
+    for k, v in attrs.items():
+        setattr(m, k, v)
+    return hf_fused.install_linears(m.to(BF16)) == 4
+
+
+def test_what_is_taken_for_a_gated_mlp(stand_in):
+    torch.manual_seed(4)
+    assert gated(lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x)))
+    assert gated(lambda self, x: self.down_proj(self.up_proj(x) * self.act_fn(self.gate_proj(x))))
+    assert gated(lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x) * self.s) * self.up_proj(x)), s=1.0)
+
+    def by_steps(self, hidden):
+        g = self.act_fn(self.gate_proj(hidden))
+        y = self.down_proj(g * self.up_proj(hidden))
+        return y
+    assert gated(by_steps)
+    others = [
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)).clamp(max=50.0) * self.up_proj(x)), {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x).clamp(-7, 7)), {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) * (self.up_proj(x) + 1e-4)), {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x)) * 1.01, {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x * 1.01)) * self.up_proj(x)), {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.up_proj(x)) * self.gate_proj(x)), {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) * self.gate_proj(x)), {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x)) if x.shape[0] < 100 else x, {}),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x) * self.s) * self.up_proj(x)), dict(s=1.01)),
+        (lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x) * self.s[0]) * self.up_proj(x)), dict(s=[1.0])),
+        (lambda self, x: (self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x)),), {}),
+        (lambda self, x, more=None: self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x)), {}),
+        (lambda self, x: self.down_proj(torch.nn.functional.silu(self.gate_proj(x)) * self.up_proj(x)), {}),
+    ]
+    for i, (forward, attrs) in enumerate(others):
+        assert not gated(forward, **attrs), i
+
+
+def test_installed_classes_are_recognised(stand_in):
+    from transformers.models.deepseek_v3.configuration_deepseek_v3 import DeepseekV3Config
+    from transformers.models.deepseek_v3.modeling_deepseek_v3 import DeepseekV3MLP
+    from transformers.models.qwen2_moe.configuration_qwen2_moe import Qwen2MoeConfig
+    from transformers.models.qwen2_moe.modeling_qwen2_moe import Qwen2MoeMLP
+    for m in (DeepseekV3MLP(DeepseekV3Config(hidden_size=32, intermediate_size=48)),
+              Qwen2MoeMLP(Qwen2MoeConfig(hidden_size=32, intermediate_size=48), 48)):
+        m = m.to(BF16).eval().requires_grad_(False)
+        own = copy.deepcopy(m)
+        assert hf_fused.install_linears(m) == 4
+        x = torch.randn(2, 3, 32).to(BF16)
+        assert close(m(x), own(x))
+
+
+def test_a_number_or_a_forward_that_changes_afterwards(stand_in):
+    class Scaled(Mlp):
+        def __init__(self):
+            super().__init__()
+            self.scale = 1.0
+
+        def forward(self, x):
+            return self.down_proj(self.act_fn(self.gate_proj(x) * self.scale) * self.up_proj(x))
+    torch.manual_seed(5)
+    m, own = installed(Scaled())
+    x = torch.randn(3, 32).to(BF16)
+    assert close(m(x), own(x))
+    first = m(x)
+    m.scale = own.scale = 3.0
+    assert close(m(x), own(x)) and not close(m(x), first)
+    m.scale = own.scale = 1.0
+    Scaled.forward = lambda self, x: self.down_proj(self.act_fn(self.gate_proj(x)) + self.up_proj(x))
+    assert close(m(x), own(x)) and not close(m(x), first)
+
+
+def test_installation_changes_no_mode_and_no_generator(stand_in):
+    torch.manual_seed(6)
+    m = Mlp().to(BF16)
+    m.act_fn.eval()
+    state = torch.get_rng_state()
+    stand_in.calls = 0
+    assert hf_fused.install_linears(m) == 4 and stand_in.calls == 0
+    assert m.training and m.gate_proj.training and not m.act_fn.training and torch.equal(state, torch.get_rng_state())
