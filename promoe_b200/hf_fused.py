@@ -152,14 +152,14 @@ class _Forward:
 
     activation = None
 
-    def __init__(self, m: torch.nn.Module):
-        self.m, self.product = m, _Product(self.activation)
+    def __init__(self, m: torch.nn.Module, settings: dict | None = None):
+        self.m, self.settings, self.product = m, settings, _Product(self.activation)
 
     def __deepcopy__(self, memo):
-        return type(self)(copy.deepcopy(self.m, memo))
+        return type(self)(copy.deepcopy(self.m, memo), self.settings)
 
     def __reduce__(self):
-        return type(self), (self.m,)
+        return type(self), (self.m, self.settings)
 
 
 class _LinearForward(_Forward):
@@ -257,10 +257,6 @@ class _GatedForward(_Forward):
 
     activation = "silu"
 
-    def __init__(self, m: torch.nn.Module):
-        super().__init__(m)
-        self.settings = _settings(m)
-
     def __call__(self, x):
         m = self.m
         gate_proj, act_fn = m._modules.get("gate_proj"), m._modules.get("act_fn")
@@ -300,7 +296,7 @@ def install_linears(model: torch.nn.Module) -> int:
             continue
         if _is_gated(m):
             _READ[type(m)] = type(m).forward
-            m.forward = _GatedForward(m)
+            m.forward = _GatedForward(m, _settings(m))
             replaced += 1
     return replaced
 

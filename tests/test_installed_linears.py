@@ -249,6 +249,8 @@ def test_a_number_or_a_forward_that_changes_afterwards(stand_in):
     x = torch.randn(3, 32).to(BF16)
     assert close(m(x), own(x))
     first = m(x)
+    stand_in.calls = 0
+    assert torch.equal(copy.deepcopy(m)(x), first) and stand_in.calls == 3
     m.scale = own.scale = 3.0
     assert close(m(x), own(x)) and not close(m(x), first)
     m.scale = own.scale = 1.0
