@@ -22,6 +22,7 @@ import weakref
 
 import torch
 import torch.fx
+from torch.autograd import forward_ad
 
 from . import ops
 from .engine import ExpertCache
@@ -115,9 +116,22 @@ def _replace_forward(block, cache: ExpertCache, layer: int):
     block.forward = fused_forward
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_tracing, _transforms, _modes = torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
+
+
+def _watched() -> bool:
+    """Whether something has to see torch's own operations: a compiler or a tracer, a transform (vmap, jvp), a dispatch mode, forward-mode
+    differentiation."""
+    return (torch.compiler.is_compiling() or _tracing() is not None or _transforms() is not None or _modes() > 0
+            or forward_ad._current_level >= 0)
+
+
 def _usable(m) -> bool:
-    return (isinstance(m, torch.nn.Linear) and m.weight.is_cuda and m.weight.dtype in (torch.bfloat16, torch.float16)
-            and m.weight.dim() == 2 and (m.bias is None or m.bias.dtype == m.weight.dtype))
+    w, b = m.weight, m.bias
+    return (isinstance(m, torch.nn.Linear) and w.is_cuda and w.dtype in (torch.bfloat16, torch.float16) and w.dim() == 2 and w.numel() > 0
+            and w.stride(1) == 1 and w.stride(0) >= w.shape[1]
+            and (b is None or (b.dtype == w.dtype and b.shape == w.shape[:1] and b.is_contiguous() and b.device == w.device)))
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -133,11 +147,16 @@ class _Product:
         self.activation, self.key, self.made = activation, None, None
 
     def of(self, m: torch.nn.Linear, x: torch.Tensor):
-        """None where m's own forward has to do: other types or devices, or a gradient to record."""
+        """None where m's own forward has to do: other types, classes or devices, a gradient to record, somebody who watches."""
         w, b = m.weight, m.bias
         if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
             return None
-        if x.dtype != w.dtype or x.device != w.device:
+        if type(x) not in _PLAIN or type(w) not in _PLAIN or not (b is None or type(b) in _PLAIN) or _watched():
+            return None
+        if x.dtype != w.dtype or x.device != w.device or x.layout is not torch.strided or x.is_nested or x.shape[-1:] != w.shape[1:]:
+            return None
+        kind = w.device.type
+        if torch.is_autocast_enabled(kind) and torch.get_autocast_dtype(kind) != w.dtype:
             return None
         key = (w.data_ptr(), w.dtype, w.shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
         if self.key != key:

@@ -266,3 +266,97 @@ def test_installation_changes_no_mode_and_no_generator(stand_in):
     stand_in.calls = 0
     assert hf_fused.install_linears(m) == 4 and stand_in.calls == 0
     assert m.training and m.gate_proj.training and not m.act_fn.training and torch.equal(state, torch.get_rng_state())
+
+
+# ---- calls that torch's own machinery has to see ------------------------------------------------------------------
+@pytest.fixture(params=[lambda: torch.nn.Linear(32, 32), lambda: Mlp(32, 48)], ids=["linear", "mlp"])
+def pair(request, stand_in):
+    torch.manual_seed(7)
+    m, own = installed(request.param())
+    x = torch.randn(3, 32).to(BF16)
+    assert close(m(x), own(x)) and stand_in.calls > 0
+    return m, own, x
+
+
+def test_forward_mode_differentiation(pair):
+    import torch.autograd.forward_ad as fw
+    m, own, x = pair
+    t = torch.randn(3, 32).to(BF16)
+    with fw.dual_level():
+        got, want = (fw.unpack_dual(f(fw.make_dual(x, t))) for f in (m, own))
+        assert got.tangent is not None and close(got.tangent, want.tangent) and close(got.primal, want.primal)
+        with torch.no_grad():
+            assert close(fw.unpack_dual(m(x)).primal, own(x))
+    for a, b in zip(torch.func.jvp(m, (x,), (t,)), torch.func.jvp(own, (x,), (t,))):
+        assert close(a, b)
+
+
+def test_transforms(pair):
+    m, own, x = pair
+    many = torch.randn(4, 3, 32).to(BF16)
+    assert close(torch.func.vmap(m)(many), torch.func.vmap(own)(many))
+    stacked = {k: torch.stack([v, 2 * v]) for k, v in own.state_dict().items()}
+    got, want = (torch.func.vmap(lambda p, f=f: torch.func.functional_call(f, p, (x,)))(stacked) for f in (m, own))
+    assert close(got, want)
+    grad = [torch.func.grad(lambda v, f=f: f(v).float().square().sum())(x) for f in (m, own)]
+    assert close(*grad)
+
+
+def test_tracers_and_compilers(pair, stand_in):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    m, own, x = pair
+    other = torch.randn(3, 32).to(BF16)
+    for recorded in (torch.jit.trace(m, x, check_trace=False), make_fx(m)(x), torch.compile(m, backend="eager", fullgraph=True)):
+        recorded(x)
+        stand_in.calls = 0
+        assert close(recorded(other), own(other)) and stand_in.calls == 0
+
+
+def test_modes_that_count_operations(pair, stand_in):
+    from torch.utils.flop_counter import FlopCounterMode
+    m, own, x = pair
+    counts, stand_in.calls = [], 0
+    for f in (m, own):
+        with FlopCounterMode(display=False) as c:
+            f(x)
+        counts.append(c.get_total_flops())
+    assert counts[0] == counts[1] > 0 and stand_in.calls == 0
+
+
+class Marked(torch.Tensor):
+    """A tensor of another class, which says what it was in."""
+    seen = []
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        Marked.seen.append(getattr(func, "__name__", str(func)))
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+def test_tensors_of_other_classes(pair):
+    m, own, x = pair
+    Marked.seen.clear()
+    y = m(x.as_subclass(Marked))
+    assert type(y) is Marked and "linear" in Marked.seen and close(y.as_subclass(torch.Tensor), own(x))
+    layer = m if isinstance(m, torch.nn.Linear) else m.up_proj
+    layer.weight = torch.nn.Parameter(layer.weight.detach().as_subclass(Marked), requires_grad=False)
+    Marked.seen.clear()
+    assert close(m(x).as_subclass(torch.Tensor), own(x)) and "linear" in Marked.seen
+
+
+def test_autocast(pair, stand_in):
+    m, own, x = pair
+    stand_in.calls = 0
+    with torch.autocast("cpu", dtype=torch.float16):
+        assert m(x).dtype == own(x).dtype == torch.float16 and close(m(x), own(x))
+    assert stand_in.calls == 0
+    with torch.autocast("cpu", dtype=BF16):
+        assert m(x.float()).dtype == own(x.float()).dtype == BF16 and close(m(x), own(x))
+
+
+def test_inputs_that_do_not_fit_fail_as_ever(pair):
+    m, own, x = pair
+    for bad in (x[:, :-1], x.float(), torch.tensor(1.0, dtype=BF16)):
+        for f in (m, own):
+            with pytest.raises(RuntimeError):
+                f(bad)
