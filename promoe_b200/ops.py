@@ -4,7 +4,8 @@ and residual, and the log probabilities of given tokens.
 Thin wrappers over the C ABI (include/promoe_b200.h: pm_k_route, pm_k_linear, pm_k_token_logprobs): they check shapes and types,
 allocate results where the caller brings none and launch on torch's current stream of the tensors' device. They
 hold no state besides what a caller hands to their constructors, run without scratch memory and can be captured into a CUDA graph.
-No gradients: tensors that require one are refused while autograd records.
+No gradients: tensors that require one are refused while autograd records, and so are those with a forward-mode tangent and calls
+that torch.jit traces.
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ import ctypes as C
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -26,6 +28,7 @@ _DROPPED = {"out": 0, "zero": 16}
 # built without CUDA has neither; it has no CUDA tensors to call these operators with either.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
+_tracing = torch._C._get_tracing_state
 _I32, _F32 = torch.int32, torch.float32
 
 
@@ -54,7 +57,13 @@ def _matrix(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES
         raise ValueError(f"the rows of {what} must not overlap (expanded tensors: call contiguous())")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires a gradient: these operators have no backward pass")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} has a forward-mode tangent: these operators have no derivative")
     return index, rows, n, pitch
+
+
+def _refuse_tracing():
+    raise ValueError("torch.jit cannot trace these operators")
 
 
 class Router:
@@ -88,6 +97,8 @@ class Router:
 
     def __call__(self, logits: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None):
         """logits [T, num_expert] float32 / bf16 / fp16 -> (ids [T, top_k] int32, weights [T, top_k] float32)."""
+        if _tracing() is not None:
+            _refuse_tracing()
         index, T, _, pitch = _matrix(logits, "logits", self.num_expert)
         if self.device_index is not None and self.device_index != index:
             raise ValueError(f"logits must be on cuda:{self.device_index}, where the bias is")
@@ -149,6 +160,8 @@ class Linear:
         """x [M, K] of the weight's type, residual [M, N] of out_dtype (dense rows, any pitch) -> y [M, N]. out may be the
         residual itself; otherwise it must not overlap it, nor ever x, the weight or the bias."""
         index = self.device_index
+        if _tracing() is not None:
+            _refuse_tracing()
         if self._learns and torch.is_grad_enabled():
             raise ValueError("the weight or the bias requires a gradient: these operators have no backward pass")
         on, M, _, ld_x = _matrix(x, "x", self.K, self._x_dtypes)
@@ -180,6 +193,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, 
 
     logits [T, V] float32 / bf16 / fp16, targets [T] int64; a negative target names no token (logp 0). Masked logits (-inf)
     have probability 0; pm_k_token_logprobs states what rows without a distribution give. out: the four results to fill."""
+    if _tracing() is not None:
+        _refuse_tracing()
     index, T, V, pitch = _matrix(logits, "logits")
     if top_n < 0:
         raise ValueError("top_n must not be negative")
