@@ -62,6 +62,11 @@ def _matrix(t: torch.Tensor, what: str, width: int | None = None, dtypes=_DTYPES
     return index, rows, n, pitch
 
 
+def _fixed(name: str):
+    """An attribute that is set once: the launch arguments made from it would not follow."""
+    return property(lambda self: getattr(self, "_" + name))
+
+
 def _refuse_tracing():
     raise ValueError("torch.jit cannot trace these operators")
 
@@ -72,7 +77,10 @@ class Router:
     scoring: "softmax" or "sigmoid". bias: [num_expert] float32 on the device, added to the scores for the choice only (a
     load-balancing correction). n_group / topk_group / group_score ("max" or "top2"): choose among the best groups
     only; dropped: what becomes of the others' experts, "out" (they cannot be chosen) or, with a bias, "zero" (their score + bias
-    counts as 0, which passes by negative ones). norm_topk: weights divided by their sum. routed_scale: multiplies the weights."""
+    counts as 0, which passes by negative ones). norm_topk: weights divided by their sum. routed_scale: multiplies the weights.
+    The bias is used in place, not copied."""
+
+    num_expert, top_k, bias, device_index = (_fixed(n) for n in ("num_expert", "top_k", "bias", "device_index"))
 
     def __init__(self, num_expert: int, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None, n_group: int = 1,
                  topk_group: int = 1, group_score: str = "max", norm_topk: bool = False, routed_scale: float = 1.0,
@@ -86,8 +94,9 @@ class Router:
         if bias is not None:
             if not bias.is_cuda or bias.dtype != torch.float32 or bias.shape != (num_expert,) or not bias.is_contiguous():
                 raise ValueError("bias must be a contiguous float32 CUDA tensor of shape [num_expert]")
-        self.num_expert, self.top_k, self.bias = num_expert, top_k, bias
-        self.device_index = None if bias is None else bias.get_device()
+            bias = bias.detach()  # keeps the memory, whatever becomes of the caller's tensor
+        self._num_expert, self._top_k, self._bias = num_expert, top_k, bias
+        self._device_index = None if bias is None else bias.get_device()
         self.rule = _lib.pm_router(num_expert, top_k, _SCORING[scoring], n_group, topk_group, _GROUP_SCORE[group_score] + _DROPPED[dropped],
                                    int(norm_topk), routed_scale, None if bias is None else bias.data_ptr())
         self._ref = C.byref(self.rule)
@@ -99,10 +108,10 @@ class Router:
         """logits [T, num_expert] float32 / bf16 / fp16 -> (ids [T, top_k] int32, weights [T, top_k] float32)."""
         if _tracing() is not None:
             _refuse_tracing()
-        index, T, _, pitch = _matrix(logits, "logits", self.num_expert)
-        if self.device_index is not None and self.device_index != index:
-            raise ValueError(f"logits must be on cuda:{self.device_index}, where the bias is")
-        shape = (T, self.top_k)
+        index, T, _, pitch = _matrix(logits, "logits", self._num_expert)
+        if self._device_index is not None and self._device_index != index:
+            raise ValueError(f"logits must be on cuda:{self._device_index}, where the bias is")
+        shape = (T, self._top_k)
         if out is None:
             device = logits.device
             ids, w = torch.empty(shape, dtype=_I32, device=device), torch.empty(shape, dtype=_F32, device=device)
@@ -134,6 +143,8 @@ class Linear:
     weight [N, K] bf16 or fp16 with dense rows, bias [N] of the same type or float32, activation None / "relu" / "silu" /
     "gelu" / "gelu_tanh", out_dtype the weight's type (default) or float32. The tensors are used in place, not copied."""
 
+    weight, bias, out_dtype, device_index, N, K = (_fixed(n) for n in ("weight", "bias", "out_dtype", "device_index", "N", "K"))
+
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
                  out_dtype: torch.dtype | None = None):
         self._learns = weight.requires_grad or (bias is not None and bias.requires_grad)
@@ -150,29 +161,29 @@ class Linear:
                 raise ValueError(f"bias must be a contiguous tensor of shape [{N}], float32 or {weight.dtype}")
             if bias.get_device() != index:
                 raise ValueError(f"bias must be on cuda:{index}, not on {bias.device}")
-        self.weight, self.bias, self.out_dtype, self.device_index, self.N, self.K = weight, bias, out_dtype, index, N, K
+        self._weight, self._bias, self._out_dtype, self._device_index, self._N, self._K = weight, bias, out_dtype, index, N, K
         self._x_dtypes, self._y_dtypes = (weight.dtype,), (out_dtype,)
-        self._bias_ptr, self._ld_w = 0 if bias is None else bias.data_ptr(), pitch
+        self._ld_w = pitch
         self._kind = (N, K, _DTYPES[weight.dtype], _DTYPES[out_dtype], 0 if bias is None else _DTYPES[bias.dtype], _ACTS[activation], 0)
         self._fn = _lib.load().pm_k_linear
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [M, K] of the weight's type, residual [M, N] of out_dtype (dense rows, any pitch) -> y [M, N]. out may be the
         residual itself; otherwise it must not overlap it, nor ever x, the weight or the bias."""
-        index = self.device_index
+        index = self._device_index
         if _tracing() is not None:
             _refuse_tracing()
         if self._learns and torch.is_grad_enabled():
             raise ValueError("the weight or the bias requires a gradient: these operators have no backward pass")
-        on, M, _, ld_x = _matrix(x, "x", self.K, self._x_dtypes)
+        on, M, _, ld_x = _matrix(x, "x", self._K, self._x_dtypes)
         if out is None:
-            out = torch.empty((M, self.N), dtype=self.out_dtype, device=x.device)
-        on_y, rows, _, ld_y = _matrix(out, "out", self.N, self._y_dtypes)
+            out = torch.empty((M, self._N), dtype=self._out_dtype, device=x.device)
+        on_y, rows, _, ld_y = _matrix(out, "out", self._N, self._y_dtypes)
         if rows != M:
             raise ValueError(f"out must have {M} rows, not {rows}")
         res, ld_r = 0, 0
         if residual is not None:
-            on_r, rows, _, ld_r = _matrix(residual, "residual", self.N, self._y_dtypes)
+            on_r, rows, _, ld_r = _matrix(residual, "residual", self._N, self._y_dtypes)
             if rows != M:
                 raise ValueError(f"residual must have {M} rows, not {rows}")
             if on_r != index:
@@ -180,7 +191,7 @@ class Linear:
             res = residual.data_ptr()
         if on != index or on_y != index:
             raise ValueError(f"x and out must be on cuda:{index}, where the weight is")
-        a = _PM_LINEAR(x.data_ptr(), self.weight.data_ptr(), self._bias_ptr, res, out.data_ptr(), ld_x, self._ld_w, ld_r, ld_y, M, *self._kind)
+        a = _PM_LINEAR(x.data_ptr(), self._weight.data_ptr(), 0 if self._bias is None else self._bias.data_ptr(), res, out.data_ptr(), ld_x, self._ld_w, ld_r, ld_y, M, *self._kind)
         rc = self._fn(a, _raw_stream(index)) if index == _current_device() else _elsewhere(index, self._fn, a)
         if rc:
             _lib.check(rc)
