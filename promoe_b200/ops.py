@@ -91,6 +91,8 @@ class Router:
             raise ValueError(f"group_score must be one of {sorted(_GROUP_SCORE)}")
         if dropped not in _DROPPED:
             raise ValueError(f"dropped must be one of {sorted(_DROPPED)}")
+        if not all(-0x80000000 <= n <= 0x7fffffff for n in (num_expert, top_k, n_group, topk_group)):  # ctypes would cut them off
+            raise ValueError("num_expert, top_k, n_group and topk_group must be 32-bit numbers")
         if bias is not None:
             if not bias.is_cuda or bias.dtype != torch.float32 or bias.shape != (num_expert,) or not bias.is_contiguous():
                 raise ValueError("bias must be a contiguous float32 CUDA tensor of shape [num_expert]")

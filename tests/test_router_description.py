@@ -205,3 +205,11 @@ def test_dropped_groups_as_zero_need_a_correction_bias(lib):
     for value in (18, 32, 48, -16):
         with pytest.raises(_lib.PromoeError):
             route(group_score=value, n_group=4, topk_group=2, choice_bias=PTR)
+
+
+@pytest.mark.parametrize("kw", [dict(num_expert=2 ** 32 + 64), dict(top_k=2 ** 32 + 6), dict(n_group=2 ** 32 + 1), dict(n_group=8, topk_group=2 ** 32 + 2),
+                                dict(n_group=8, topk_group=2 - 2 ** 32)])
+def test_numbers_beyond_32_bits_are_refused(lib, kw):
+    from promoe_b200 import ops
+    with pytest.raises(ValueError):
+        ops.Router(**(dict(num_expert=64, top_k=6) | kw))
