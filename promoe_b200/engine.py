@@ -41,6 +41,7 @@ class ExpertCache:
         self._ctx = C.c_void_p()
         _lib.call("pm_ctx_create", C.byref(self._ctx), num_layer, num_expert, _config_text(config))
         self._keep: list = []          # device tensors whose addresses the context holds
+        self._device: int | None = None  # where they are
         self._hidden = 0
         self._n_params = 0
         self.pinned = False
@@ -244,6 +245,7 @@ class ExpertCache:
             if not t.is_cuda or t.dtype != dtype or not t.is_contiguous():
                 raise ValueError(f"layer weights must be contiguous CUDA tensors of {dtype}")
             self._keep.append(t)
+            self._device = t.get_device()
             return t.data_ptr()
         w = _lib.pm_layer_weights()
         w.gate_w = dev(gate_w, torch.bfloat16)
@@ -265,6 +267,8 @@ class ExpertCache:
         if router is None:
             _lib.call("pm_layer_set_router", self._ctx, layer, None)
             return
+        if router.device_index is not None and self._device not in (None, router.device_index):
+            raise ValueError(f"the router's bias must be on cuda:{self._device}, where the layer's weights are, not on cuda:{router.device_index}")
         _lib.call("pm_layer_set_router", self._ctx, layer, C.byref(router.rule))
         if router.bias is not None:
             self._keep.append(router.bias)

@@ -213,3 +213,13 @@ def test_numbers_beyond_32_bits_are_refused(lib, kw):
     from promoe_b200 import ops
     with pytest.raises(ValueError):
         ops.Router(**(dict(num_expert=64, top_k=6) | kw))
+
+
+def test_a_layer_refuses_a_router_of_another_device(lib):
+    import types
+    from promoe_b200.engine import ExpertCache
+    cache = ExpertCache(1, 16, num_expert_per_token=4)
+    cache._device = 0  # as its weights would leave it
+    with pytest.raises(ValueError, match="cuda:1"):
+        cache.set_router(0, types.SimpleNamespace(device_index=1, rule=None, bias=None))
+    cache.close()
