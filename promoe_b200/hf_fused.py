@@ -16,6 +16,7 @@ worth to the model.
 from __future__ import annotations
 
 import copy
+import inspect
 import operator
 import types
 import weakref
@@ -324,7 +325,8 @@ def install_linears(model: torch.nn.Module) -> int:
 def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, top_n: int = 0) -> dict:
     """What a causal LM thinks of a text: for every position but the last, the log probability of the token that follows, the
     entropy of the model's prediction there and its top_n favourites. input_ids [B, S] -> {"logp": [B, S - 1], "entropy": [B, S - 1],
-    "top_ids", "top_logp": [B, S - 1, top_n]}. Tokens outside attention_mask are not scored (logp 0). The vocabulary
+    "top_ids", "top_logp": [B, S - 1, top_n]}. Only tokens inside attention_mask [B, S] that follow one inside it are scored, the others' logp
+    is 0; positions count from a text's first token inside it, so that padding on either side changes nothing. The vocabulary
     projection (bf16 or fp16, on the GPU) runs with float32 logits, for as many positions at a time as 64 Mi logits hold,
     so a long text does not need all its logits at once. Models that cap or scale their logits afterwards are refused."""
     for name in ("final_logit_softcapping", "logit_scale", "logits_scaling", "lm_head_multiplier"):
@@ -332,13 +334,19 @@ def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask
             raise ValueError(f"this model changes its logits behind the vocabulary projection ({name})")
     head = model.get_output_embeddings()
     trunk = getattr(model, model.base_model_prefix)
-    hidden = trunk(input_ids=input_ids, attention_mask=attention_mask).last_hidden_state
+    given = {}
+    if attention_mask is not None:
+        if attention_mask.shape != input_ids.shape:
+            raise ValueError(f"attention_mask must have the shape of input_ids, {tuple(input_ids.shape)}")
+        if "position_ids" in inspect.signature(trunk.forward).parameters:
+            given["position_ids"] = (attention_mask.long().cumsum(-1) - 1).clamp_min(0)
+    hidden = trunk(input_ids=input_ids, attention_mask=attention_mask, **given).last_hidden_state
     lin = ops.Linear(head.weight, getattr(head, "bias", None), out_dtype=torch.float32)
     B, S = input_ids.shape
     x = hidden[:, :-1].reshape(B * (S - 1), hidden.shape[-1]).to(head.weight.dtype)
     targets = input_ids[:, 1:].to(torch.int64)
     if attention_mask is not None:
-        targets = targets.masked_fill(attention_mask[:, 1:] == 0, -100)
+        targets = targets.masked_fill((attention_mask[:, 1:] == 0) | (attention_mask[:, :-1] == 0), -100)
     targets = targets.reshape(-1)
     T = x.shape[0]
     new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=x.device)  # noqa: E731
