@@ -334,11 +334,12 @@ def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask
             raise ValueError(f"this model changes its logits behind the vocabulary projection ({name})")
     head = model.get_output_embeddings()
     trunk = getattr(model, model.base_model_prefix)
-    given = {}
+    takes = inspect.signature(trunk.forward).parameters
+    given = {"use_cache": False} if "use_cache" in takes else {}  # keys and values that nobody reads
     if attention_mask is not None:
         if attention_mask.shape != input_ids.shape:
             raise ValueError(f"attention_mask must have the shape of input_ids, {tuple(input_ids.shape)}")
-        if "position_ids" in inspect.signature(trunk.forward).parameters:
+        if "position_ids" in takes:
             given["position_ids"] = (attention_mask.long().cumsum(-1) - 1).clamp_min(0)
     hidden = trunk(input_ids=input_ids, attention_mask=attention_mask, **given).last_hidden_state
     lin = ops.Linear(head.weight, getattr(head, "bias", None), out_dtype=torch.float32)

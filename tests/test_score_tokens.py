@@ -73,3 +73,12 @@ def test_padding_changes_nothing(stand_ins, make, side):
         assert bool((got["logp"][b, outside] == 0).all())  # nothing is scored from or to a padding position
     with pytest.raises(ValueError):
         hf_fused.score_tokens(model, ids, mask[:, :-1])
+
+
+@pytest.mark.parametrize("make", [qwen, gpt2])
+def test_no_keys_and_values_are_kept(stand_ins, make):
+    model = make()
+    out = []
+    model.base_model.register_forward_hook(lambda m, args, kwargs, o: out.append((kwargs.get("use_cache"), o.past_key_values)), with_kwargs=True)
+    hf_fused.score_tokens(model, torch.arange(8)[None])
+    assert out and all(o == (False, None) for o in out)
