@@ -321,6 +321,20 @@ def install_linears(model: torch.nn.Module) -> int:
     return replaced
 
 
+def _compare_logits(lin, rows: torch.Tensor, own: torch.Tensor) -> None:
+    """Raises where a model's logits are not what its vocabulary projection makes of these hidden rows. Its own are rounded to the
+    projection's type, perhaps twice: a step of the value and of a usual one."""
+    mine = lin(rows)
+    if own.shape[-1] != mine.shape[-1] or own.numel() != mine.numel():
+        raise ValueError("this model's logits have another shape than its vocabulary projection gives them")
+    own = own.reshape(mine.shape).float()
+    usual = mine.square().mean(1, keepdim=True).sqrt()
+    off = (own - mine).abs() > torch.finfo(rows.dtype).eps * (mine.abs() + usual) + 1e-4 * usual
+    off |= own.isnan() != mine.isnan()
+    if bool((off & rows.isfinite().all(1, keepdim=True)).any()):
+        raise ValueError("this model changes its logits behind the vocabulary projection")
+
+
 @torch.no_grad()
 def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, top_n: int = 0) -> dict:
     """What a causal LM thinks of a text: for every position but the last, the log probability of the token that follows, the
@@ -328,7 +342,8 @@ def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask
     "top_ids", "top_logp": [B, S - 1, top_n]}. Only tokens inside attention_mask [B, S] that follow one inside it are scored, the others' logp
     is 0; positions count from a text's first token inside it, so that padding on either side changes nothing. The vocabulary
     projection (bf16 or fp16, on the GPU) runs with float32 logits, for as many positions at a time as 64 Mi logits hold,
-    so a long text does not need all its logits at once. Models that cap or scale their logits afterwards are refused."""
+    so a long text does not need all its logits at once. Models whose logits are something else than that projection (they cap or
+    scale them, or have an adapter there) are refused: some of them are compared with the model's own."""
     for name in ("final_logit_softcapping", "logit_scale", "logits_scaling", "lm_head_multiplier"):
         if getattr(model.config, name, None) not in (None, 1.0):
             raise ValueError(f"this model changes its logits behind the vocabulary projection ({name})")
@@ -341,9 +356,28 @@ def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask
             raise ValueError(f"attention_mask must have the shape of input_ids, {tuple(input_ids.shape)}")
         if "position_ids" in takes:
             given["position_ids"] = (attention_mask.long().cumsum(-1) - 1).clamp_min(0)
-    hidden = trunk(input_ids=input_ids, attention_mask=attention_mask, **given).last_hidden_state
-    lin = ops.Linear(head.weight, getattr(head, "bias", None), out_dtype=torch.float32)
     B, S = input_ids.shape
+    lin = ops.Linear(head.weight, getattr(head, "bias", None), out_dtype=torch.float32)
+    own_takes = inspect.signature(model.forward).parameters
+    seen = []  # what the trunk gives the model's own forward
+    handle = trunk.register_forward_hook(lambda m, args, out: seen.append(out.last_hidden_state if hasattr(out, "last_hidden_state") else out[0]))
+    try:
+        def logits_of(ids, **kw):
+            kw.update({k: v for k, v in (("use_cache", False), ("output_router_logits", False)) if k in own_takes})
+            own = model(input_ids=ids, **kw).logits
+            if len(seen) != 1:
+                raise ValueError(f"this model's forward does not take its hidden rows from {model.base_model_prefix!r} once")
+            return own, seen.pop()
+        if "logits_to_keep" in own_takes:  # one pass for both; the first and the last position, of which one lies inside the mask
+            at = torch.tensor(sorted({0, S - 1}), device=input_ids.device)
+            own, hidden = logits_of(input_ids, attention_mask=attention_mask, logits_to_keep=at, **{k: v for k, v in given.items() if k in own_takes})
+            rows = hidden[:, at]
+        else:
+            own, rows = logits_of(input_ids[:1, :4])
+            hidden = trunk(input_ids=input_ids, attention_mask=attention_mask, **given).last_hidden_state
+    finally:
+        handle.remove()
+    _compare_logits(lin, rows.reshape(-1, rows.shape[-1]).to(head.weight.dtype), own)
     x = hidden[:, :-1].reshape(B * (S - 1), hidden.shape[-1]).to(head.weight.dtype)
     targets = input_ids[:, 1:].to(torch.int64)
     if attention_mask is not None:

@@ -82,3 +82,73 @@ def test_no_keys_and_values_are_kept(stand_ins, make):
     model.base_model.register_forward_hook(lambda m, args, kwargs, o: out.append((kwargs.get("use_cache"), o.past_key_values)), with_kwargs=True)
     hf_fused.score_tokens(model, torch.arange(8)[None])
     assert out and all(o == (False, None) for o in out)
+
+
+def change(model, f):
+    """The model with f between its vocabulary projection and its logits."""
+    own = type(model).forward
+
+    class Changed(type(model)):
+        def forward(self, input_ids=None, attention_mask=None, position_ids=None, use_cache=None, logits_to_keep=0, **kw):
+            out = own(self, input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids, use_cache=use_cache,
+                      logits_to_keep=logits_to_keep, **kw)
+            out.logits = f(out.logits)
+            return out
+    model.__class__ = Changed
+    return model
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_models_that_change_their_logits_are_refused(stand_ins, dtype):
+    ids = torch.arange(10)[None]
+    mask = torch.ones_like(ids)
+    mask[:, :3] = 0
+    hf_fused.score_tokens(change(qwen().to(dtype), lambda l: l), ids, mask)
+    for f in (lambda l: l * 0.97, lambda l: l / 1.5, lambda l: 0.5 * torch.tanh(l / 0.5), lambda l: torch.log_softmax(l, -1), lambda l: l + 0.1,
+              lambda l: l[..., :-1], lambda l: l.masked_fill(torch.arange(97) > 90, -float("inf"))):
+        with pytest.raises(ValueError):
+            hf_fused.score_tokens(change(qwen().to(dtype), f), ids, mask)
+
+
+def test_an_adapter_on_the_vocabulary_projection_is_refused(stand_ins):
+    class Adapter(torch.nn.Module):
+        def __init__(self, base):
+            super().__init__()
+            self.base = base
+            self.a, self.b = torch.randn(2, 32), torch.randn(97, 2) * 0.1
+        weight, bias = property(lambda self: self.base.weight), None
+
+        def forward(self, x):
+            return self.base(x) + x @ self.a.T @ self.b.T
+    model = qwen()
+    model.lm_head = Adapter(model.lm_head)
+    with pytest.raises(ValueError):
+        hf_fused.score_tokens(model, torch.arange(8)[None])
+
+
+def test_a_model_that_gives_all_its_logits_or_has_another_trunk(stand_ins):
+    model, ids = qwen(), torch.randint(0, 97, (2, 9))
+    want = hf_fused.score_tokens(model, ids, top_n=2)
+    own = type(model).forward
+
+    class All(type(model)):
+        def forward(self, input_ids=None, attention_mask=None, use_cache=None):
+            out = own(self, input_ids=input_ids, attention_mask=attention_mask, use_cache=use_cache)
+            out.logits = out.logits * self.factor
+            return out
+    model.__class__, model.factor = All, 1.0
+    got = hf_fused.score_tokens(model, ids, top_n=2)
+    for k in want:
+        torch.testing.assert_close(got[k], want[k])
+    model.factor = 0.9
+    with pytest.raises(ValueError):
+        hf_fused.score_tokens(model, ids)
+
+    class Twice(type(model)):
+        def forward(self, input_ids=None, attention_mask=None, use_cache=None):
+            self.model(input_ids)
+            return own(self, input_ids=input_ids)
+    model.__class__ = Twice
+    with pytest.raises(ValueError):
+        hf_fused.score_tokens(model, ids)
+    assert not model.model._forward_hooks

@@ -29,3 +29,15 @@ def test_a_left_padded_text_scores_as_the_text_alone(lib):
         assert n == 1 or float((got["logp"][b, S - n:] - alone["logp"][0]).abs().max()) < 8 * 4 * 2.0 ** -8
         assert bool((got["logp"][b, :S - n] == 0).all())
     cache.close()
+
+
+def test_the_models_own_logits_are_compared(lib):
+    from promoe_b200.hf_fused import score_tokens
+    model, cache = injected()
+    ids = torch.randint(0, 128, (2, 9), device="cuda")
+    score_tokens(model, ids)
+    own = model.lm_head.forward
+    model.lm_head.forward = lambda x: own(x) * 0.95
+    with pytest.raises(ValueError):
+        score_tokens(model, ids)
+    cache.close()
