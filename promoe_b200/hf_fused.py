@@ -135,36 +135,59 @@ def _usable(m) -> bool:
             and (b is None or (b.dtype == w.dtype and b.shape == w.shape[:1] and b.is_contiguous() and b.device == w.device)))
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x as a matrix with dense rows, none over another."""
-    x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]) else x.contiguous()
+# Calls that the library's product is at least as fast for as torch's; others keep torch's. us in a CUDA graph with cold weights, bf16,
+# torch's and this one's: up to 16 tokens 2048 -> 512 5.3 and 2.5-3.0, 2048 -> 2048 5.5-8.4 and 3.0-3.5, 4096 -> 4096 9.7-13.7 and 6.5-7.5,
+# 3584 -> 4608 8.6-9.9 and 6.6-7.4, 2048 -> 9472 8.7-8.9 and 6.4-7.7; 17 tokens 5.3 and 5.4, 5.6 and 6.6, 9.8 and 10.9, 8.6 and 10.6; 512
+# tokens 5.5 and 7.7, 7.2 and 11.8, 14.8 and 19.6, 14.7 and 18.3. More results of few tokens: 2048 -> 11008 9.4-10.6 and 9.7-11.6, -> 40000
+# 26-30 and 32-33 (but -> 32000, at most 8 tokens, 25 and 22). Result rows off 16-byte boundaries slow torch's down at every number of
+# tokens: 2048 -> 2050 6.2 and 3.0 for one, 20 and 7.4 for 64, 62 and 17 for 2048; 2048 -> 100003 97 and 65, 409 and 70. Rows of
+# tokens or weights off them slow this one's down more from 17 on: 2050 -> 4096 21 and 27 for 64, 135 and 283 for 2048.
+_FEW, _NARROW = 16, 9472
+
+
+def _most(w: torch.Tensor) -> float:
+    """The number of input values up to which a call takes the library's product with these weights."""
+    N, K = w.shape
+    if N % 8 and K % 8 == 0 and w.stride(0) % 8 == 0 and w.data_ptr() % 16 == 0:
+        return float("inf")
+    return _FEW * K if N % 8 or N <= _NARROW else 0
 
 
 class _Product:
     """The library's product with a module's weights as they are now, kept while they stay where they are."""
 
     def __init__(self, activation: str | None = None):
-        self.activation, self.key, self.made = activation, None, None
+        self.activation, self.key, self.made, self.most = activation, None, None, float("inf")
 
-    def of(self, m: torch.nn.Linear, x: torch.Tensor):
-        """None where m's own forward has to do: other types, classes or devices, a gradient to record, somebody who watches."""
-        w, b = m.weight, m.bias
-        if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+    def of(self, m: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor | None:
+        """x times m's weights; None where m's own forward has to do: it is faster, other types, kinds of tensors, devices or shapes, a
+        gradient to record, operations that something has to see."""
+        if _tracing() is not None or (n := x.numel()) > self.most:
             return None
+        p = m._parameters
+        w, b = p.get("weight"), p.get("bias")
         if type(x) not in _PLAIN or type(w) not in _PLAIN or not (b is None or type(b) in _PLAIN) or _watched():
             return None
-        if x.dtype != w.dtype or x.device != w.device or x.layout is not torch.strided or x.is_nested or x.shape[-1:] != w.shape[1:]:
+        if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
             return None
-        kind = w.device.type
-        if torch.is_autocast_enabled(kind) and torch.get_autocast_dtype(kind) != w.dtype:
+        device, dtype, shape = w.device, w.dtype, w.shape
+        if x.dtype is not dtype or x.device != device or x.layout is not torch.strided or x.is_nested or x.shape[-1:] != shape[1:]:
             return None
-        key = (w.data_ptr(), w.dtype, w.shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
+        kind = device.type
+        if torch.is_autocast_enabled(kind) and torch.get_autocast_dtype(kind) is not dtype:
+            return None
+        key = (w.data_ptr(), dtype, shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
         if self.key != key:
             if not _usable(m):
                 return None
             self.key, self.made = key, ops.Linear(w.detach(), None if b is None else b.detach(), self.activation)
-        return self.made
+            self.most = _most(w)
+            if n > self.most:
+                return None
+        rows = n // shape[1]
+        if rows > 1 << 30 or (rows > _FEW and x.data_ptr() % 16):
+            return None
+        return self.made._dense(x if x.is_contiguous() else x.contiguous(), rows)
 
 
 class _Forward:
@@ -184,10 +207,8 @@ class _Forward:
 
 class _LinearForward(_Forward):
     def __call__(self, input):  # noqa: A002 - torch.nn.Linear's own name for it
-        lin = self.product.of(self.m, input)
-        if lin is None:
-            return type(self.m).forward(self.m, input)
-        return lin(_rows(input)).view(*input.shape[:-1], lin.N)
+        y = self.product.of(self.m, input)
+        return type(self.m).forward(self.m, input) if y is None else y
 
 
 _HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
@@ -281,24 +302,26 @@ class _GatedForward(_Forward):
         m = self.m
         gate_proj, act_fn = m._modules.get("gate_proj"), m._modules.get("act_fn")
         learns = torch.is_grad_enabled() and any(p.requires_grad for p in m.parameters())
-        gate = None
+        y = None
         same = _READ.get(type(m)) is type(m).forward and all(vars(m).get(n) == v for n, v in self.settings.items())
         if same and not (m.training or learns) and gate_proj is not None and act_fn is not None:
             if _untouched(gate_proj, (torch.nn.Linear,)) and _silu(act_fn):
-                gate = self.product.of(gate_proj, x)
-        if gate is None:
+                y = self.product.of(gate_proj, x)
+        if y is None:
             return type(m).forward(m, x)
         up = m.up_proj(x)
-        y = gate(_rows(x)).view(*x.shape[:-1], gate.N)
         return m.down_proj(y.mul_(up) if up.dtype == y.dtype and up.shape == y.shape else y * up)
 
 
 def install_linears(model: torch.nn.Module) -> int:
-    """Replaces the forward of every torch.nn.Linear with bf16 or fp16 weights on a GPU by promoe_b200.ops.Linear (bias in the
-    product's epilogue), and of gated MLPs (`gate_proj`, `up_proj`, `down_proj` around a SiLU and nothing else: dense layers
-    between MoE blocks) by three such products, SiLU in the first one's epilogue. For inference, under torch.no_grad() or with
-    parameters that require no gradient: calls that a gradient is to be recorded for keep the module's own forward, a gated
-    MLP's also in training mode. Call it once the model is on its device. Weights are used in place; they may be changed or
+    """Gives every torch.nn.Linear with bf16 or fp16 weights on a GPU a forward that takes promoe_b200.ops.Linear (bias in the
+    product's epilogue) where that is faster: calls of at most 16 tokens (decoding), and any number of them where the rows of the
+    result do not start on 16-byte boundaries; prompts keep torch's product. Gated MLPs (`gate_proj`, `up_proj`, `down_proj` around a
+    SiLU and nothing else: dense layers between MoE blocks) get one with SiLU in the first product's epilogue. For inference, under
+    torch.no_grad() or with parameters that require no gradient: calls that a gradient is to be recorded for keep the module's own forward, as
+    do those that torch traces, compiles, transforms, casts or counts, and a gated MLP's in training mode or with hooks or adapters on
+    gate_proj or act_fn. A token's result may differ in its last bits with the number of tokens of the call, as with torch's.
+    Call it once the model is on its device. Weights are used in place; they may be changed or
     exchanged afterwards, and a copied model works on its own. Modules of other classes than torch.nn.Linear itself, or with a forward of
     their own (hooks of other libraries), stay as they are. MoE blocks that inject_hf_fused_model replaced do
     not call theirs any more. Returns the number of replaced modules."""

@@ -199,6 +199,17 @@ class Linear:
             _lib.check(rc)
         return out
 
+    def _dense(self, x: torch.Tensor, M: int) -> torch.Tensor:
+        """x [..., K] -> [..., N] for a caller that has looked: x is contiguous, of the weight's type and device, M rows."""
+        index = self._device_index
+        out = torch.empty((*x.shape[:-1], self._N), dtype=self._out_dtype, device=x.device)
+        a = _PM_LINEAR(x.data_ptr(), self._weight.data_ptr(), 0 if self._bias is None else self._bias.data_ptr(), 0, out.data_ptr(), self._K,
+                       self._ld_w, 0, self._N, M, *self._kind)
+        rc = self._fn(a, _raw_stream(index)) if index == _current_device() else _elsewhere(index, self._fn, a)
+        if rc:
+            _lib.check(rc)
+        return out
+
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_n: int = 0, out=None):
     """Log probability of targets[t] under softmax(logits[t]), the entropy of that distribution and its top_n best

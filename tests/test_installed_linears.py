@@ -18,9 +18,9 @@ class StandIn:
     def __init__(self, weight, bias=None, activation=None, out_dtype=None):
         self.weight, self.bias, self.act, (self.N, self.K) = weight.detach(), bias, activation, weight.shape
 
-    def __call__(self, x, residual=None, out=None):
+    def _dense(self, x, M):
         StandIn.calls += 1
-        assert x.dim() == 2 and x.stride(1) == 1 and not (torch.is_grad_enabled() and x.requires_grad)
+        assert x.is_contiguous() and x.numel() == M * self.K and not (torch.is_grad_enabled() and x.requires_grad)
         y = torch.nn.functional.linear(x.detach(), self.weight, self.bias)
         return torch.nn.functional.silu(y) if self.act == "silu" else y
 
@@ -360,3 +360,39 @@ def test_inputs_that_do_not_fit_fail_as_ever(pair):
         for f in (m, own):
             with pytest.raises(RuntimeError):
                 f(bad)
+
+
+# ---- which calls take the product ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("K,N", [(32, 48), (32, 9472), (32, 9480), (32, 9473), (32, 50), (36, 48), (36, 50), (33, 50), (1, 8), (1, 1)])
+def test_calls_that_torch_is_faster_for_keep_it(stand_in, K, N):
+    m, own = installed(torch.nn.Linear(K, N))
+    aligned, odd = K % 8 == 0, N % 8 != 0
+    m(torch.zeros(1, K, dtype=BF16))
+    for M in (1, 8, 16, 17, 64, 600):
+        for x in (torch.randn(M, K).to(BF16), torch.randn(1, M, K).to(BF16)):
+            stand_in.calls = 0
+            assert close(m(x), own(x))
+            assert stand_in.calls == ((odd or N <= 9472) if M <= 16 else (odd and aligned)), M
+
+
+def test_weights_exchanged_for_others_of_another_size(stand_in):
+    m, own = installed(torch.nn.Linear(32, 48))
+    x = torch.randn(16, 32).to(BF16)
+    m(x)
+    for shape in ((24, 64), (24, 16), (9480, 8), (9472, 8), (5, 64)):
+        for model in (m, own):
+            model.weight, model.bias = (torch.nn.Parameter(t, requires_grad=False) for t in (torch.ones(shape).to(BF16), torch.ones(shape[0]).to(BF16)))
+        for M in (1, 16, 40):
+            x = torch.randn(M, shape[1]).to(BF16)
+            assert close(m(x), own(x))
+    m.weight.data = m.weight.data[:4]  # the same memory, fewer rows
+    m.bias.data = m.bias.data[:4]
+    assert m(x).shape == (40, 4) and m(x[:2]).shape == (2, 4)
+
+
+def test_inputs_with_strides(stand_in):
+    m, own = installed(torch.nn.Linear(32, 50))
+    for x in (torch.randn(32, 9).to(BF16).t(), torch.randn(4, 64).to(BF16)[:, 1:33], torch.randn(1, 32).to(BF16).expand(7, 32),
+              torch.randn(2, 3, 40).to(BF16)[..., 8:], torch.randn(700, 32).to(BF16)[::2], torch.randn(0, 32).to(BF16), torch.randn(32).to(BF16)):
+        y = m(x)
+        assert y.shape == own(x).shape and close(y, own(x))
