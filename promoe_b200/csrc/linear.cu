@@ -78,38 +78,64 @@ __device__ __forceinline__ float load_bias(const void* bias, int type, int n) {
   return __half2float(static_cast<const __half*>(bias)[n]);
 }
 
-// Short code (the epilogue is unrolled over columns, and a launch of few tiles pays for every instruction it fetches): quick
-// divisions, and the error function's complement by formula 7.1.26 of Abramowitz and Stegun (1.5e-7).
-template <int ACT>
+// sigma(z) = (z > 0 ? 1 : e) / (1 + e), e = exp(-|z|): nothing overflows, and small values keep their digits. Results of 16 bits take the
+// quick exponential, off by 2 + 1.2 |z| steps of float32 (their own rounding is 2^-9 or 2^-12), float32 results the one that is
+// good to a step (512 x 3584 -> 4608 22.6 -> 23.7 us with SiLU, 8192 x 64 -> 8192 105 -> 134). The quick division is good to two steps between its bounds, and all denominators are (1 to 20). The code is short
+// on purpose: the epilogue is unrolled over columns, and a launch of few tiles pays for every instruction it fetches.
+template <bool QUICK> __device__ __forceinline__ float exponential(float v) { return QUICK ? __expf(v) : expf(v); }
+template <bool QUICK>
+__device__ __forceinline__ float times_sigmoid(float v, float z) {
+  const float e = exponential<QUICK>(-fabsf(z));
+  return v * __fdividef(z > 0.f ? 1.f : e, 1.f + e);
+}
+// The complement of the error function for x = |v| / sqrt 2, as exp(-v^2 / 2) t P(t), t = 1 / (1 + 0.375 x). P was fitted to
+// exp(x^2) erfc(x) / t over 0 <= x <= 9.4 (least largest relative error, 1.1e-8); in float32 the whole is off by 2^-21 of itself at most,
+// in the tail too, where 1 - erf has lost every digit. exp(-v^2 / 2) takes the rounding of v^2 along.
+template <bool QUICK>
+__device__ __forceinline__ float erfc_of(float v) {
+  const float t = __fdividef(1.f, fmaf(0.375f * 0.70710678f, fabsf(v), 1.f)), sq = v * v;
+  float p = 0.0616966151f;
+  p = fmaf(p, t, -0.288075387f);
+  p = fmaf(p, t, 0.433893770f);
+  p = fmaf(p, t, -0.231076419f);
+  p = fmaf(p, t, 0.274844110f);
+  p = fmaf(p, t, 0.121038958f);
+  p = fmaf(p, t, 0.205430418f);
+  p = fmaf(p, t, 0.210633501f);
+  p = fmaf(p, t, 0.211614415f);
+  float e = exponential<QUICK>(-0.5f * sq);
+  if (!QUICK) e = fmaf(e, -0.5f * fmaf(v, v, -sq), e);
+  return sq < 400.f ? p * t * e : 0.f;
+}
+template <int ACT, bool QUICK>
 __device__ __forceinline__ float activate(float v) {
   if (ACT == PM_ACT_RELU) return v < 0.f ? 0.f : v;  // NaN stays
-  if (ACT == PM_ACT_SILU) return __fdividef(v, 1.f + __expf(-v));
+  if (ACT == PM_ACT_SILU) return times_sigmoid<QUICK>(v, v);
   if (ACT == PM_ACT_GELU) {  // v/2 erfc(-v / sqrt 2)
-    const float x = fabsf(v) * 0.70710678f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = p * __expf(-x * x);  // erfc(x)
+    const float tail = erfc_of<QUICK>(v);
     return 0.5f * v * (v > 0.f ? 2.f - tail : tail);
   }
-  if (ACT == PM_ACT_GELU_TANH)  // 0.5 v (1 + tanh u) = v / (1 + exp(-2u))
-    return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
+  if (ACT == PM_ACT_GELU_TANH)  // v/2 (1 + tanh u) = v sigma(2 u)
+    return times_sigmoid<QUICK>(v, 1.5957691216057308f * (v + 0.044715f * v * v * v));
   return v;
 }
-template <int N>
+template <bool QUICK, int N>
 __device__ __forceinline__ void activate_all(float (&v)[N], int act) {
   auto all = [&](auto f) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = f(v[i]);
   };
   switch (act) {
-    case PM_ACT_RELU: return all(activate<PM_ACT_RELU>);
-    case PM_ACT_SILU: return all(activate<PM_ACT_SILU>);
-    case PM_ACT_GELU: return all(activate<PM_ACT_GELU>);
-    case PM_ACT_GELU_TANH: return all(activate<PM_ACT_GELU_TANH>);
+    case PM_ACT_RELU: return all(activate<PM_ACT_RELU, QUICK>);
+    case PM_ACT_SILU: return all(activate<PM_ACT_SILU, QUICK>);
+    case PM_ACT_GELU: return all(activate<PM_ACT_GELU, QUICK>);
+    case PM_ACT_GELU_TANH: return all(activate<PM_ACT_GELU_TANH, QUICK>);
   }
 }
+template <class OT>
 __device__ __forceinline__ float activate_one(float v, int act) {
   float a[1] = {v};
-  activate_all(a, act);
+  activate_all<sizeof(OT) == 2>(a, act);
   return a[0];
 }
 
@@ -142,7 +168,7 @@ __device__ __forceinline__ void finish(const LinearTc& a, float (&o)[C], const O
   const bool whole = __all_sync(0xffffffffu, left >= C);
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] += bias;
-  activate_all(o, a.act);
+  activate_all<sizeof(OT) == 2>(o, a.act);
   if (ADD) {
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] += to_float<OT>(r[c]);
@@ -610,7 +636,7 @@ linear_plain_kernel(const __grid_constant__ LinearCall a) {
         for (int h = 0; h < 2; ++h) {
           const int m = m0 + wm + 16 * i + (lane >> 2) + 8 * h;
           if (m >= a.M) continue;
-          float v = activate_one((kPromote ? sum[kPromote ? i : 0][kPromote ? j : 0] : acc[i][j])[2 * h + e] + b, a.act);
+          float v = activate_one<OT>((kPromote ? sum[kPromote ? i : 0][kPromote ? j : 0] : acc[i][j])[2 * h + e] + b, a.act);
           if (a.res != nullptr) v += to_float<OT>(static_cast<const OT*>(a.res)[(int64_t)m * a.ldr + n]);
           static_cast<OT*>(a.y)[(int64_t)m * a.ldy + n] = from_float<OT>(v);
         }
@@ -786,7 +812,7 @@ __global__ void __launch_bounds__(WARPS * 32, (ALIGNED ? 16 : 24) / WARPS) linea
     float v = 0.f;
 #pragma unroll
     for (int k = 0; k < WARPS; ++k) v += part[k][m][row];
-    v = activate_one(v + load_bias(a.bias, a.bias_type, n), a.act);
+    v = activate_one<OT>(v + load_bias(a.bias, a.bias_type, n), a.act);
     if (a.res != nullptr) v += to_float<OT>(static_cast<const OT*>(a.res)[(int64_t)m * a.ldr + n]);
     static_cast<OT*>(a.y)[(int64_t)m * a.ldy + n] = from_float<OT>(v);
   }
