@@ -80,8 +80,9 @@ __device__ __forceinline__ float load_bias(const void* bias, int type, int n) {
 
 // sigma(z) = (z > 0 ? 1 : e) / (1 + e), e = exp(-|z|): nothing overflows, and small values keep their digits. Results of 16 bits take the
 // quick exponential, off by 2 + 1.2 |z| steps of float32 (their own rounding is 2^-9 or 2^-12), float32 results the one that is
-// good to a step (512 x 3584 -> 4608 22.6 -> 23.7 us with SiLU, 8192 x 64 -> 8192 105 -> 134). The quick division is good to two steps between its bounds, and all denominators are (1 to 20). The code is short
-// on purpose: the epilogue is unrolled over columns, and a launch of few tiles pays for every instruction it fetches.
+// good to a step (512 x 3584 -> 4608 22.6 -> 23.7 us with SiLU, 8192 x 64 -> 8192 105 -> 134). The quick division is good to two steps
+// for such denominators (1 to 7). The code is short on purpose: the epilogue is unrolled over columns, and a launch of few tiles pays
+// for every instruction it fetches.
 template <bool QUICK> __device__ __forceinline__ float exponential(float v) { return QUICK ? __expf(v) : expf(v); }
 template <bool QUICK>
 __device__ __forceinline__ float times_sigmoid(float v, float z) {
@@ -1035,7 +1036,7 @@ int launch_linear(const LinearCall& a, cudaStream_t s) {
     LinearShape shape;
   };
   static thread_local Plan plans[16] = {};
-  Plan& plan = plans[(unsigned)(a.M * 31 + a.N * 7 + a.K) % 16];
+  Plan& plan = plans[((unsigned)a.M * 31u + (unsigned)a.N * 7u + (unsigned)a.K) % 16u];
   if (!(plan.key == key)) plan = Plan{key, choose_shape(a.M, a.N, a.K, promote, cap)};
   const LinearShape& c = plan.shape;
   LinearTc t{};
