@@ -287,6 +287,7 @@ int pm_k_linear(const pm_linear* a, void* stream) {
 int pm_k_token_logprobs(const void* logits, int dtype, int64_t ld_logits, int n_rows, int vocab, const int64_t* targets, int top_n,
                         float* logp, float* entropy, int32_t* top_ids, float* top_logp, void* stream) {
   if (n_rows < 0 || vocab <= 0) return fail(PM_ERR_INVALID, "token_logprobs: vocab must be positive, n_rows not negative");
+  if (vocab > 0x7fff0000) return fail(PM_ERR_INVALID, "token_logprobs: vocab is above 2^31 - 2^16");  // loops step beyond a row's end
   if (!is_dtype(dtype)) return fail(PM_ERR_INVALID, "token_logprobs: unknown logits type");
   if (ld_logits < vocab) return fail(PM_ERR_INVALID, "token_logprobs: ld_logits is smaller than vocab");
   if (top_n < 0 || top_n > 32 || top_n > vocab) return fail(PM_ERR_INVALID, "token_logprobs: top_n must be in [0, min(32, vocab)]");
