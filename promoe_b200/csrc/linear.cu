@@ -876,16 +876,16 @@ cudaError_t launch_few(const LinearCall& a, FewShape f, cudaStream_t s) {
 }
 
 template <class T, class OT>
-cudaError_t launch_plain_for(const LinearCall& a, cudaStream_t s) {
+cudaError_t launch_plain_for(const LinearCall& a, int sms, cudaStream_t s) {
   // narrow weight tiles where wide ones would leave SMs without any
-  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) < 148) return launch_plain_tiles<T, OT, 32, 64>(a, s);
+  if ((long long)((a.N + 127) / 128) * ((a.M + 63) / 64) < sms) return launch_plain_tiles<T, OT, 32, 64>(a, s);
   return launch_plain_tiles<T, OT, 64, 128>(a, s);
 }
 
 template <class T>
 cudaError_t launch_plain(const LinearCall& a, int sms, cudaStream_t s) {
   if (a.M <= 16) return a.out_type == PM_F32 ? launch_few_shifted<T, float>(a, sms, s) : launch_few_shifted<T, T>(a, sms, s);
-  return a.out_type == PM_F32 ? launch_plain_for<T, float>(a, s) : launch_plain_for<T, T>(a, s);
+  return a.out_type == PM_F32 ? launch_plain_for<T, float>(a, sms, s) : launch_plain_for<T, T>(a, sms, s);
 }
 
 // ---- launch plan ------------------------------------------------------------------------------------------
