@@ -154,7 +154,7 @@ def _most(w: torch.Tensor) -> float:
 
 
 class _Product:
-    """The library's product with a module's weights as they are now, kept while they stay where they are."""
+    """The library's product with a module's weights as they are now, remade where they have moved. It holds none of their memory."""
 
     def __init__(self, activation: str | None = None):
         self.activation, self.key, self.made, self.most = activation, None, None, float("inf")
@@ -180,14 +180,15 @@ class _Product:
         if self.key != key:
             if not _usable(m):
                 return None
-            self.key, self.made = key, ops.Linear(w.detach(), None if b is None else b.detach(), self.activation)
+            self.key = key
+            self.made = ops.Linear(w.detach(), None if b is None else b.detach(), self.activation)._without_memory()
             self.most = _most(w)
             if n > self.most:
                 return None
         rows = n // shape[1]
         if rows > 1 << 30 or (rows > _FEW and x.data_ptr() % 16):
             return None
-        return self.made._dense(x if x.is_contiguous() else x.contiguous(), rows)
+        return self.made._dense(x if x.is_contiguous() else x.contiguous(), rows, w, b)
 
 
 class _Forward:

@@ -199,11 +199,17 @@ class Linear:
             _lib.check(rc)
         return out
 
-    def _dense(self, x: torch.Tensor, M: int) -> torch.Tensor:
-        """x [..., K] -> [..., N] for a caller that has looked: x is contiguous, of the weight's type and device, M rows."""
+    def _without_memory(self) -> "Linear":
+        """For a caller that keeps the weight and the bias itself and says at each call (_dense) where they are."""
+        self._weight = self._bias = None
+        return self
+
+    def _dense(self, x: torch.Tensor, M: int, weight: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor:
+        """x [..., K] -> [..., N] for a caller that has looked: x is contiguous, of the weight's type and device, M rows; weight and bias
+        are laid out like those this product was made from."""
         index = self._device_index
         out = torch.empty((*x.shape[:-1], self._N), dtype=self._out_dtype, device=x.device)
-        a = _PM_LINEAR(x.data_ptr(), self._weight.data_ptr(), 0 if self._bias is None else self._bias.data_ptr(), 0, out.data_ptr(), self._K,
+        a = _PM_LINEAR(x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0, out.data_ptr(), self._K,
                        self._ld_w, 0, self._N, M, *self._kind)
         rc = self._fn(a, _raw_stream(index)) if index == _current_device() else _elsewhere(index, self._fn, a)
         if rc:

@@ -16,12 +16,16 @@ class StandIn:
     calls = 0
 
     def __init__(self, weight, bias=None, activation=None, out_dtype=None):
-        self.weight, self.bias, self.act, (self.N, self.K) = weight.detach(), bias, activation, weight.shape
+        self.like, self.act = (weight.shape, weight.stride(), None if bias is None else bias.shape), activation
 
-    def _dense(self, x, M):
+    def _without_memory(self):
+        return self
+
+    def _dense(self, x, M, weight, bias):
         StandIn.calls += 1
-        assert x.is_contiguous() and x.numel() == M * self.K and not (torch.is_grad_enabled() and x.requires_grad)
-        y = torch.nn.functional.linear(x.detach(), self.weight, self.bias)
+        assert self.like == (weight.shape, weight.stride(), None if bias is None else bias.shape)
+        assert x.is_contiguous() and x.numel() == M * weight.shape[1] and not (torch.is_grad_enabled() and x.requires_grad)
+        y = torch.nn.functional.linear(x.detach(), weight.detach(), bias)
         return torch.nn.functional.silu(y) if self.act == "silu" else y
 
 
