@@ -143,7 +143,8 @@ class Linear:
     """y = activation(x weight^T + bias) + residual in one kernel (pm_k_linear).
 
     weight [N, K] bf16 or fp16 with dense rows, bias [N] of the same type or float32, activation None / "relu" / "silu" /
-    "gelu" / "gelu_tanh", out_dtype the weight's type (default) or float32. The tensors are used in place, not copied."""
+    "gelu" / "gelu_tanh", out_dtype the weight's type (default) or float32. The tensors are used in place, not copied.
+    A row of y depends on no other row; its last bits depend on the number of rows, which the order of the sums follows."""
 
     weight, bias, out_dtype, device_index, N, K = (_fixed(n) for n in ("weight", "bias", "out_dtype", "device_index", "N", "K"))
 
