@@ -157,7 +157,7 @@ class _Product:
     """The library's product with a module's weights as they are now, remade where they have moved. It holds none of their memory."""
 
     def __init__(self, activation: str | None = None):
-        self.activation, self.key, self.made, self.most = activation, None, None, float("inf")
+        self.activation, self.have, self.most = activation, (None, None), float("inf")
 
     def of(self, m: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor | None:
         """x times m's weights; None where m's own forward has to do: it is faster, other types, kinds of tensors, devices or shapes, a
@@ -176,19 +176,19 @@ class _Product:
         kind = device.type
         if torch.is_autocast_enabled(kind) and torch.get_autocast_dtype(kind) is not dtype:
             return None
-        key = (w.data_ptr(), dtype, shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype))
-        if self.key != key:
+        key = (w.data_ptr(), dtype, shape, w.stride(), None if b is None else (b.data_ptr(), b.dtype, b.shape, b.stride()))
+        have, made = self.have  # in one step: other threads may be here too
+        if have != key:
             if not _usable(m):
                 return None
-            self.key = key
-            self.made = ops.Linear(w.detach(), None if b is None else b.detach(), self.activation)._without_memory()
-            self.most = _most(w)
+            made = ops.Linear(w.detach(), None if b is None else b.detach(), self.activation)._without_memory()
+            self.have, self.most = (key, made), _most(w)
             if n > self.most:
                 return None
         rows = n // shape[1]
         if rows > 1 << 30 or (rows > _FEW and x.data_ptr() % 16):
             return None
-        return self.made._dense(x if x.is_contiguous() else x.contiguous(), rows, w, b)
+        return made._dense(x if x.is_contiguous() else x.contiguous(), rows, w, b)
 
 
 class _Forward:

@@ -400,3 +400,21 @@ def test_inputs_with_strides(stand_in):
               torch.randn(2, 3, 40).to(BF16)[..., 8:], torch.randn(700, 32).to(BF16)[::2], torch.randn(0, 32).to(BF16), torch.randn(32).to(BF16)):
         y = m(x)
         assert y.shape == own(x).shape and close(y, own(x))
+
+
+def test_a_call_while_another_one_makes_the_product(stand_in, monkeypatch):
+    """As a second thread would come in between."""
+    m, own = installed(torch.nn.Linear(32, 48))
+    x, inside = torch.randn(3, 32).to(BF16), []
+
+    class Slow(StandIn):
+        def __init__(self, *args, **kw):
+            super().__init__(*args, **kw)
+            if len(inside) < 2:
+                inside.append(None)
+                inside[-1] = m(x)
+    monkeypatch.setattr(hf_fused.ops, "Linear", Slow)
+    assert close(m(x), own(x)) and all(close(y, own(x)) for y in inside) and len(inside) == 2
+    m.weight, own.weight = (torch.nn.Parameter(2 * own.weight.detach(), requires_grad=False) for _ in range(2))
+    inside.clear()
+    assert close(m(x), own(x)) and all(close(y, own(x)) for y in inside) and len(inside) == 2
