@@ -418,3 +418,24 @@ def test_a_call_while_another_one_makes_the_product(stand_in, monkeypatch):
     m.weight, own.weight = (torch.nn.Parameter(2 * own.weight.detach(), requires_grad=False) for _ in range(2))
     begun.clear()
     assert close(m(x), own(x)) and close(inside[1], own(x))
+
+
+def test_a_bias_cut_short_in_place(stand_in):
+    """The same address, fewer values: there is nothing to read behind them."""
+    m, own = installed(torch.nn.Linear(32, 48))
+    x = torch.randn(3, 32).to(BF16)
+    m(x)
+    for model in (m, own):
+        model.bias.data = model.bias.data[:40]
+        with pytest.raises(RuntimeError):
+            model(x)
+
+
+def test_an_up_projection_of_another_tensor_class(stand_in):
+    torch.manual_seed(8)
+    m, own = installed(Mlp())
+    x = torch.randn(3, 32).to(BF16)
+    m(x)
+    for model in (m, own):
+        model.up_proj.register_forward_hook(lambda mod, args, out: out.as_subclass(Marked))
+    assert type(m(x)) is type(own(x)) is Marked and close(m(x).as_subclass(torch.Tensor), own(x).as_subclass(torch.Tensor))
