@@ -449,7 +449,10 @@ __device__ __forceinline__ void route_token(const float (&l)[NPL], int npl, cons
   }
   const bool chosen = id >= 0 && rank < r.k;
   float w = 0.f;
-  if (chosen) w = sigmoid ? __fdividef(1.f, 1.f + expf(-v_id)) : __fdividef(expf(v_id - top), sum);
+  if (chosen) {
+    const float e = expf(sigmoid ? -fabsf(v_id) : v_id - top);  // at most 1: the quick division gives 0 for quotients by more than 2^126
+    w = __fdividef(sigmoid && v_id >= 0.f ? 1.f : e, sigmoid ? 1.f + e : sum);
+  }
   if (r.norm) {
     float all = w;
 #pragma unroll
