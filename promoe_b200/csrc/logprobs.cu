@@ -553,7 +553,8 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   __syncthreads();
 
   Sums t = sh.part;
-  bool again = !(t.m > fmaxf(V::kLow + kFar, -kPlain)) || t.m > kPlain;
+  // Also where the sums are not finite: a part of the row may have begun with maxima below -kPlain (or holds a NaN).
+  bool again = !(t.m > fmaxf(V::kLow + kFar, -kPlain)) || t.m > kPlain || !(t.s + fabsf(t.u) < CUDART_INF_F);
   // Neither NaN nor anything above -inf: no distribution, without a second look (33 x 50001 with one such row: 9.5 -> 6.0 us).
   if (again && n > 0 && sh.best[0] == 0 && t.m == V::kLow && t.s == t.s) {
     again = false;

@@ -74,3 +74,27 @@ def test_large_logits_a_few_steps_apart(lib, V, sign):
     for i in (0, 3):
         assert bool(((got[i].double() - want[i]).abs() <= tolerance(V, want[i].abs())).all()), i
     assert bool(((got[1].double() - want[1]).abs() <= 20 * tolerance(V, want[1].abs())).all())
+
+
+@pytest.mark.parametrize("V", [700, 5000, 131072])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [-1e9, -1e12, -1e17, -1e19, -3e38])
+def test_ordinary_logits_among_very_low_ones(lib, V, dtype, low):
+    """Threads that meet the low ones first, wherever the ordinary ones lie."""
+    g = gen(V)
+    logits = low * (1 + 0.01 * torch.rand(6, V, generator=g, device="cuda"))
+    logits[0, -1] = 1.0
+    logits[1, :V // 2] = randn(g, V // 2)
+    logits[2, V // 2:] = randn(g, V - V // 2)
+    logits[3, ::3] = -65504.0
+    logits[4, torch.randperm(V, generator=g, device="cuda")[:V // 50]] = randn(g, V // 50)
+    logits[5, 1] = -2.0
+    logits[5, V - 2] = 3.0
+    logits = logits.clamp(min=torch.finfo(dtype).min).to(dtype)
+    targets = torch.tensor([V - 1, 0, V - 1, 3, 0, 1], device="cuda")
+    got, want = ops.token_logprobs(logits, targets, 3), logprob_oracle(logits, targets, 3)
+    assert torch.equal(got[2], want[2])
+    for i in (0, 3):
+        ok = want[i] > -3e38
+        assert bool(((got[i].double() - want[i]).abs()[ok] <= tolerance(V, want[i].abs())[ok]).all()), i
+    assert bool(((got[1].double() - want[1]).abs() <= 20 * tolerance(V, want[1].abs())).all())
