@@ -101,14 +101,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // register of it. raise(): all values at least kLow, NaN kept. top(): the larger (NaN ignored). pair(i): values 2i, 2i + 1. first(): the
 // lowest value of a 64-bit word.
 constexpr float kFar = 300.f;
-// Maxima whose c is off by at most 4, half a step of 1e8 log2 e: its rounding stays among the exponents that the sums can hold.
-// (Of 1e10 it is off by up to 512; from about 1e33 on the sums' rescaling meets infinity.) Rows beyond are summed again.
+// Rows with a larger maximum are summed again. c is off by half a step, at most 4 between kLow and here, which the exponents of the sums
+// can hold; a maximum of 1e10 would be off by 512, one of 1e33 would take the sums' rescaling to infinity, and a thread that meets
+// values of -1e9 first (masks) before any ordinary one would make them infinite too, hence kLow.
 constexpr float kPlain = 1e8f;
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int kN = 4;
-  static constexpr float kLow = -0x1p64f;
-  static constexpr uint32_t kLowBits = 0xDF800000u;
+  static constexpr float kLow = -0x1p26f;
+  static constexpr uint32_t kLowBits = 0xCC800000u;
   static __device__ __forceinline__ uint32_t raise(uint32_t w) { return __float_as_uint(max_nan(__uint_as_float(w), kLow)); }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
@@ -121,8 +122,8 @@ template <> struct Vec<float> {
 };
 template <> struct Vec<__nv_bfloat16> {
   static constexpr int kN = 8;
-  static constexpr float kLow = -0x1p64f;
-  static constexpr uint32_t kLowBits = 0xDF80DF80u;
+  static constexpr float kLow = -0x1p26f;
+  static constexpr uint32_t kLowBits = 0xCC80CC80u;
   static __device__ __forceinline__ uint32_t raise(uint32_t w) {
     const uint32_t low = kLowBits;
     const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&low));
@@ -553,8 +554,7 @@ logprobs_kernel(const __grid_constant__ LogprobArgs a, int parts) {
   __syncthreads();
 
   Sums t = sh.part;
-  // Also where the sums are not finite: a part of the row may have begun with maxima below -kPlain (or holds a NaN).
-  bool again = !(t.m > fmaxf(V::kLow + kFar, -kPlain)) || t.m > kPlain || !(t.s + fabsf(t.u) < CUDART_INF_F);
+  bool again = !(t.m > V::kLow + kFar) || t.m > kPlain;
   // Neither NaN nor anything above -inf: no distribution, without a second look (33 x 50001 with one such row: 9.5 -> 6.0 us).
   if (again && n > 0 && sh.best[0] == 0 && t.m == V::kLow && t.s == t.s) {
     again = false;
