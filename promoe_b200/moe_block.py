@@ -168,7 +168,8 @@ def _weights_by_rule(logits: torch.Tensor, d: dict, bias: torch.Tensor | None) -
 def confirm_router(block: torch.nn.Module, d: dict, gate_w: torch.Tensor) -> None:
     """Compares the description with how a copy of the block routes. Blocks that renormalise their weights without an attribute
     that says so, or the other way round, are followed (d["norm_topk"]), and so are those that count the choices of dropped groups as 0
-    beside a correction bias (d["router"]["dropped"]); one that routes by another rule is refused (ValueError). Of a block that cannot be run like that, a gate that holds more than the description knows is refused."""
+    beside a correction bias (d["router"]["dropped"]); one that routes by another rule is refused (ValueError). Of a block that cannot
+    be run like that, a gate that holds more than the description knows is refused."""
     what = f"{type(block).__name__} chooses or weighs its experts in a way that this library does not know"
     seen = _observe(block, gate_w)
     if seen is not None:
