@@ -47,7 +47,7 @@ def describe_router(block: torch.nn.Module, config=None) -> dict | None:
     if groups["n_group"] == 1:
         groups["topk_group"] = 1
     bias = getattr(gate, "e_score_correction_bias", None)
-    method = getattr(gate, "topk_method", getattr(block, "topk_method", None))
+    method = attr("topk_method")
     scoring = attr("scoring_func") or ("softmax" if bias is None else "sigmoid")
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"the router scores by softmax or sigmoid; this block uses {scoring!r}")

@@ -50,6 +50,20 @@ def test_scores_are_what_the_block_says(where, method, scoring):
         assert got is None
 
 
+@pytest.mark.parametrize("where", ["gate", "block", "config", "given config"])
+def test_the_method_is_where_the_block_says(where):
+    said, kw, given = {"topk_method": "group_limited_greedy"}, dict(n_group=4, topk_group=2), None
+    if where == "gate":
+        kw["gate"] = said
+    elif where == "block":
+        kw.update(said)
+    elif where == "config":
+        kw["config"] = said
+    else:
+        given = types.SimpleNamespace(**said)
+    assert describe_router(block(**kw), given) == dict(scoring="softmax", group_score="max", n_group=4, topk_group=2)
+
+
 @pytest.mark.parametrize("scoring", [None, "softmax", "sigmoid"])
 def test_scores_beside_a_correction_bias(scoring):
     b = torch.randn(16)
