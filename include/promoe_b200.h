@@ -410,9 +410,10 @@ int pm_k_route(const pm_router* router, const void* logits, int dtype, int64_t l
 
 /* y = act(x w^T + bias) + residual. x [M, K] and w [N, K] are of `dtype` (PM_BF16 or PM_F16), y and the optional residual
  * [M, N] of `out_dtype` (PM_F32 or dtype), the optional bias [N] of bias_dtype (PM_F32 or dtype). Sums are float32, y is
- * rounded once. A row of y depends on no other row; its last bits depend on M, which the order of the sums follows. y may be the
- * residual itself (same address and pitch); otherwise it must not overlap it, nor ever the other inputs.
- * x and w whose rows start on 16-byte boundaries (address and pitch) go to the tcgen05 kernel or, 16 tokens and fewer, to one
+ * rounded once; float32 results are added up from sums of 512 products, 16-bit results are one sum, off by some 2^-24 of itself for
+ * every 16 products beside a rounding of 2^-9 or 2^-12. A row of y depends on no other row; its last bits depend on M, which the
+ * order of the sums follows. y may be the residual itself (same address and pitch); otherwise it must not overlap it, nor ever the
+ * other inputs. x and w whose rows start on 16-byte boundaries (address and pitch) go to the tcgen05 kernel or, 16 tokens and fewer, to one
  * that streams the weights; others to a slower one. The optional
  * err_flag (device int32) receives 1 if a bounded wait of the kernel gave up; the outputs concerned are then NaN. */
 #define PM_ACT_NONE 0

@@ -37,7 +37,9 @@ constexpr int kWBytes = 128 * 128;  // a CTA's 128 weight rows of a k step
 constexpr int kMaxStages = 12;
 constexpr int kSmemMost = 232448;
 // k of one accumulator of float32 outputs. The tensor cores cut their running sums off where float32 ends, which shrinks a sum by
-// about 2^-24 of itself per addition of 16 k: 2.1e-6 for K = 2048 in one accumulator, 4.7e-7 in four.
+// about 2^-24 of itself per addition of 16 k: 2.1e-6 for K = 2048 in one accumulator, 4.7e-7 in four. (16-bit results take one: their own
+// rounding is 2^-9 or 2^-12, which that reaches where K is half a million or 65536; the sums of 256 columns would not fit the
+// epilogue's registers.)
 constexpr int kPromoteK = 512;
 
 struct LinearTc {

@@ -10,7 +10,7 @@ into the fused device path. Supported blocks: Qwen2-MoE (shared expert with sigm
 Mixtral (renormalised top-k), DeepSeek-V2 with greedy or group-limited top-k (shared experts, routed scaling), and blocks
 whose gate ranks sigmoid scores with a correction bias.
 
-`install_linears` hands the model's other matrix products to the library too, `score_tokens` says what a text's tokens were
+`install_linears` hands the model's other matrix products to the library where it is faster, `score_tokens` says what a text's tokens were
 worth to the model.
 """
 from __future__ import annotations
@@ -392,10 +392,10 @@ def score_tokens(model: torch.nn.Module, input_ids: torch.Tensor, attention_mask
             if len(seen) != 1:
                 raise ValueError(f"this model's forward does not take its hidden rows from {model.base_model_prefix!r} once")
             return own, seen.pop()
-        if "logits_to_keep" in own_takes:  # one pass for both; the first and the last position, of which one lies inside the mask
-            at = torch.tensor(sorted({0, S - 1}), device=input_ids.device)
-            own, hidden = logits_of(input_ids, attention_mask=attention_mask, logits_to_keep=at, **{k: v for k, v in given.items() if k in own_takes})
-            rows = hidden[:, at]
+        if "logits_to_keep" in own_takes:  # one pass for both, the logits of the last two positions
+            last = min(2, S)
+            own, hidden = logits_of(input_ids, attention_mask=attention_mask, logits_to_keep=last, **{k: v for k, v in given.items() if k in own_takes})
+            rows = hidden[:, -last:]
         else:
             own, rows = logits_of(input_ids[:1, :4])
             hidden = trunk(input_ids=input_ids, attention_mask=attention_mask, **given).last_hidden_state

@@ -152,3 +152,21 @@ def test_a_model_that_gives_all_its_logits_or_has_another_trunk(stand_ins):
     with pytest.raises(ValueError):
         hf_fused.score_tokens(model, ids)
     assert not model.model._forward_hooks
+
+
+def test_a_model_that_counts_its_kept_logits(stand_ins):
+    """logits_to_keep as a number of last positions, as all models know it."""
+    model, ids = qwen(), torch.randint(0, 97, (2, 9))
+    want = hf_fused.score_tokens(model, ids)
+    own = type(model).forward
+
+    class Counts(type(model)):
+        def forward(self, input_ids=None, attention_mask=None, use_cache=None, logits_to_keep=0):
+            assert isinstance(logits_to_keep, int)
+            out = own(self, input_ids=input_ids, attention_mask=attention_mask, use_cache=use_cache)
+            out.logits = out.logits[:, -logits_to_keep:]
+            return out
+    model.__class__ = Counts
+    for k, v in hf_fused.score_tokens(model, ids).items():
+        torch.testing.assert_close(v, want[k])
+    assert hf_fused.score_tokens(model, ids[:, :1])["logp"].shape == (2, 0)
